@@ -17,6 +17,9 @@ import torch  # noqa: F401  (must be imported first: see module docstring)
 LIB_PATH = Path(os.environ.get("CGAN3D_LIB_PATH") or Path(__file__).resolve().parent / "libcgan3d.so")
 
 ACT_NONE, ACT_RELU, ACT_LRELU, ACT_TANH, ACT_NEG_DTANH = 0, 1, 2, 3, 4
+ACT_GELU, ACT_SILU = 5, 6  # the linear block only
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+DTYPES = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 WGRAD_ACCUMULATE, WGRAD_WS_CLEAN, WGRAD_DEFER_UNPACK, WGRAD_DEFER_REDUCE = 1, 2, 4, 8  # cgan3d_conv3d_wgrad_ex flags
 # device loss slots written by the loss kernels (include/cgan3d.h)
 L_D, L_WD, L_GP, L_G, L_SIM, L_HU, L_GFULL = range(7)
@@ -89,6 +92,26 @@ class Epilogue(C.Structure):
                 ("bn_ss", C.c_void_p), ("bn_mi", C.c_void_p), ("bn_act", C.c_int32), ("bn_slope", C.c_float),
                 ("x_bf16", C.c_void_p), ("bn_fold", C.c_int32), ("fuse", C.POINTER(BnFuse)),
                 ("out_bf16", C.c_int32), ("pre", C.POINTER(BnPre))]
+
+
+class LinearArgs(C.Structure):
+    """include/cgan3d.h cgan3d_linear_args: the linear block's operands, forward and backward."""
+    _fields_ = [("rows", C.c_int64), ("k", C.c_int32), ("n", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+                ("slope", C.c_float), ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("bias", C.c_void_p), ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("preact", C.c_void_p), ("dy", C.c_void_p), ("lddy", C.c_int64),
+                ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p), ("dbias", C.c_void_p)]
+
+
+class OrthoMat(C.Structure):
+    """include/cgan3d.h cgan3d_ortho_mat: one matrix of an orthogonalisation."""
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("ldg", C.c_int64), ("ldo", C.c_int64), ("rows", C.c_int32),
+                ("cols", C.c_int32)]
+
+
+class MuonSeg(C.Structure):
+    """include/cgan3d.h cgan3d_muon_seg: one segment of a parameter arena (rows 0: a vector)."""
+    _fields_ = [("offset", C.c_int64), ("rows", C.c_int64), ("cols", C.c_int64), ("lr_scale", C.c_float)]
 
 
 _P, _I32, _I64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
@@ -173,6 +196,14 @@ _SIGS = {
     "cgan3d_host_alloc": ([_I64, _P, _P], _I32),
     "cgan3d_host_free": ([_P], _I32),
     "cgan3d_wgrad_unpack_multi": ([_P, _I32, _I64, _P], _I32),
+    "cgan3d_linear_fwd_ws_bytes": ([_P], _I64),
+    "cgan3d_linear_fwd": ([_P, _P, _I64, _P], _I32),
+    "cgan3d_linear_bwd_ws_bytes": ([_P], _I64),
+    "cgan3d_linear_bwd": ([_P, _P, _I64, _P], _I32),
+    "cgan3d_orthogonalize_ws_bytes": ([_P, _I32, _I32], _I64),
+    "cgan3d_orthogonalize": ([_P, _I32, _I32, _I32, _P, _F, _P, _I64, _P], _I32),
+    "cgan3d_muon_ws_bytes": ([_P, _I32], _I64),
+    "cgan3d_muon_step": ([_P, _P, _P, _P, _P, _I32, _P, _I32, _P, _F, _P, _I64, _P], _I32),
     "cgan3d_ln_partial_doubles": ([_I32, _I64], _I64),
     "cgan3d_ln_reduce": ([_P, _P, _P], _I32),
     "cgan3d_ln_apply": ([_P, _P, _P], _I32),

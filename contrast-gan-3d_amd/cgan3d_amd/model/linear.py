@@ -1,0 +1,113 @@
+"""Linear block ``act(x W^T + b) + residual`` over channels-last rows, with its gradient.
+
+The pointwise counterpart of ``ConvBlock`` (blocks.py): a 1 x 1 x 1 convolution over NDHWC voxels is a
+matrix product of the voxels' rows with the weight, and bias, activation and the residual's addition ride
+on its epilogue (``ops.linear``).  Under autograd the backward pass is the hand-written one
+(``ops.linear_backward``): first order, all four gradients.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor, nn
+
+from .. import _lib as L
+from .. import ops
+
+
+def _act_code(mod: nn.Module):
+    if isinstance(mod, nn.ReLU):
+        return L.ACT_RELU, 0.0
+    if isinstance(mod, nn.LeakyReLU):
+        return L.ACT_LRELU, float(mod.negative_slope)
+    if isinstance(mod, nn.Tanh):
+        return L.ACT_TANH, 0.0
+    if isinstance(mod, nn.GELU) and mod.approximate == "none":
+        return L.ACT_GELU, 0.0
+    if isinstance(mod, nn.SiLU):
+        return L.ACT_SILU, 0.0
+    if isinstance(mod, nn.Identity):
+        return L.ACT_NONE, 0.0
+    raise NotImplementedError(f"activation {mod} has no HIP kernel")
+
+
+def _rows(t: Tensor, cols: int) -> Tensor:
+    """``t`` [..., cols] as a matrix with contiguous rows (a view wherever its strides allow one)."""
+    if t.dim() != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: Tensor | None = None,
+                 act: int = L.ACT_NONE, slope: float = 0.0) -> Tensor:
+    """``act(x weight^T + bias) + residual``: x [..., k], weight [n, k], bias [n], residual of the result's
+    shape [..., n]; all of one dtype (float32, bfloat16 or float16).  ``act``: an activation code
+    (``_lib.ACT_NONE``, ``ACT_RELU``, ``ACT_LRELU`` with ``slope``, ``ACT_TANH``, ``ACT_GELU``, ``ACT_SILU``).
+    Differentiable once.  A HIP graph that captures the backward pass must be the only autograd graph alive
+    on its leaves (torch's own rule: their gradient accumulators belong to the stream they were made on)."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"fused_linear: x {tuple(x.shape)} does not multiply weight {tuple(weight.shape)}")
+    if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
+        raise ValueError(f"fused_linear: residual {tuple(residual.shape)} is not of the result's shape "
+                         f"{(*x.shape[:-1], weight.shape[0])}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearFn.apply(x, weight, bias, residual, act, slope)
+    return _forward(x, weight, bias, residual, act, slope, None)
+
+
+def _forward(x, weight, bias, residual, act, slope, preact):
+    n, k = weight.shape
+    x2 = _rows(x.detach(), k)
+    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    ops.linear(x2, _rows(weight.detach(), k), y.view(x2.shape[0], n),
+               bias=bias.detach().contiguous() if bias is not None else None,
+               residual=_rows(residual.detach(), n) if residual is not None else None, act=act, slope=slope,
+               preact=preact)
+    return y
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, slope):
+        preact = None
+        if act != L.ACT_NONE and any(ctx.needs_input_grad[:3]):
+            preact = torch.empty((math.prod(x.shape[:-1]), weight.shape[0]), dtype=ops.linear_preact_dtype(x.dtype), device=x.device)
+        y = _forward(x, weight, bias, residual, act, slope, preact)
+        ctx.act, ctx.slope = act, slope
+        ctx.save_for_backward(x, weight, preact)
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        if torch.is_grad_enabled():
+            raise NotImplementedError("double backward through the HIP linear block is not implemented")
+        x, weight, preact = ctx.saved_tensors
+        n, k = weight.shape
+        nx, nw, nb, nr = ctx.needs_input_grad[:4]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if nx else None
+        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if nw else None
+        db = torch.empty(n, dtype=x.dtype, device=x.device) if nb else None
+        if nx or nw or nb:
+            x2 = _rows(x.detach(), k)
+            ops.linear_backward(_rows(grad_out, n), x2, _rows(weight.detach(), k),
+                                dx=dx.view(x2.shape) if nx else None, dw=dw, dbias=db, act=ctx.act, slope=ctx.slope,
+                                preact=preact)
+        return dx, dw, db, grad_out if nr else None, None, None
+
+
+class LinearBlock(nn.Module):
+    """``activation_fn(linear(x)) + residual`` on channels-last tensors [..., channels_in]: parameters in
+    ``nn.Linear``'s layout under ``linear``."""
+
+    def __init__(self, channels_in: int, channels_out: int, activation_fn: type = nn.ReLU, bias: bool = True, **kwargs):
+        super().__init__()
+        self.linear = nn.Linear(channels_in, channels_out, bias=bias)
+        self.activation_fn = activation_fn(**kwargs)
+        _act_code(self.activation_fn)  # refuse what has no kernel where the block is built
+
+    def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
+        act, slope = _act_code(self.activation_fn)
+        return fused_linear(x, self.linear.weight, self.linear.bias, residual, act, slope)

@@ -1437,3 +1437,215 @@ def patch_normalize(out: torch.Tensor, weight: torch.Tensor):
     _need(weight, out.numel(), "patch_normalize weight")
     _need(out, out.numel(), "patch_normalize out")
     check(_launch("cgan3d_patch_normalize", ptr(out), ptr(weight), out.numel()), "patch_normalize")
+
+
+# --- linear block and orthogonalised updates ----------------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # a s + b s^3 + c s^5 of one Newton-Schulz step
+
+
+def _matrix(t, rows, cols, what, dtype, device):
+    """Row stride of a [rows, cols] operand whose rows are contiguous (a padded or sliced row stride is
+    fine); anything else is refused."""
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: dtype {t.dtype} != {dtype}")
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, the other operands are on {device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise ValueError(f"{what}: shape {tuple(t.shape)} != {(rows, cols)}")
+    ld = t.stride(0) if rows > 1 else max(cols, 1)
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise ValueError(f"{what}: rows must be contiguous and apart (strides {t.stride()})")
+    return ld
+
+
+def _flat(t, n, what, dtype, device):
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, the other operands are on {device}")
+    _need(t, n, what, dtype=dtype)
+
+
+def _dt(t, what):
+    if t.dtype not in L.DTYPES:
+        raise TypeError(f"{what}: dtype {t.dtype} (float32, bfloat16 or float16)")
+    if not t.is_cuda and not DRY_RUN:
+        raise ValueError(f"{what}: operands must be on the GPU, got {t.device}")
+    return L.DTYPES[t.dtype]
+
+
+def _workspace(ws, need, what, device):
+    """The caller's workspace (uint8, at least ``need`` bytes), or one for this call."""
+    if need < 0:
+        raise ValueError(f"{what}: {L.load().cgan3d_get_last_error().decode()}")
+    if ws is None:
+        if need and recording():
+            raise ValueError(f"{what}: a recorded plan keeps its workspace's address: pass ws ({need} bytes)")
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != device:
+        raise ValueError(f"{what}: ws must be contiguous uint8 on {device}")
+    if ws.numel() < need:
+        raise ValueError(f"{what}: ws has {ws.numel()} bytes, the kernels use {need}")
+    return ws
+
+
+def _launch_on(device, name, *args):
+    """``_launch`` on ``device``'s current stream, whichever device is current."""
+    if DRY_RUN or device.index is None or device.index == torch.cuda.current_device():
+        return _launch(name, *args)
+    with torch.cuda.device(device):
+        return _launch(name, *args)
+
+
+LINEAR_ACTS = (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU, L.ACT_TANH, L.ACT_GELU, L.ACT_SILU)
+
+
+def linear_preact_dtype(dtype):
+    """dtype of the pre-activation kept for the backward pass (include/cgan3d.h cgan3d_linear_args)."""
+    return torch.float32 if dtype == torch.float32 else torch.float16
+
+
+def _linear_args(x, w, act, slope, what):
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"{what}: x and w must be matrices, got {tuple(x.shape)} and {tuple(w.shape)}")
+    if act not in LINEAR_ACTS:
+        raise ValueError(f"{what}: activation code {act} (none, relu, lrelu, tanh, gelu or silu)")
+    a = L.LinearArgs()
+    a.dtype = _dt(x, f"{what} x")
+    a.rows, a.k = x.shape
+    a.n = w.shape[0]
+    a.act, a.slope = act, slope
+    a.x, a.ldx = x.data_ptr(), _matrix(x, a.rows, a.k, f"{what} x", x.dtype, x.device)
+    a.w, a.ldw = w.data_ptr(), _matrix(w, a.n, a.k, f"{what} w", x.dtype, x.device)
+    return a
+
+
+def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
+    """``y = act(x w^T + bias) + residual`` (cgan3d_linear_fwd): x [rows, k], w [n, k], bias [n], residual
+    and y [rows, n], all of one dtype (f32, bf16 or f16), rows strided as they like.  ``preact`` [rows, n]
+    (``linear_preact_dtype``) receives x w^T + bias for ``linear_backward``.  y may be the residual."""
+    a = _linear_args(x, w, act, slope, "linear")
+    dev = x.device
+    a.y, a.ldy = y.data_ptr(), _matrix(y, a.rows, a.n, "linear y", x.dtype, dev)
+    if bias is not None:
+        _flat(bias, a.n, "linear bias", x.dtype, dev)
+        a.bias = bias.data_ptr()
+    if residual is not None:
+        a.residual, a.ldr = residual.data_ptr(), _matrix(residual, a.rows, a.n, "linear residual", x.dtype, dev)
+    if preact is not None:
+        _flat(preact, a.rows * a.n, "linear preact", linear_preact_dtype(x.dtype), dev)
+        a.preact = preact.data_ptr()
+    ref = ctypes.byref(a)
+    ws = _workspace(ws, int(L.load().cgan3d_linear_fwd_ws_bytes(ref)), "linear", dev)
+    check(_launch_on(dev, "cgan3d_linear_fwd", ref, ptr(ws), 0 if ws is None else ws.numel()), "linear")
+
+
+def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
+    """Gradients of ``linear`` (cgan3d_linear_bwd) into those of ``dx`` [rows, k], ``dw`` [n, k] and
+    ``dbias`` [n] that are given (overwritten); ``preact`` is the forward call's (not needed without an
+    activation).  The residual's gradient is dy itself."""
+    a = _linear_args(x, w, act, slope, "linear_backward")
+    dev = x.device
+    a.dy, a.lddy = dy.data_ptr(), _matrix(dy, a.rows, a.n, "linear_backward dy", x.dtype, dev)
+    if act != L.ACT_NONE:
+        if preact is None:
+            raise ValueError("linear_backward: the activation's gradient needs the forward call's preact")
+        _flat(preact, a.rows * a.n, "linear_backward preact", linear_preact_dtype(x.dtype), dev)
+        a.preact = preact.data_ptr()
+    if dx is not None:
+        a.dx, a.lddx = dx.data_ptr(), _matrix(dx, a.rows, a.k, "linear_backward dx", x.dtype, dev)
+    if dw is not None:
+        _matrix(dw, a.n, a.k, "linear_backward dw", x.dtype, dev)
+        _flat(dw, a.n * a.k, "linear_backward dw", x.dtype, dev)
+        a.dw = dw.data_ptr()
+    if dbias is not None:
+        _flat(dbias, a.n, "linear_backward dbias", x.dtype, dev)
+        a.dbias = dbias.data_ptr()
+    ref = ctypes.byref(a)
+    ws = _workspace(ws, int(L.load().cgan3d_linear_bwd_ws_bytes(ref)), "linear_backward", dev)
+    check(_launch_on(dev, "cgan3d_linear_bwd", ref, ptr(ws), 0 if ws is None else ws.numel()), "linear_backward")
+
+
+def _ns_args(steps, coefficients, eps, what):
+    co = tuple(float(c) for c in coefficients)
+    if len(co) != 3:
+        raise ValueError(f"{what}: three coefficients (a, b, c) needed, got {len(co)}")
+    return int(steps), (ctypes.c_float * 3)(*co), float(eps)
+
+
+def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, out=None, ws=None):
+    """Newton-Schulz orthogonalisation of each matrix of ``g`` [..., rows, cols] (cgan3d_orthogonalize):
+    every singular value of g / (|g| + eps) goes through ``steps`` passes of a s + b s^3 + c s^5.  The result
+    has g's dtype (f32, bf16 or f16); the iteration keeps f32 accuracy.  ``out``: a tensor of g's
+    shape (g itself, or one that does not overlap it)."""
+    if g.dim() < 2:
+        raise ValueError(f"orthogonalize: matrices needed, got shape {tuple(g.shape)}")
+    if g.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("orthogonalize has no gradient: call it under torch.no_grad() or on g.detach()")
+    dt, dev = _dt(g, "orthogonalize g"), g.device
+    rows, cols = g.shape[-2:]
+    src = g.detach()
+    src = (src if src.is_contiguous() else src.contiguous()).view(-1, rows, cols) if g.numel() else src
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=dev)
+    elif out.dtype != g.dtype or out.shape != g.shape or out.device != dev or not out.is_contiguous():
+        raise ValueError("orthogonalize: out must be contiguous and of g's shape, dtype and device")
+    elif out.data_ptr() != g.data_ptr() and _spans_meet(out, src):
+        raise ValueError("orthogonalize: out overlaps g")
+    steps, co, eps = _ns_args(steps, coefficients, eps, "orthogonalize")
+    n = src.shape[0] if g.numel() else 0
+    step, e = rows * cols * g.element_size(), (src.data_ptr(), out.data_ptr())
+    mats = (L.OrthoMat * max(n, 1))(*[L.OrthoMat(e[0] + i * step, e[1] + i * step, cols, cols, rows, cols)
+                                      for i in range(n)])
+    ws = _workspace(ws, int(L.load().cgan3d_orthogonalize_ws_bytes(mats, n, dt)), "orthogonalize", dev)
+    check(_launch_on(dev, "cgan3d_orthogonalize", mats, n, dt, steps, co, eps, ptr(ws), 0 if ws is None else ws.numel()),
+          "orthogonalize")
+    return out
+
+
+def _spans_meet(a, b):
+    """Whether two contiguous tensors share memory."""
+    if not a.numel() or not b.numel():
+        return False
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
+            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
+class MuonSegments:
+    """The segments of a parameter arena that one Muon step updates (cgan3d_muon_seg): ``matrices`` as
+    (offset, rows, cols, lr_scale), ``vectors`` as (offset, length).  Checked once: inside the arena, no two
+    of them overlapping."""
+
+    def __init__(self, numel: int, matrices, vectors):
+        mats = [(int(o), int(r), int(c), float(s)) for o, r, c, s in matrices]
+        vecs = [(int(o), 0, int(k), 1.0) for o, k in vectors]
+        if any(min(q[:3]) < 0 for q in mats + vecs):
+            raise ValueError("MuonSegments: negative offset or size")
+        # rows == 0 says "vector" to the kernels: an empty matrix is left out
+        segs, at = [q for q in mats if q[1] * q[2]] + vecs, 0
+        for o, r, c, _ in sorted(segs, key=lambda q: q[0]):
+            k = r * c if r else c
+            if o + k > numel:
+                raise ValueError(f"MuonSegments: segment at {o} of {k} values leaves the arena of {numel}")
+            if k and o < at:
+                raise ValueError(f"MuonSegments: the segment at {o} overlaps the one before it")
+            at = max(at, o + k)
+        self.numel, self.n = numel, len(segs)
+        self.c = (L.MuonSeg * max(self.n, 1))(*[L.MuonSeg(*q) for q in segs])
+
+    def ws_bytes(self) -> int:
+        return int(L.load().cgan3d_muon_ws_bytes(self.c, self.n))
+
+
+def muon_step(param, grad, momentum, exp_avg_sq, segs: MuonSegments, hyper, steps: int = 5,
+              coefficients=NS_COEFFICIENTS, eps: float = 1e-7, ws=None):
+    """One Muon update of a parameter arena (cgan3d_muon_step): momentum, its orthogonalisation and the
+    update of the matrices, Adam of the vectors, the step counter.  ``hyper`` (device, 10 floats): see
+    include/cgan3d.h."""
+    dev = param.device
+    _dt(param, "muon_step param")
+    for t, nm in ((param, "param"), (grad, "grad"), (momentum, "momentum"), (exp_avg_sq, "exp_avg_sq")):
+        _flat(t, segs.numel, f"muon_step {nm}", torch.float32, dev)
+    _flat(hyper, 10, "muon_step hyper", torch.float32, dev)
+    steps, co, eps = _ns_args(steps, coefficients, eps, "muon_step")
+    ws = _workspace(ws, segs.ws_bytes(), "muon_step", dev)
+    check(_launch_on(dev, "cgan3d_muon_step", ptr(param), ptr(grad), ptr(momentum), ptr(exp_avg_sq), segs.c, segs.n,
+                     ptr(hyper), steps, co, eps, ptr(ws), 0 if ws is None else ws.numel()), "muon_step")

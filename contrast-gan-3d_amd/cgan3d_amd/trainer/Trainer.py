@@ -29,7 +29,7 @@ from .. import _lib as L
 from .. import ops
 from ..engine import Arena, StepEngine, _planar_dims
 from ..model.loss import WassersteinLoss, ZNCCLoss
-from .optim import FusedAdam, adam_hyper_from_partial
+from .optim import optimizer_from_partial
 
 try:  # tqdm is what the reference uses for progress; optional here
     from tqdm.auto import trange
@@ -67,14 +67,13 @@ class Trainer:
         self.gp_w, self.weight_clip = gp_weight, weight_clip
 
         self.generator: nn.Module = generator_class().to(self.device)
-        g_h = adam_hyper_from_partial(generator_optim_class)
-        self.optimizer_G = FusedAdam(Arena(self.generator, self.device), **g_h)
+        self.optimizer_G = optimizer_from_partial(generator_optim_class, Arena(self.generator, self.device))
         self.lr_scheduler_G = generator_lr_scheduler_class(self.optimizer_G) if generator_lr_scheduler_class else None
 
         self.critic: nn.Module = critic_class().to(self.device)
-        d_h = adam_hyper_from_partial(critic_optim_class)
-        # weight clipping (Trainer.py:136-138) is applied by the critic's Adam kernel after the update
-        self.optimizer_D = FusedAdam(Arena(self.critic, self.device), **d_h, weight_clip=weight_clip)
+        # weight clipping (Trainer.py:136-138) is applied by the critic's optimiser kernel after the update
+        self.optimizer_D = optimizer_from_partial(critic_optim_class, Arena(self.critic, self.device),
+                                                  weight_clip=weight_clip)
         self.lr_scheduler_D = critic_lr_scheduler_class(self.optimizer_D) if critic_lr_scheduler_class else None
 
         self.loss_GAN = WassersteinLoss()

@@ -1,0 +1,250 @@
+// Matrix products C[I, J] = sum_t A(i, t) * B(j, t) of the linear block (linear.hip) and the
+// Newton-Schulz iteration (muon.hip): the tile kernel that takes any size, stride and alignment.
+//
+// Either operand is "t-contiguous" (element (i, t) at i * ld + t: a row-major matrix whose columns are
+// summed) or "t-strided" (element (i, t) at t * ld + i: its rows are summed), so the forward product,
+// both gradients and the products of the iteration are one template.
+#pragma once
+#include <hip/hip_fp16.h>
+
+#include "common.h"
+
+namespace cg {
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+typedef float f32x4_m __attribute__((ext_vector_type(4)));
+typedef f16_t f16x8_m __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8_m __attribute__((ext_vector_type(8)));
+
+template <typename T> struct MatT;
+template <> struct MatT<float> { static constexpr int VEC = 4, PAD = 4; };
+template <> struct MatT<f16_t> { static constexpr int VEC = 8, PAD = 8; };
+template <> struct MatT<bf16_t> { static constexpr int VEC = 8, PAD = 8; };
+
+template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+// one rounding to nearest even on the way out of the 32-bit accumulators
+template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
+
+// 16 x 16 x 32 (16-bit) or 8 x (16 x 16 x 4) (f32: element e of both 8-element fragments is one k of
+// the instruction; the sum over t does not mind the order) on fragments of 8 t-values per lane:
+// lane l holds row l % 16, t = (l / 16) * 8 .. + 7.  D: column (second operand's row) l % 16, rows
+// (first operand's) (l / 16) * 4 + r.
+__device__ __forceinline__ f32x4_m mfma_8(const bf16_t* a, const bf16_t* b, f32x4_m c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8_m*>(a),
+                                                 *reinterpret_cast<const bf16x8_m*>(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_m mfma_8(const f16_t* a, const f16_t* b, f32x4_m c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const f16x8_m*>(a),
+                                                *reinterpret_cast<const f16x8_m*>(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_m mfma_8(const float* a, const float* b, f32x4_m c) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x4_m x = *reinterpret_cast<const f32x4_m*>(a + 4 * h), y = *reinterpret_cast<const f32x4_m*>(b + 4 * h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+  }
+  return c;
+}
+
+// --- activations of the linear block (all in 32 bits) ---
+__device__ __forceinline__ float mat_act(float z, int act, float slope) {
+  switch (act) {
+    case CGAN3D_ACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);  // NaN stays NaN
+    case CGAN3D_ACT_LRELU: return z > 0.f ? z : slope * z;
+    case CGAN3D_ACT_TANH: return tanhf(z);
+    case CGAN3D_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case CGAN3D_ACT_SILU: return z / (1.f + expf(-z));
+  }
+  return z;
+}
+// derivative at the pre-activation z.  The smooth ones are constant to the last bit of an f32 beyond
+// |z| = 100, so z is clamped there: an infinite (or saturated, see mat_preact) z gives their limits,
+// not inf * 0
+__device__ __forceinline__ float mat_act_grad(float z, int act, float slope) {
+  if (act == CGAN3D_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (act == CGAN3D_ACT_LRELU) return z > 0.f ? 1.f : slope;
+  if (act == CGAN3D_ACT_NONE) return 1.f;
+  if (z == z) z = fminf(fmaxf(z, -100.f), 100.f);
+  if (act == CGAN3D_ACT_TANH) {
+    // 1 - tanh^2 = 4 e / (1 + e)^2, e = exp(-2 |z|): no cancellation where tanh is near 1
+    const float e = expf(-2.f * fabsf(z)), d = 1.f + e;
+    return 4.f * e / (d * d);
+  }
+  if (act == CGAN3D_ACT_GELU)
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  const float s = 1.f / (1.f + expf(-z));  // SiLU
+  return s * (1.f + z * (1.f - s));
+}
+
+// The pre-activation kept for the backward pass.  f32 tensors keep it as it is; 16-bit tensors keep
+// an f16 whatever their own type: eleven bits of z leave act'(z) exact to about the rounding of dz
+// itself, where eight would double that error; values beyond f16's range saturate (act' is constant
+// there) and a value that would round to zero keeps its sign in the smallest f16 (ReLU's derivative).
+__device__ __forceinline__ void mat_preact(float* p, float z) { *p = z; }
+__device__ __forceinline__ void mat_preact(f16_t* p, float z) {
+  if (z == z) z = fminf(fmaxf(z, -65504.f), 65504.f);
+  f16_t h = (f16_t)z;
+  if (z != 0.f && h == (f16_t)0.f) h = z > 0.f ? (f16_t)5.9604645e-8f : (f16_t)-5.9604645e-8f;
+  *p = h;
+}
+template <typename T> struct PreT { typedef f16_t type; };
+template <> struct PreT<float> { typedef float type; };
+
+// what happens to a product's element on its way out: v = alpha * acc + bias[j]; preact = v;
+// v = act(v) + beta * residual[i, j]
+struct MatEpi {
+  const void* bias;
+  const void* residual;
+  long long ldr;
+  void* preact;  // [I, J], PreT
+  void* out;
+  long long ldo;
+  float alpha, beta;
+  int act;
+  float slope;
+};
+
+struct MatArgs {
+  const void* a;
+  const void* b;
+  long long lda, ldb;
+  long long I, J, K;
+  long long tj;      // column tiles
+  long long kchunk;  // t-values per split (whole K: one split)
+  float* part;       // splits > 1: [split][I][J] partial sums
+  MatEpi e;
+};
+
+template <typename T>
+__device__ __forceinline__ void mat_store(const MatEpi& e, long long J, long long i, long long j, float acc) {
+  float v = e.alpha * acc;
+  if (e.bias) v += to_f(static_cast<const T*>(e.bias)[j]);
+  if (e.preact) mat_preact(static_cast<typename PreT<T>::type*>(e.preact) + i * J + j, v);
+  v = mat_act(v, e.act, e.slope);
+  if (e.residual) v += e.beta * to_f(static_cast<const T*>(e.residual)[i * e.ldr + j]);
+  static_cast<T*>(e.out)[i * e.ldo + j] = from_f<T>(v);
+}
+
+// One BM x BN tile, 4 waves as 2 x 2, BK t-values a step: global -> registers -> LDS (rows padded by
+// 16 bytes), the next step's loads in flight under this step's products.
+template <typename T, bool AT, bool BT, int BM, int BN>
+__global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
+  constexpr int BK = 32, V = MatT<T>::VEC, LD = BK + MatT<T>::PAD;
+  constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
+  constexpr int NA = BM * BK / V / 256, NB = BN * BK / V / 256;  // 16-byte chunks per thread
+  static_assert(NA >= 1 && NB >= 1 && BM * BK % (V * 256) == 0 && BN * BK % (V * 256) == 0, "whole chunks per thread");
+  __shared__ __align__(16) T la[BM * LD];
+  __shared__ __align__(16) T lb[BN * LD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long long ti = blockIdx.x / p.tj, tjj = blockIdx.x - ti * p.tj;
+  const long long i0 = ti * BM, j0 = tjj * BN;
+  const long long k0 = (long long)blockIdx.y * p.kchunk, k1 = std::min(p.K, k0 + p.kchunk);
+  const int wi = (wave >> 1) * WM, wj = (wave & 1) * WN;
+  f32x4_m acc[FN][FM] = {};
+  typedef T vecT __attribute__((ext_vector_type(V)));
+  vecT ra[NA], rb[NB];
+  // one chunk of V values along the operand's contiguous axis: `inner` counts along it up to `ni`,
+  // `outer` across it up to `no`; what is outside is zero
+  auto load = [&](const T* base, long long ld, long long outer, long long no, long long inner, long long ni) {
+    vecT v = {};
+    if (outer < no && inner < ni) {
+      const T* s = base + outer * ld + inner;
+      if (inner + V <= ni && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
+        v = *reinterpret_cast<const vecT*>(s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (inner + e < ni) v[e] = s[e];
+      }
+    }
+    return v;
+  };
+  const T* A = static_cast<const T*>(p.a);
+  const T* B = static_cast<const T*>(p.b);
+  auto fetch = [&](long long k) {
+#pragma unroll
+    for (int c = 0; c < NA; ++c) {
+      const int q = c * 256 + tid;
+      if constexpr (AT) ra[c] = load(A, p.lda, k + q / (BM / V), k1, i0 + (q % (BM / V)) * V, p.I);
+      else ra[c] = load(A, p.lda, i0 + q / (BK / V), p.I, k + (q % (BK / V)) * V, k1);
+    }
+#pragma unroll
+    for (int c = 0; c < NB; ++c) {
+      const int q = c * 256 + tid;
+      if constexpr (BT) rb[c] = load(B, p.ldb, k + q / (BN / V), k1, j0 + (q % (BN / V)) * V, p.J);
+      else rb[c] = load(B, p.ldb, j0 + q / (BK / V), p.J, k + (q % (BK / V)) * V, k1);
+    }
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int c = 0; c < NA; ++c) {
+      const int q = c * 256 + tid;
+      if constexpr (AT) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) la[((q % (BM / V)) * V + e) * LD + q / (BM / V)] = ra[c][e];
+      } else {
+        *reinterpret_cast<vecT*>(&la[q / (BK / V) * LD + (q % (BK / V)) * V]) = ra[c];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NB; ++c) {
+      const int q = c * 256 + tid;
+      if constexpr (BT) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) lb[((q % (BN / V)) * V + e) * LD + q / (BN / V)] = rb[c][e];
+      } else {
+        *reinterpret_cast<vecT*>(&lb[q / (BK / V) * LD + (q % (BK / V)) * V]) = rb[c];
+      }
+    }
+  };
+  if (k0 < k1) fetch(k0);
+  for (long long k = k0; k < k1; k += BK) {
+    __syncthreads();  // the previous step's reads are done
+    put();
+    __syncthreads();
+    if (k + BK < k1) fetch(k + BK);
+    const T* pa = &la[(wi + (lane & 15)) * LD + (lane >> 4) * 8];
+    const T* pb = &lb[(wj + (lane & 15)) * LD + (lane >> 4) * 8];
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+      for (int m = 0; m < FM; ++m) acc[n][m] = mfma_8(pb + n * 16 * LD, pa + m * 16 * LD, acc[n][m]);
+  }
+  // a lane holds four neighbouring columns j of one row i
+#pragma unroll
+  for (int m = 0; m < FM; ++m) {
+    const long long i = i0 + wi + m * 16 + (lane & 15);
+    if (i >= p.I) continue;
+#pragma unroll
+    for (int n = 0; n < FN; ++n) {
+      const long long j = j0 + wj + n * 16 + (lane >> 4) * 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (j + r >= p.J) break;
+        if (p.part) p.part[((long long)blockIdx.y * p.I + i) * p.J + j + r] = acc[n][m][r];
+        else mat_store<T>(p.e, p.J, i, j + r, acc[n][m][r]);
+      }
+    }
+  }
+}
+
+// the splits' partial sums, added in their order, and the epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void mat_join_kernel(MatArgs p, int splits) {
+  const long long total = p.I * p.J;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long long)gridDim.x * 256) {
+    float s = 0.f;
+    for (int z = 0; z < splits; ++z) s += p.part[z * total + q];
+    const long long i = q / p.J;
+    mat_store<T>(p.e, p.J, i, q - i * p.J, s);
+  }
+}
+
+// f32 product with its epilogue, splits and tiles chosen for the sizes (linear.hip); at / bt: that
+// operand is t-strided.  Workspace: mat_f32_ws_bytes.
+long long mat_f32_ws_bytes(long long I, long long J, long long K);
+void mat_f32(bool at, bool bt, const MatArgs& p, void* ws, hipStream_t st);
+
+}  // namespace cg

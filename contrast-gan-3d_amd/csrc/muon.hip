@@ -1,0 +1,374 @@
+// Orthogonalised updates: the Newton-Schulz iteration on a list of matrices, and the Muon optimiser's
+// step over a parameter arena.
+//
+//   X_0 = G / (|G|_F + eps)        (over the short side: a tall G is taken transposed)
+//   A = X X^T,  B = b A + c A A,  X <- a X + B X        `steps` times
+//
+// which applies the odd quintic a s + b s^3 + c s^5 to every singular value s and leaves the singular
+// vectors alone; with (3.4445, -4.7750, 2.0315) five steps bring all but the smallest close to 1.
+//
+// Muon (arena segments that are matrices):  m <- m + (1 - mu)(g - m),  u = g + mu (m - g) (Nesterov) or m,
+//   p <- p (1 - lr wd) - lr scale NS(u);   segments that are vectors: Adam with their own rate.
+//
+// The norm is summed in 64 bits (a gradient of 1e-25 squares to nothing in 32), everything else is f32.
+#include <climits>
+#include <cmath>
+
+#include "mat.h"
+
+namespace cg {
+namespace {
+
+constexpr int kNormBlocks = 64;  // partial sums per matrix
+constexpr int kList = 24;        // segments a launch takes by value
+
+// hyper (device): see include/cgan3d.h cgan3d_muon_step
+enum { H_LR, H_MU, H_WD, H_NESTEROV, H_STEP, H_CLIP, H_VLR, H_VB1, H_VB2, H_VEPS, H_COUNT };
+
+struct Mat {
+  const void* g;
+  void* out;  // orthogonalize: the result; muon: the parameter
+  long long ldg, ldo;
+  int rows, cols;
+  float scale;  // muon: factor of lr
+  float* x;     // iterate, [short][long]
+  double* part;
+};
+
+__device__ __forceinline__ double block_sum_d(double v) {
+  __shared__ double red[4];
+  v = wave_sum_d(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+struct MatList {
+  Mat m[kList];
+};
+struct SegList {
+  cgan3d_muon_seg s[kList];
+  long long u[kList];  // offset of the segment's update in the workspace
+  int mat[kList];      // index of the matrix (its partial sums), -1: a vector
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void norm_kernel(MatList l) {
+  const Mat& m = l.m[blockIdx.y];
+  const T* g = static_cast<const T*>(m.g);
+  const long long total = (long long)m.rows * m.cols;
+  double s = 0.;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += kNormBlocks * 256LL) {
+    const long long i = q / m.cols;
+    const double v = to_f(g[i * m.ldg + (q - i * m.cols)]);
+    s += v * v;
+  }
+  s = block_sum_d(s);
+  if (threadIdx.x == 0) m.part[blockIdx.x] = s;
+}
+
+// momentum and the update's squares (matrices), Adam (vectors)
+__global__ __launch_bounds__(256) void muon_moment_kernel(SegList l, float* __restrict__ param,
+                                                          const float* __restrict__ grad, float* __restrict__ mom,
+                                                          float* __restrict__ sq, const float* __restrict__ hyper,
+                                                          float* __restrict__ u, double* __restrict__ part) {
+  const cgan3d_muon_seg sg = l.s[blockIdx.y];
+  const long long total = sg.rows > 0 ? sg.rows * sg.cols : sg.cols, base = sg.offset;
+  if (sg.rows == 0) {
+    const float h[6] = {hyper[H_VLR], hyper[H_VB1], hyper[H_VB2], hyper[H_VEPS], 0.f, hyper[H_CLIP]};
+    const AdamK k = adam_k(h, hyper[H_STEP] + 1.f);
+    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += kNormBlocks * 256LL)
+      adam_elem(k, param, grad, mom, sq, base + q);
+    return;
+  }
+  const float mu = hyper[H_MU];
+  const bool nest = hyper[H_NESTEROV] != 0.f;
+  double s = 0.;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += kNormBlocks * 256LL) {
+    const float g = grad[base + q];
+    float m = mom[base + q];
+    m += (1.f - mu) * (g - m);
+    mom[base + q] = m;
+    const float v = nest ? g + mu * (m - g) : m;
+    u[l.u[blockIdx.y] + q] = v;
+    s += (double)v * v;
+  }
+  s = block_sum_d(s);
+  if (threadIdx.x == 0) part[(long long)l.mat[blockIdx.y] * kNormBlocks + blockIdx.x] = s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void scale_kernel(MatList l, float eps) {
+  const Mat& m = l.m[blockIdx.y];
+  double s = 0.;
+  for (int b = 0; b < kNormBlocks; ++b) s += m.part[b];
+  const float norm = (float)(sqrt(s) + (double)eps);
+  const T* g = static_cast<const T*>(m.g);
+  const bool tall = m.rows > m.cols;
+  const int lng = tall ? m.rows : m.cols;
+  const long long total = (long long)m.rows * m.cols;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256LL) {
+    const long long i = q / lng, t = q - i * lng;
+    m.x[q] = to_f(tall ? g[t * m.ldg + i] : g[i * m.ldg + t]) / norm;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void ortho_out_kernel(MatList l) {
+  const Mat& m = l.m[blockIdx.y];
+  const bool tall = m.rows > m.cols;
+  const long long total = (long long)m.rows * m.cols;
+  T* o = static_cast<T*>(m.out);
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256LL) {
+    const long long i = q / m.cols, j = q - i * m.cols;
+    o[i * m.ldo + j] = from_f<T>(tall ? m.x[j * m.rows + i] : m.x[q]);
+  }
+}
+
+__global__ __launch_bounds__(256) void muon_apply_kernel(MatList l, const float* __restrict__ hyper) {
+  const Mat& m = l.m[blockIdx.y];
+  const bool tall = m.rows > m.cols;
+  const long long total = (long long)m.rows * m.cols;
+  float* p = static_cast<float*>(m.out);
+  const float lr = hyper[H_LR], keep = 1.f - lr * hyper[H_WD], rate = lr * m.scale, clip = hyper[H_CLIP];
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256LL) {
+    const long long i = q / m.cols, j = q - i * m.cols;
+    float v = p[q] * keep - rate * (tall ? m.x[j * m.rows + i] : m.x[q]);
+    if (clip > 0.f) v = fminf(fmaxf(v, -clip), clip);
+    p[q] = v;
+  }
+}
+
+__global__ void muon_tick_kernel(float* hyper) { hyper[H_STEP] += 1.f; }
+
+long long up256(long long v) { return (v + 255) / 256 * 256; }
+
+struct Layout {
+  long long part, u, x, x2, a, b, mat, total;
+};
+// The matrices run one after the other, so the iterates and products share one region sized for the largest;
+// every matrix has its own partial sums and (muon) its own update.
+void size_mat(Layout& w, long long rows, long long cols) {
+  const long long s = std::min(rows, cols), l = std::max(rows, cols);
+  w.x = std::max(w.x, up256(s * l * 4));
+  w.a = std::max(w.a, up256(s * s * 4));
+  w.mat = std::max({w.mat, mat_f32_ws_bytes(s, s, l), mat_f32_ws_bytes(s, s, s), mat_f32_ws_bytes(s, l, s)});
+}
+void place(Layout& w, long long nmat, long long ubytes) {
+  const long long x = w.x, a = w.a, m = w.mat;
+  w.part = 0;
+  w.u = up256(nmat * kNormBlocks * 8);
+  w.x = w.u + up256(ubytes);
+  w.x2 = w.x + x;
+  w.a = w.x2 + x;
+  w.b = w.a + a;
+  w.mat = w.b + a;
+  w.total = w.mat + m;
+}
+
+// `steps` iterations on m.x; returns where the result is
+float* iterate(const Mat& m, const Layout& w, char* ws, int steps, const float* co, hipStream_t st) {
+  const long long s = std::min(m.rows, m.cols), l = std::max(m.rows, m.cols);
+  float* x = m.x;
+  float* y = reinterpret_cast<float*>(ws + w.x2);
+  float* A = reinterpret_cast<float*>(ws + w.a);
+  float* B = reinterpret_cast<float*>(ws + w.b);
+  for (int k = 0; k < steps; ++k) {
+    MatArgs p = {};
+    p.a = p.b = x; p.lda = p.ldb = l;
+    p.I = p.J = s; p.K = l;
+    p.e.out = A; p.e.ldo = s; p.e.alpha = 1.f;
+    mat_f32(false, false, p, ws + w.mat, st);
+    p.a = p.b = A; p.lda = p.ldb = s;  // A is symmetric: A A = A A^T
+    p.K = s;
+    p.e.out = B; p.e.alpha = co[2];
+    p.e.residual = A; p.e.ldr = s; p.e.beta = co[1];
+    mat_f32(false, false, p, ws + w.mat, st);
+    p.a = B; p.b = x; p.ldb = l;
+    p.J = l;
+    p.e.out = y; p.e.ldo = l; p.e.alpha = 1.f;
+    p.e.residual = x; p.e.ldr = l; p.e.beta = co[0];
+    mat_f32(false, true, p, ws + w.mat, st);
+    std::swap(x, y);
+  }
+  return x;
+}
+
+const char* ns_check(int steps, const float* co, float eps) {
+  if (steps < 0 || steps > 64) return "steps must be 0..64";
+  if (!co || !std::isfinite(co[0]) || !std::isfinite(co[1]) || !std::isfinite(co[2])) return "three finite coefficients needed";
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return "eps must be finite and not negative";
+  return nullptr;
+}
+
+const char* mats_check(const cgan3d_ortho_mat* m, int n, int dt) {
+  if (n < 0 || (n > 0 && !m)) return "null list";
+  if (dt < CGAN3D_DT_F32 || dt > CGAN3D_DT_F16) return "unknown dtype";
+  for (int i = 0; i < n; ++i) {
+    if (m[i].rows < 0 || m[i].cols < 0) return "negative size";
+    if ((long long)m[i].rows * m[i].cols == 0) continue;
+    if (!m[i].g || !m[i].out) return "null matrix";
+    if (m[i].ldg < m[i].cols || m[i].ldo < m[i].cols) return "row stride smaller than the row";
+    const long long t = (std::max(m[i].rows, m[i].cols) + 63LL) / 64, u = (std::min(m[i].rows, m[i].cols) + 63LL) / 64;
+    if (t * u > INT_MAX) return "matrix too large for one launch";
+  }
+  return nullptr;
+}
+
+Layout ortho_layout(const cgan3d_ortho_mat* m, int n) {
+  Layout w = {};
+  for (int i = 0; i < n; ++i) size_mat(w, m[i].rows, m[i].cols);
+  place(w, n, 0);
+  return w;
+}
+
+template <typename T>
+void ortho_run(const cgan3d_ortho_mat* mats, int n, const Layout& w, char* ws, int steps, const float* co, float eps,
+               hipStream_t st) {
+  for (int i = 0; i < n; ++i) {
+    const cgan3d_ortho_mat& q = mats[i];
+    const long long total = (long long)q.rows * q.cols;
+    if (!total) continue;
+    MatList l;
+    l.m[0] = {q.g, q.out, q.ldg, q.ldo, q.rows, q.cols, 1.f, reinterpret_cast<float*>(ws + w.x),
+              reinterpret_cast<double*>(ws + w.part) + (long long)i * kNormBlocks};
+    const unsigned blocks = (unsigned)std::min((total + 1023) / 1024, 4096LL);
+    launch(norm_kernel<T>, dim3(kNormBlocks, 1), dim3(256), 0, st, l);
+    launch(scale_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l, eps);
+    l.m[0].x = iterate(l.m[0], w, ws, steps, co, st);
+    launch(ortho_out_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l);
+  }
+}
+
+const char* segs_check(const cgan3d_muon_seg* s, int n) {
+  if (n < 0 || (n > 0 && !s)) return "null list";
+  for (int i = 0; i < n; ++i) {
+    if (s[i].offset < 0 || s[i].rows < 0 || s[i].cols < 0 || s[i].rows > INT_MAX) return "negative or too large size";
+    if (s[i].rows > 0 && s[i].cols > INT_MAX) return "negative or too large size";
+    if (s[i].rows > 0) {
+      const long long t = (std::max(s[i].rows, s[i].cols) + 63) / 64, u = (std::min(s[i].rows, s[i].cols) + 63) / 64;
+      if (t * u > INT_MAX) return "matrix too large for one launch";
+    }
+  }
+  return nullptr;
+}
+
+Layout muon_layout(const cgan3d_muon_seg* s, int n) {
+  Layout w = {};
+  long long nm = 0, u = 0;
+  for (int i = 0; i < n; ++i)
+    if (s[i].rows > 0) {
+      size_mat(w, s[i].rows, s[i].cols);
+      u += up256(s[i].rows * s[i].cols * 4);
+      ++nm;
+    }
+  place(w, nm, u);
+  return w;
+}
+
+}  // namespace
+}  // namespace cg
+
+using namespace cg;
+
+extern "C" int64_t cgan3d_orthogonalize_ws_bytes(const cgan3d_ortho_mat* mats, int32_t n, int32_t dtype) {
+  if (const char* e = mats_check(mats, n, dtype)) {
+    set_error("cgan3d_orthogonalize_ws_bytes: %s", e);
+    return -1;
+  }
+  return ortho_layout(mats, n).total;
+}
+
+extern "C" int cgan3d_orthogonalize(const cgan3d_ortho_mat* mats, int32_t n, int32_t dtype, int32_t steps,
+                                    const float* coefficients, float eps, void* ws, int64_t ws_bytes,
+                                    void* stream) try {
+  const char* e = mats_check(mats, n, dtype);
+  CG_CHECK_ARG(!e, "cgan3d_orthogonalize: %s", e);
+  e = ns_check(steps, coefficients, eps);
+  CG_CHECK_ARG(!e, "cgan3d_orthogonalize: %s", e);
+  const Layout w = ortho_layout(mats, n);
+  CG_CHECK_ARG(ws_bytes >= w.total && (w.total == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
+               "cgan3d_orthogonalize: workspace of %lld bytes (16-byte aligned) needed, got %lld", w.total,
+               (long long)ws_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  char* base = static_cast<char*>(ws);
+  if (dtype == CGAN3D_DT_F32) ortho_run<float>(mats, n, w, base, steps, coefficients, eps, st);
+  else if (dtype == CGAN3D_DT_BF16) ortho_run<bf16_t>(mats, n, w, base, steps, coefficients, eps, st);
+  else ortho_run<f16_t>(mats, n, w, base, steps, coefficients, eps, st);
+  CG_LAUNCH_CHECK("cgan3d_orthogonalize");
+  return CGAN3D_OK;
+} catch (...) {
+  set_error("cgan3d_orthogonalize: out of host memory");
+  return CGAN3D_EHIP;
+}
+
+extern "C" int64_t cgan3d_muon_ws_bytes(const cgan3d_muon_seg* segs, int32_t n) {
+  if (const char* e = segs_check(segs, n)) {
+    set_error("cgan3d_muon_ws_bytes: %s", e);
+    return -1;
+  }
+  return muon_layout(segs, n).total;
+}
+
+extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum, float* exp_avg_sq,
+                                const cgan3d_muon_seg* segs, int32_t n, float* hyper, int32_t steps,
+                                const float* coefficients, float eps, void* ws, int64_t ws_bytes, void* stream) try {
+  const char* e = segs_check(segs, n);
+  CG_CHECK_ARG(!e, "cgan3d_muon_step: %s", e);
+  e = ns_check(steps, coefficients, eps);
+  CG_CHECK_ARG(!e, "cgan3d_muon_step: %s", e);
+  CG_CHECK_ARG(param && grad && momentum && exp_avg_sq && hyper, "cgan3d_muon_step: null operand");
+  const Layout w = muon_layout(segs, n);
+  CG_CHECK_ARG(ws_bytes >= w.total && (w.total == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
+               "cgan3d_muon_step: workspace of %lld bytes (16-byte aligned) needed, got %lld", w.total,
+               (long long)ws_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  char* base = static_cast<char*>(ws);
+  float* u = reinterpret_cast<float*>(base + w.u);
+  double* part = reinterpret_cast<double*>(base + w.part);
+  long long uo = 0;
+  int nm = 0, at = 0;
+  SegList l;
+  const auto flush = [&]() {
+    if (at > 0)
+      launch(muon_moment_kernel, dim3(kNormBlocks, at), dim3(256), 0, st, l, param, grad, momentum, exp_avg_sq,
+             (const float*)hyper, u, part);
+    at = 0;
+  };
+  for (int i = 0; i < n; ++i) {
+    const long long total = segs[i].rows > 0 ? segs[i].rows * segs[i].cols : segs[i].cols;
+    if (segs[i].rows > 0) {
+      l.mat[at] = nm++;
+      l.u[at] = uo / 4;
+      uo += up256(total * 4);
+    } else {
+      l.mat[at] = -1;
+    }
+    if (!total) continue;
+    l.s[at] = segs[i];
+    if (++at == kList) flush();
+  }
+  flush();
+  uo = 0;
+  nm = 0;
+  for (int i = 0; i < n; ++i) {
+    if (segs[i].rows == 0) continue;
+    const long long total = segs[i].rows * segs[i].cols;
+    MatList q;
+    q.m[0] = {u + uo / 4, param + segs[i].offset, segs[i].cols, segs[i].cols, (int)segs[i].rows, (int)segs[i].cols,
+              segs[i].lr_scale, reinterpret_cast<float*>(base + w.x), part + (long long)nm * kNormBlocks};
+    ++nm;
+    uo += up256(total * 4);
+    if (!total) continue;
+    const unsigned blocks = (unsigned)std::min((total + 1023) / 1024, 4096LL);
+    launch(scale_kernel<float>, dim3(blocks, 1), dim3(256), 0, st, q, eps);
+    q.m[0].x = iterate(q.m[0], w, base, steps, coefficients, st);
+    launch(muon_apply_kernel, dim3(blocks, 1), dim3(256), 0, st, q, (const float*)hyper);
+  }
+  launch(muon_tick_kernel, dim3(1), dim3(1), 0, st, hyper);
+  CG_LAUNCH_CHECK("cgan3d_muon_step");
+  return CGAN3D_OK;
+} catch (...) {
+  set_error("cgan3d_muon_step: out of host memory");
+  return CGAN3D_EHIP;
+}

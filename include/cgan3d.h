@@ -79,6 +79,11 @@ typedef struct cgan3d_conv_geom {
  * their gradient can be computed beside the critic update and only this fold stays on the path. */
 #define CGAN3D_ACT_NEG_DTANH 4
 
+/* the linear block only (cgan3d_linear_fwd / cgan3d_linear_bwd): x Phi(x) with the exact error function, and
+ * x / (1 + exp(-x)) */
+#define CGAN3D_ACT_GELU 5
+#define CGAN3D_ACT_SILU 6
+
 /* Fused epilogue: v = acc (+ bias[c]); v = act(v); v *= (mask_src > 0 ? 1 : slope) if mask_src;
  * v += residual if residual; out = v; if out2: out2 = minuend - v (cout == 1 only).
  * stats != NULL: per-block BatchNorm partials (sum, M2, count) of v, consumed by
@@ -575,6 +580,80 @@ int cgan3d_ln_reduce(const cgan3d_ln_args* args, double* partials, void* stream)
 int cgan3d_ln_apply(const cgan3d_ln_args* args, float* out, void* stream);
 int cgan3d_adam(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t n,
                 const float* hyper, void* stream);
+
+/* --- linear block: y = act(x w^T + bias) + residual, and its gradient ---
+ * A pointwise convolution over channels-last voxels, or any layer of rows times a weight in torch's
+ * [out, in] layout.  Every tensor is of `dtype`; products are summed in f32 and rounded once, in the
+ * epilogue.  Rows may be strided (ld*, elements; at least the row's length); preact, dz, dw and dbias are
+ * contiguous.  Any size, zero included, and any alignment of whole elements.
+ *   forward : x, w, y; optional bias [n], residual (may be y itself), preact.
+ *             preact [rows, n], f32 for f32 tensors and f16 for 16-bit ones (saturating): z = x w^T + bias,
+ *             which the backward pass of an activation reads.
+ *   backward: dy, x (for dw), w (for dx), preact (unless act is none); outputs dx, dw, dbias, each
+ *             optional.  dz = dy * act'(z), dx = dz w, dw = dz^T x, dbias = column sums of dz (f32, before
+ *             dz's rounding).  The residual's gradient is dy.  All sums run in a fixed order.
+ * Workspaces: cgan3d_linear_*_ws_bytes (16-byte aligned, -1: refused args), used by one call at a time. */
+#define CGAN3D_DT_F32 0
+#define CGAN3D_DT_BF16 1
+#define CGAN3D_DT_F16 2
+typedef struct cgan3d_linear_args {
+  int64_t rows;
+  int32_t k, n;
+  int32_t dtype;
+  int32_t act;
+  float slope;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* y;
+  int64_t ldy;
+  void* preact;
+  const void* dy;
+  int64_t lddy;
+  void* dx;
+  int64_t lddx;
+  void* dw;
+  void* dbias;
+} cgan3d_linear_args;
+int64_t cgan3d_linear_fwd_ws_bytes(const cgan3d_linear_args* args);
+int cgan3d_linear_fwd(const cgan3d_linear_args* args, void* ws, int64_t ws_bytes, void* stream);
+int64_t cgan3d_linear_bwd_ws_bytes(const cgan3d_linear_args* args);
+int cgan3d_linear_bwd(const cgan3d_linear_args* args, void* ws, int64_t ws_bytes, void* stream);
+
+/* --- orthogonalised updates (the Muon optimiser) ---
+ * Newton-Schulz iteration on each of n matrices (host list): X = g / (|g|_F + eps), then `steps` times
+ * X = a X + (b A + c A A) X with A = X X^T (a tall g by its transpose); out = X, of g's dtype.
+ * coefficients (host): a, b, c.  out may be g itself.  The norm is summed in f64, the iteration keeps f32
+ * accuracy whatever the dtype. */
+typedef struct cgan3d_ortho_mat {
+  const void* g;
+  void* out;
+  int64_t ldg, ldo; /* row strides, elements */
+  int32_t rows, cols;
+} cgan3d_ortho_mat;
+int64_t cgan3d_orthogonalize_ws_bytes(const cgan3d_ortho_mat* mats, int32_t n, int32_t dtype);
+int cgan3d_orthogonalize(const cgan3d_ortho_mat* mats, int32_t n, int32_t dtype, int32_t steps,
+                         const float* coefficients, float eps, void* ws, int64_t ws_bytes, void* stream);
+/* One Muon update of a parameter arena (f32, as cgan3d_adam's), whose segments are listed by segs (host):
+ * rows > 0: a matrix [rows, cols] at offset: momentum m += (1 - mu)(g - m); u = nesterov ? g + mu (m - g)
+ *           : m; p = p (1 - lr weight_decay) - lr lr_scale X(u), X the iteration above;
+ * rows == 0: a vector of cols values: torch.optim.Adam with vector_lr and vector_betas (m is its exp_avg).
+ * Then the weight clip (as cgan3d_adam), if any.  Segments must not overlap; values outside them are left.
+ * hyper (device): [lr, momentum, weight_decay, nesterov, step, clip, vector_lr, vector_beta1,
+ * vector_beta2, vector_eps]; the step counter is advanced at the end. */
+typedef struct cgan3d_muon_seg {
+  int64_t offset;
+  int64_t rows, cols;
+  float lr_scale;
+} cgan3d_muon_seg;
+int64_t cgan3d_muon_ws_bytes(const cgan3d_muon_seg* segs, int32_t n);
+int cgan3d_muon_step(float* param, const float* grad, float* momentum, float* exp_avg_sq, const cgan3d_muon_seg* segs,
+                     int32_t n, float* hyper, int32_t steps, const float* coefficients, float eps, void* ws,
+                     int64_t ws_bytes, void* stream);
 
 /* --- launch plans (the step engine's replacement for a replayed hipGraph; Trainer.py:163-203 is
  * the sequence recorded) ---
