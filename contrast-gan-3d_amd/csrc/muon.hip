@@ -10,14 +10,23 @@
 // Muon (arena segments that are matrices):  m <- m + (1 - mu)(g - m),  u = g + mu (m - g) (Nesterov) or m,
 //   p <- p (1 - lr wd) - lr scale NS(u);   segments that are vectors: Adam with their own rate.
 //
-// The norm is summed in 64 bits (a gradient of 1e-25 squares to nothing in 32), everything else is f32.
+// The norm is summed in 64 bits (a gradient of 1e-25 squares to nothing in 32).  The iteration keeps f32's
+// accuracy on two f16 planes per matrix (planes.h): the iterates are bounded (|X| <= 1.2, |A| <= 1.5 with the
+// coefficients above), so a fixed power of two keeps hi + lo within f16's range: X at 2^12 (an entry of a
+// large orthogonal matrix, ~2^-6, and one of a fresh gradient's, ~2^-12, both keep 22 bits), A and B at 2^10.
+// The first term a X is added in the epilogue from X's own planes: as part of B it would lose the
+// products of the low planes, which directions that start near zero then carry a^5 = 485 times larger.
+// Coefficients that let the iterates leave that range, and no steps at all, take the f32 products of mat.h.
+// A and B are symmetric: the lower triangle's tiles are computed and stored twice.
 #include <climits>
 #include <cmath>
 
-#include "mat.h"
+#include "planes.h"
 
 namespace cg {
 namespace {
+
+long long up256(long long v) { return (v + 255) / 256 * 256; }
 
 constexpr int kNormBlocks = 64;  // partial sums per matrix
 constexpr int kList = 24;        // segments a launch takes by value
@@ -139,22 +148,227 @@ __global__ __launch_bounds__(256) void muon_apply_kernel(MatList l, const float*
   }
 }
 
-__global__ void muon_tick_kernel(float* hyper) { hyper[H_STEP] += 1.f; }
+// --- the iteration on planes ---
+constexpr int kJobs = 12;  // matrices in flight
+constexpr float kXs = 4096.f, kAs = 1024.f;
 
-long long up256(long long v) { return (v + 255) / 256 * 256; }
+// A = X X^T (beta 0) or B = b A + c A A, from sums in the operands' scales to planes in A's
+struct GramEpi {
+  f16_t* out;
+  const f16_t* in;  // A's planes
+  int ld;
+  long long plane;  // elements between planes
+  float alpha, beta;
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool mirror) const {
+    const long long o = (long long)i * ld + j;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r >= jn) break;
+      float x = alpha * v[r];
+      if (in) x += beta * ((float)in[o + r] + (float)in[plane + o + r]);
+      f16_t s[2];
+      split2(x, s);
+      out[o + r] = s[0];
+      out[plane + o + r] = s[1];
+      if (mirror) {
+        const long long m = (long long)(j + r) * ld + i;
+        out[m] = s[0];
+        out[plane + m] = s[1];
+      }
+    }
+  }
+};
+
+// X <- a X + B X: to planes, or where it is the last step to the result / the parameter
+struct StepEpi {
+  f16_t* out;
+  const f16_t* in;  // X's planes
+  long long plane;
+  int ld;
+  int mode;  // 0 planes, 1 + dtype: the result, 4: the parameter
+  float alpha, beta;
+  void* res;
+  long long ldr;
+  int tall;
+  float scale;
+  const float* hyper;
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+    const long long o = (long long)i * ld + j;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r >= jn) break;
+      float x = alpha * v[r] + beta * ((float)in[o + r] + (float)in[plane + o + r]);
+      if (mode == 0) {
+        f16_t s[2];
+        split2(x, s);
+        out[o + r] = s[0];
+        out[plane + o + r] = s[1];
+        continue;
+      }
+      x *= 1.f / kXs;
+      const long long d = tall ? (j + r) * ldr + i : i * ldr + j + r;
+      if (mode == 1 + CGAN3D_DT_F32) {
+        static_cast<float*>(res)[d] = x;
+      } else if (mode == 1 + CGAN3D_DT_BF16) {
+        static_cast<bf16_t*>(res)[d] = (bf16_t)x;
+      } else if (mode == 1 + CGAN3D_DT_F16) {
+        static_cast<f16_t*>(res)[d] = (f16_t)x;
+      } else {
+        float* p = static_cast<float*>(res);
+        const float lr = hyper[H_LR], clip = hyper[H_CLIP];
+        x = p[d] * (1.f - lr * hyper[H_WD]) - lr * scale * x;
+        if (clip > 0.f) x = fminf(fmaxf(x, -clip), clip);
+        p[d] = x;
+      }
+    }
+  }
+};
+
+struct PlaneMat {  // one matrix's planes in the workspace
+  f16_t *x, *y, *a, *b;
+  int s, l, lda, ldx;  // short and long side, row strides of A / B and X / Y (multiples of 32)
+};
+struct PlaneMats {
+  PlaneMat p[kJobs];
+};
+
+// X's planes from G; the padding of the rows is zeroed in all four, once: the products read it, nothing
+// writes it
+template <typename T>
+__global__ __launch_bounds__(256) void planes_kernel(MatList l, PlaneMats pm, float eps) {
+  const Mat& m = l.m[blockIdx.y];
+  const PlaneMat& p = pm.p[blockIdx.y];
+  double s = 0.;
+  for (int b = 0; b < kNormBlocks; ++b) s += m.part[b];
+  const float norm = (float)(sqrt(s) + (double)eps);
+  const T* g = static_cast<const T*>(m.g);
+  const bool tall = m.rows > m.cols;
+  const long long total = (long long)p.s * p.ldx, xp = total, ap = (long long)p.s * p.lda;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256LL) {
+    const long long i = q / p.ldx, t = q - i * p.ldx;
+    f16_t v[2] = {0, 0};
+    if (t < p.l) split2(to_f(tall ? g[t * m.ldg + i] : g[i * m.ldg + t]) / norm * kXs, v);
+    else p.y[q] = p.y[xp + q] = 0;
+    p.x[q] = v[0];
+    p.x[xp + q] = v[1];
+  }
+  const int pad = p.lda - p.s;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < (long long)pad * p.s; q += gridDim.x * 256LL) {
+    const long long o = q / pad * p.lda + p.s + q % pad;
+    p.a[o] = p.a[ap + o] = p.b[o] = p.b[ap + o] = 0;
+  }
+}
+
+int up32(int v) { return (v + 31) / 32 * 32; }
+
+struct PlaneLayout {
+  long long bytes = 0, part = 0;
+};
+// planes of `n` matrices from `ws` on (null: the size alone), then the partial sums of the largest launch
+PlaneLayout plane_layout(const int (*sl)[2], int n, char* ws, PlaneMat* out) {
+  PlaneLayout w;
+  PlaneShape gram[kJobs], poly[kJobs], step[kJobs];
+  for (int i = 0; i < n; ++i) {
+    const int s = sl[i][0], l = sl[i][1], ldx = up32(l), lda = up32(s);
+    const long long xb = up256((long long)s * ldx * 4), ab = up256((long long)s * lda * 4);
+    if (out) {
+      f16_t* at = reinterpret_cast<f16_t*>(ws + w.bytes);
+      out[i] = {at, at + xb / 2, at + xb, at + xb + ab / 2, s, l, lda, ldx};
+    }
+    w.bytes += 2 * xb + 2 * ab;
+    gram[i] = {s, s, ldx};
+    poly[i] = {s, s, lda};
+    step[i] = {s, l, lda};
+  }
+  w.part = w.bytes;
+  const long long f = std::max({plane_pick<2>(gram, n, true).part_floats, plane_pick<2>(poly, n, true).part_floats,
+                                plane_pick<2>(step, n, false).part_floats});
+  w.bytes += up256(f * 4);
+  return w;
+}
+
+// `steps` >= 1 iterations on the matrices of l; the last one writes the results (dt) or the parameters (hyper)
+template <typename T>
+void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co, float eps, int dt, const float* hyper,
+                   hipStream_t st) {
+  PlaneMats pm;
+  int sl[kJobs][2];
+  long long most = 1;
+  for (int i = 0; i < n; ++i) {
+    sl[i][0] = std::min(l.m[i].rows, l.m[i].cols);
+    sl[i][1] = std::max(l.m[i].rows, l.m[i].cols);
+    most = std::max(most, (long long)sl[i][0] * up32(sl[i][1]));
+  }
+  const PlaneLayout w = plane_layout(sl, n, ws, pm.p);
+  float* part = reinterpret_cast<float*>(ws + w.part);
+  launch(planes_kernel<T>, dim3((unsigned)std::min((most + 1023) / 1024, 2048LL), n), dim3(256), 0, st, l, pm, eps);
+  PlaneShape gram[kJobs], poly[kJobs], step[kJobs];
+  PlaneJobs<GramEpi, kJobs> jg, jp;
+  PlaneJobs<StepEpi, kJobs> js;
+  jg.n = jp.n = js.n = n;
+  for (int i = 0; i < n; ++i) {
+    const PlaneMat& p = pm.p[i];
+    gram[i] = {p.s, p.s, p.ldx};
+    poly[i] = {p.s, p.s, p.lda};
+    step[i] = {p.s, p.l, p.lda};
+    const long long xp = (long long)p.s * p.ldx, ap = (long long)p.s * p.lda;
+    jg.j[i] = {{p.x, p.ldx, xp}, {p.x, p.ldx, xp}, p.s, p.s, p.ldx, 0, 0, 0, 0, nullptr,
+               {p.a, nullptr, p.lda, ap, kAs / (kXs * kXs), 0.f}};
+    jp.j[i] = {{p.a, p.lda, ap}, {p.a, p.lda, ap}, p.s, p.s, p.lda, 0, 0, 0, 0, nullptr,
+               {p.b, p.a, p.lda, ap, co[2] / kAs, co[1]}};
+    js.j[i] = {{p.b, p.lda, ap}, {p.x, p.ldx, xp}, p.s, p.l, p.s, 0, 0, 0, 0, nullptr,
+               {p.y, p.x, xp, p.ldx, 0, 1.f / kAs, co[0], l.m[i].out, l.m[i].ldo, l.m[i].rows > l.m[i].cols,
+                l.m[i].scale, hyper}};
+  }
+  const PlanePick pg = plane_pick<2>(gram, n, true), pp = plane_pick<2>(poly, n, true), ps = plane_pick<2>(step, n, false);
+  for (int k = 0; k < steps; ++k) {
+    plane_run<f16_t, 2, false, false, true>(jg, pg, part, st);
+    plane_run<f16_t, 2, false, false, true>(jp, pp, part, st);
+    if (k == steps - 1)
+      for (int i = 0; i < n; ++i) js.j[i].e.mode = hyper ? 4 : 1 + dt;
+    plane_run<f16_t, 2, false, true, false>(js, ps, part, st);
+    for (int i = 0; i < n; ++i) {  // X and Y change places
+      const f16_t* x = js.j[i].e.out;
+      f16_t* y = const_cast<f16_t*>(js.j[i].e.in);
+      js.j[i].e.out = y;
+      js.j[i].e.in = x;
+      js.j[i].b.p = jg.j[i].a.p = jg.j[i].b.p = x;
+    }
+  }
+}
+
+// Whether iterates that start within |X| <= 1 stay where the planes hold them: |X| < 2^16 / kXs, |A| and |B|
+// (largest entry <= largest singular value) < 2^16 / kAs
+bool planes_hold(int steps, const float* co) {
+  if (steps < 1) return false;
+  double r = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    if (r > 7.5 || std::fabs(co[1]) * r * r + std::fabs(co[2]) * r * r * r * r > 60.) return false;
+    double next = 0;
+    for (int q = 1; q <= 4096; ++q) {
+      const double x = r * q / 4096, x2 = x * x;
+      next = std::max(next, std::fabs(x * (co[0] + x2 * (co[1] + x2 * co[2]))));
+    }
+    r = next * 1.01;
+  }
+  return r <= 7.5;
+}
+
+__global__ void muon_tick_kernel(float* hyper) { hyper[H_STEP] += 1.f; }
 
 struct Layout {
   long long part, u, x, x2, a, b, mat, total;
 };
-// The matrices run one after the other, so the iterates and products share one region sized for the largest;
-// every matrix has its own partial sums and (muon) its own update.
+// Every matrix has its own partial sums and (muon) its own update.  Behind them one region, either for the
+// planes of up to kJobs matrices at a time (`planes`) or, with the f32 products, for one matrix after the
+// other.
 void size_mat(Layout& w, long long rows, long long cols) {
   const long long s = std::min(rows, cols), l = std::max(rows, cols);
   w.x = std::max(w.x, up256(s * l * 4));
   w.a = std::max(w.a, up256(s * s * 4));
   w.mat = std::max({w.mat, mat_f32_ws_bytes(s, s, l), mat_f32_ws_bytes(s, s, s), mat_f32_ws_bytes(s, l, s)});
 }
-void place(Layout& w, long long nmat, long long ubytes) {
+void place(Layout& w, long long nmat, long long ubytes, long long planes) {
   const long long x = w.x, a = w.a, m = w.mat;
   w.part = 0;
   w.u = up256(nmat * kNormBlocks * 8);
@@ -163,7 +377,28 @@ void place(Layout& w, long long nmat, long long ubytes) {
   w.a = w.x2 + x;
   w.b = w.a + a;
   w.mat = w.b + a;
-  w.total = w.mat + m;
+  w.total = std::max(w.mat + m, w.x + planes);
+}
+
+// bytes of the largest group of kJobs matrices, in the order the runs take them; rc(i): rows and cols of
+// matrix i (empty ones are left out)
+template <class F> long long plane_bytes(int n, F rc) {
+  int sl[kJobs][2], at = 0;
+  long long most = 0;
+  for (int i = 0; i <= n; ++i) {
+    long long r = 0, c = 0;
+    if (i < n) rc(i, r, c);
+    if (r * c > 0) {
+      sl[at][0] = (int)std::min(r, c);
+      sl[at][1] = (int)std::max(r, c);
+      ++at;
+    }
+    if (at == kJobs || (i == n && at > 0)) {
+      most = std::max(most, plane_layout(sl, at, nullptr, nullptr).bytes);
+      at = 0;
+    }
+  }
+  return most;
 }
 
 // `steps` iterations on m.x; returns where the result is
@@ -218,26 +453,37 @@ const char* mats_check(const cgan3d_ortho_mat* m, int n, int dt) {
 Layout ortho_layout(const cgan3d_ortho_mat* m, int n) {
   Layout w = {};
   for (int i = 0; i < n; ++i) size_mat(w, m[i].rows, m[i].cols);
-  place(w, n, 0);
+  place(w, n, 0, plane_bytes(n, [&](int i, long long& r, long long& c) { r = m[i].rows; c = m[i].cols; }));
   return w;
 }
 
 template <typename T>
-void ortho_run(const cgan3d_ortho_mat* mats, int n, const Layout& w, char* ws, int steps, const float* co, float eps,
-               hipStream_t st) {
+void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, char* ws, int steps, const float* co,
+               float eps, hipStream_t st) {
+  const bool planes = planes_hold(steps, co);
+  MatList l;
+  int at = 0;
+  const auto flush = [&]() {
+    if (!at) return;
+    launch(norm_kernel<T>, dim3(kNormBlocks, at), dim3(256), 0, st, l);
+    if (planes) {
+      plane_iterate<T>(l, at, ws + w.x, steps, co, eps, dt, nullptr, st);
+    } else {
+      const unsigned blocks = (unsigned)std::min(((long long)l.m[0].rows * l.m[0].cols + 1023) / 1024, 4096LL);
+      launch(scale_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l, eps);
+      l.m[0].x = iterate(l.m[0], w, ws, steps, co, st);
+      launch(ortho_out_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l);
+    }
+    at = 0;
+  };
   for (int i = 0; i < n; ++i) {
     const cgan3d_ortho_mat& q = mats[i];
-    const long long total = (long long)q.rows * q.cols;
-    if (!total) continue;
-    MatList l;
-    l.m[0] = {q.g, q.out, q.ldg, q.ldo, q.rows, q.cols, 1.f, reinterpret_cast<float*>(ws + w.x),
-              reinterpret_cast<double*>(ws + w.part) + (long long)i * kNormBlocks};
-    const unsigned blocks = (unsigned)std::min((total + 1023) / 1024, 4096LL);
-    launch(norm_kernel<T>, dim3(kNormBlocks, 1), dim3(256), 0, st, l);
-    launch(scale_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l, eps);
-    l.m[0].x = iterate(l.m[0], w, ws, steps, co, st);
-    launch(ortho_out_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l);
+    if ((long long)q.rows * q.cols == 0) continue;
+    l.m[at++] = {q.g, q.out, q.ldg, q.ldo, q.rows, q.cols, 1.f, reinterpret_cast<float*>(ws + w.x),
+                 reinterpret_cast<double*>(ws + w.part) + (long long)i * kNormBlocks};
+    if (at == (planes ? kJobs : 1)) flush();
   }
+  flush();
 }
 
 const char* segs_check(const cgan3d_muon_seg* s, int n) {
@@ -262,7 +508,7 @@ Layout muon_layout(const cgan3d_muon_seg* s, int n) {
       u += up256(s[i].rows * s[i].cols * 4);
       ++nm;
     }
-  place(w, nm, u);
+  place(w, nm, u, plane_bytes(n, [&](int i, long long& r, long long& c) { r = s[i].rows; c = s[i].cols; }));
   return w;
 }
 
@@ -292,9 +538,9 @@ extern "C" int cgan3d_orthogonalize(const cgan3d_ortho_mat* mats, int32_t n, int
                (long long)ws_bytes);
   hipStream_t st = (hipStream_t)stream;
   char* base = static_cast<char*>(ws);
-  if (dtype == CGAN3D_DT_F32) ortho_run<float>(mats, n, w, base, steps, coefficients, eps, st);
-  else if (dtype == CGAN3D_DT_BF16) ortho_run<bf16_t>(mats, n, w, base, steps, coefficients, eps, st);
-  else ortho_run<f16_t>(mats, n, w, base, steps, coefficients, eps, st);
+  if (dtype == CGAN3D_DT_F32) ortho_run<float>(mats, n, dtype, w, base, steps, coefficients, eps, st);
+  else if (dtype == CGAN3D_DT_BF16) ortho_run<bf16_t>(mats, n, dtype, w, base, steps, coefficients, eps, st);
+  else ortho_run<f16_t>(mats, n, dtype, w, base, steps, coefficients, eps, st);
   CG_LAUNCH_CHECK("cgan3d_orthogonalize");
   return CGAN3D_OK;
 } catch (...) {
@@ -351,20 +597,31 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   flush();
   uo = 0;
   nm = 0;
+  const bool planes = planes_hold(steps, coefficients);
+  MatList q;
+  int qn = 0;
+  const auto run = [&]() {
+    if (!qn) return;
+    if (planes) {
+      plane_iterate<float>(q, qn, base + w.x, steps, coefficients, eps, 0, hyper, st);
+    } else {
+      const unsigned blocks = (unsigned)std::min(((long long)q.m[0].rows * q.m[0].cols + 1023) / 1024, 4096LL);
+      launch(scale_kernel<float>, dim3(blocks, 1), dim3(256), 0, st, q, eps);
+      q.m[0].x = iterate(q.m[0], w, base, steps, coefficients, st);
+      launch(muon_apply_kernel, dim3(blocks, 1), dim3(256), 0, st, q, (const float*)hyper);
+    }
+    qn = 0;
+  };
   for (int i = 0; i < n; ++i) {
     if (segs[i].rows == 0) continue;
     const long long total = segs[i].rows * segs[i].cols;
-    MatList q;
-    q.m[0] = {u + uo / 4, param + segs[i].offset, segs[i].cols, segs[i].cols, (int)segs[i].rows, (int)segs[i].cols,
-              segs[i].lr_scale, reinterpret_cast<float*>(base + w.x), part + (long long)nm * kNormBlocks};
+    q.m[qn] = {u + uo / 4, param + segs[i].offset, segs[i].cols, segs[i].cols, (int)segs[i].rows, (int)segs[i].cols,
+               segs[i].lr_scale, reinterpret_cast<float*>(base + w.x), part + (long long)nm * kNormBlocks};
     ++nm;
     uo += up256(total * 4);
-    if (!total) continue;
-    const unsigned blocks = (unsigned)std::min((total + 1023) / 1024, 4096LL);
-    launch(scale_kernel<float>, dim3(blocks, 1), dim3(256), 0, st, q, eps);
-    q.m[0].x = iterate(q.m[0], w, base, steps, coefficients, st);
-    launch(muon_apply_kernel, dim3(blocks, 1), dim3(256), 0, st, q, (const float*)hyper);
+    if (total && ++qn == (planes ? kJobs : 1)) run();
   }
+  run();
   launch(muon_tick_kernel, dim3(1), dim3(1), 0, st, hyper);
   CG_LAUNCH_CHECK("cgan3d_muon_step");
   return CGAN3D_OK;
