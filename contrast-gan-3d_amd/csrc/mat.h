@@ -14,6 +14,8 @@ namespace cg {
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;
 typedef float f32x4_m __attribute__((ext_vector_type(4)));
+typedef f16_t f16x4_m __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x4_m __attribute__((ext_vector_type(4)));
 typedef f16_t f16x8_m __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8_m __attribute__((ext_vector_type(8)));
 

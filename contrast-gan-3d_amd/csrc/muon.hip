@@ -28,7 +28,7 @@ namespace {
 
 long long up256(long long v) { return (v + 255) / 256 * 256; }
 
-constexpr int kNormBlocks = 64;  // partial sums per matrix
+constexpr int kNormBlocks = 256;  // partial sums per matrix
 constexpr int kList = 24;        // segments a launch takes by value
 
 // hyper (device): see include/cgan3d.h cgan3d_muon_step
@@ -44,6 +44,7 @@ struct Mat {
   double* part;
 };
 
+static_assert(kNormBlocks == 256, "the partial sums are added by a block of 256 threads");
 __device__ __forceinline__ double block_sum_d(double v) {
   __shared__ double red[4];
   v = wave_sum_d(v);
@@ -61,16 +62,34 @@ struct SegList {
   int mat[kList];      // index of the matrix (its partial sums), -1: a vector
 };
 
+// sum of squares of a matrix, kNormBlocks partial sums; 16 bytes a lane where its rows follow each other
 template <typename T>
 __global__ __launch_bounds__(256) void norm_kernel(MatList l) {
+  constexpr int V = MatT<T>::VEC;
+  typedef T vecT __attribute__((ext_vector_type(V)));
   const Mat& m = l.m[blockIdx.y];
   const T* g = static_cast<const T*>(m.g);
-  const long long total = (long long)m.rows * m.cols;
+  const long long total = (long long)m.rows * m.cols, tid = (long long)blockIdx.x * 256 + threadIdx.x;
   double s = 0.;
-  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += kNormBlocks * 256LL) {
-    const long long i = q / m.cols;
-    const double v = to_f(g[i * m.ldg + (q - i * m.cols)]);
-    s += v * v;
+  if ((m.ldg == m.cols || m.rows == 1) && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+    for (long long q = tid; q < total / V; q += kNormBlocks * 256LL) {
+      const vecT x = reinterpret_cast<const vecT*>(g)[q];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const double v = to_f(x[e]);
+        s += v * v;
+      }
+    }
+    if (tid < total % V) {
+      const double v = to_f(g[total / V * V + tid]);
+      s += v * v;
+    }
+  } else {
+    for (long long q = tid; q < total; q += kNormBlocks * 256LL) {
+      const long long i = q / m.cols;
+      const double v = to_f(g[i * m.ldg + (q - i * m.cols)]);
+      s += v * v;
+    }
   }
   s = block_sum_d(s);
   if (threadIdx.x == 0) m.part[blockIdx.x] = s;
@@ -109,8 +128,7 @@ __global__ __launch_bounds__(256) void muon_moment_kernel(SegList l, float* __re
 template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(MatList l, float eps) {
   const Mat& m = l.m[blockIdx.y];
-  double s = 0.;
-  for (int b = 0; b < kNormBlocks; ++b) s += m.part[b];
+  const double s = block_sum_d(m.part[threadIdx.x]);  // one partial sum a thread
   const float norm = (float)(sqrt(s) + (double)eps);
   const T* g = static_cast<const T*>(m.g);
   const bool tall = m.rows > m.cols;
@@ -156,11 +174,67 @@ constexpr float kXs = 4096.f, kAs = 1024.f;
 struct GramEpi {
   f16_t* out;
   const f16_t* in;  // A's planes
-  int ld;
+  int ld, n;        // row stride, side
   long long plane;  // elements between planes
   float alpha, beta;
+  // called by whole waves: lane l has row l % 16 and columns 4 (l / 16) .. + 3 of a 16 x 16 block
   __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool mirror) const {
     const long long o = (long long)i * ld + j;
+    const int lane = threadIdx.x & 63, t = lane & 3;
+    if (jn >= 4) {
+      f16x4_m h, l;
+      f32x4_m x = alpha * v;
+      if (in) {
+        const f16x4_m a = *reinterpret_cast<const f16x4_m*>(in + o), c = *reinterpret_cast<const f16x4_m*>(in + plane + o);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] += beta * ((float)a[r] + (float)c[r]);
+      }
+      unsigned w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f16_t s[2];
+        split2(x[r], s);
+        h[r] = s[0];
+        l[r] = s[1];
+        w[r] = __builtin_bit_cast(unsigned short, s[0]) | (unsigned)__builtin_bit_cast(unsigned short, s[1]) << 16;
+      }
+      *reinterpret_cast<f16x4_m*>(out + o) = h;
+      *reinterpret_cast<f16x4_m*>(out + plane + o) = l;
+      if (!mirror) return;
+      if ((i & ~15) + 16 <= n) {
+        // 4 x 4 transposes in the quads of lanes (rows i .. i + 3 of four columns): lane t ends up with column
+        // j + t of the quad's four rows, which are neighbours in the mirrored row
+#define CG_SWAP(A, B, CTRL, BIT)                                                                              \
+  {                                                                                                           \
+    const unsigned pa = __builtin_amdgcn_mov_dpp(A, CTRL, 0xf, 0xf, true),                                    \
+                   pb = __builtin_amdgcn_mov_dpp(B, CTRL, 0xf, 0xf, true);                                    \
+    A = (t & BIT) ? pb : A;                                                                                   \
+    B = (t & BIT) ? B : pa;                                                                                   \
+  }
+        CG_SWAP(w[0], w[1], 0xB1, 1)
+        CG_SWAP(w[2], w[3], 0xB1, 1)
+        CG_SWAP(w[0], w[2], 0x4E, 2)
+        CG_SWAP(w[1], w[3], 0x4E, 2)
+#undef CG_SWAP
+        const long long m = (long long)(j + t) * ld + (i & ~3);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          h[r] = __builtin_bit_cast(f16_t, (unsigned short)w[r]);
+          l[r] = __builtin_bit_cast(f16_t, (unsigned short)(w[r] >> 16));
+        }
+        *reinterpret_cast<f16x4_m*>(out + m) = h;
+        *reinterpret_cast<f16x4_m*>(out + plane + m) = l;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const long long m = (long long)(j + r) * ld + i;
+          out[m] = h[r];
+          out[plane + m] = l[r];
+        }
+      }
+      return;
+    }
+    // the last columns of the last tile, which is on the diagonal: no mirror
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if (r >= jn) break;
@@ -170,11 +244,6 @@ struct GramEpi {
       split2(x, s);
       out[o + r] = s[0];
       out[plane + o + r] = s[1];
-      if (mirror) {
-        const long long m = (long long)(j + r) * ld + i;
-        out[m] = s[0];
-        out[plane + m] = s[1];
-      }
     }
   }
 };
@@ -192,33 +261,63 @@ struct StepEpi {
   int tall;
   float scale;
   const float* hyper;
-  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
-    const long long o = (long long)i * ld + j;
+  template <typename T> __device__ __forceinline__ void store(int i, int j, f32x4_m x, int jn) const {
+    T* p = static_cast<T*>(res);
+    if (tall) {  // 16 lanes write 16 neighbours
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (r >= jn) break;
-      float x = alpha * v[r] + beta * ((float)in[o + r] + (float)in[plane + o + r]);
-      if (mode == 0) {
+      for (int r = 0; r < 4; ++r)
+        if (r < jn) p[(j + r) * ldr + i] = (T)x[r];
+      return;
+    }
+    p += i * ldr + j;
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    if (jn >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0) {
+      v4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = (T)x[r];
+      *reinterpret_cast<v4*>(p) = o;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < jn) p[r] = (T)x[r];
+    }
+  }
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+    const long long o = (long long)i * ld + j;  // rows of whole 32s: four columns are always there to read
+    const f16x4_m a = *reinterpret_cast<const f16x4_m*>(in + o), c = *reinterpret_cast<const f16x4_m*>(in + plane + o);
+    f32x4_m x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = alpha * v[r] + beta * ((float)a[r] + (float)c[r]);
+    if (mode == 0) {
+      f16x4_m h, l;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
         f16_t s[2];
-        split2(x, s);
-        out[o + r] = s[0];
-        out[plane + o + r] = s[1];
-        continue;
+        split2(r < jn ? x[r] : 0.f, s);  // the padding stays zero
+        h[r] = s[0];
+        l[r] = s[1];
       }
-      x *= 1.f / kXs;
-      const long long d = tall ? (j + r) * ldr + i : i * ldr + j + r;
-      if (mode == 1 + CGAN3D_DT_F32) {
-        static_cast<float*>(res)[d] = x;
-      } else if (mode == 1 + CGAN3D_DT_BF16) {
-        static_cast<bf16_t*>(res)[d] = (bf16_t)x;
-      } else if (mode == 1 + CGAN3D_DT_F16) {
-        static_cast<f16_t*>(res)[d] = (f16_t)x;
-      } else {
-        float* p = static_cast<float*>(res);
-        const float lr = hyper[H_LR], clip = hyper[H_CLIP];
-        x = p[d] * (1.f - lr * hyper[H_WD]) - lr * scale * x;
-        if (clip > 0.f) x = fminf(fmaxf(x, -clip), clip);
-        p[d] = x;
+      *reinterpret_cast<f16x4_m*>(out + o) = h;
+      *reinterpret_cast<f16x4_m*>(out + plane + o) = l;
+      return;
+    }
+    x *= 1.f / kXs;
+    if (mode == 1 + CGAN3D_DT_F32) {
+      store<float>(i, j, x, jn);
+    } else if (mode == 1 + CGAN3D_DT_BF16) {
+      store<bf16_t>(i, j, x, jn);
+    } else if (mode == 1 + CGAN3D_DT_F16) {
+      store<f16_t>(i, j, x, jn);
+    } else {
+      float* p = static_cast<float*>(res);
+      const float lr = hyper[H_LR], clip = hyper[H_CLIP], keep = 1.f - lr * hyper[H_WD], rate = lr * scale;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (r >= jn) break;
+        const long long d = tall ? (j + r) * ldr + i : i * ldr + j + r;
+        float w = p[d] * keep - rate * x[r];
+        if (clip > 0.f) w = fminf(fmaxf(w, -clip), clip);
+        p[d] = w;
       }
     }
   }
@@ -232,25 +331,52 @@ struct PlaneMats {
   PlaneMat p[kJobs];
 };
 
-// X's planes from G; the padding of the rows is zeroed in all four, once: the products read it, nothing
-// writes it
+// X's planes from G, 32 x 64 of them at a time (a tall G is turned in LDS); the padding of the rows is zeroed
+// in all four, once: the products read it, nothing else is written there
 template <typename T>
 __global__ __launch_bounds__(256) void planes_kernel(MatList l, PlaneMats pm, float eps) {
+  __shared__ float tile[64][33];
   const Mat& m = l.m[blockIdx.y];
   const PlaneMat& p = pm.p[blockIdx.y];
-  double s = 0.;
-  for (int b = 0; b < kNormBlocks; ++b) s += m.part[b];
+  const double s = block_sum_d(m.part[threadIdx.x]);  // one partial sum a thread
   const float norm = (float)(sqrt(s) + (double)eps);
   const T* g = static_cast<const T*>(m.g);
   const bool tall = m.rows > m.cols;
-  const long long total = (long long)p.s * p.ldx, xp = total, ap = (long long)p.s * p.lda;
-  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256LL) {
-    const long long i = q / p.ldx, t = q - i * p.ldx;
-    f16_t v[2] = {0, 0};
-    if (t < p.l) split2(to_f(tall ? g[t * m.ldg + i] : g[i * m.ldg + t]) / norm * kXs, v);
-    else p.y[q] = p.y[xp + q] = 0;
-    p.x[q] = v[0];
-    p.x[xp + q] = v[1];
+  const long long xp = (long long)p.s * p.ldx, ap = (long long)p.s * p.lda;
+  const int nc = (p.ldx + 63) / 64, nt = (p.s + 31) / 32 * nc;
+  for (int b = blockIdx.x; b < nt; b += gridDim.x) {
+    const int i0 = b / nc * 32, t0 = b % nc * 64;
+    if (tall) {
+      __syncthreads();
+      for (int q = threadIdx.x; q < 64 * 32; q += 256) {  // rows of G are columns of X
+        const int t = t0 + q / 32, i = i0 + q % 32;
+        tile[q / 32][q % 32] = t < p.l && i < p.s ? to_f(g[t * m.ldg + i]) : 0.f;
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int q = threadIdx.x; q < 32 * 16; q += 256) {
+      const int i = i0 + q / 16, t = t0 + q % 16 * 4;
+      if (i >= p.s || t >= p.ldx) continue;
+      f16x4_m h, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = 0.f;
+        if (t + r < p.l) x = (tall ? tile[t - t0 + r][i - i0] : to_f(g[i * m.ldg + t + r])) / norm * kXs;
+        f16_t v[2];
+        split2(x, v);
+        h[r] = v[0];
+        lo[r] = v[1];
+      }
+      const long long o = (long long)i * p.ldx + t;
+      *reinterpret_cast<f16x4_m*>(p.x + o) = h;
+      *reinterpret_cast<f16x4_m*>(p.x + xp + o) = lo;
+      if (t + 4 > p.l) {
+        const f16x4_m z = {0, 0, 0, 0};  // values of the iterate itself come later
+        *reinterpret_cast<f16x4_m*>(p.y + o) = z;
+        *reinterpret_cast<f16x4_m*>(p.y + xp + o) = z;
+      }
+    }
   }
   const int pad = p.lda - p.s;
   for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < (long long)pad * p.s; q += gridDim.x * 256LL) {
@@ -297,11 +423,11 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
   for (int i = 0; i < n; ++i) {
     sl[i][0] = std::min(l.m[i].rows, l.m[i].cols);
     sl[i][1] = std::max(l.m[i].rows, l.m[i].cols);
-    most = std::max(most, (long long)sl[i][0] * up32(sl[i][1]));
+    most = std::max(most, (sl[i][0] + 31LL) / 32 * ((up32(sl[i][1]) + 63) / 64));
   }
   const PlaneLayout w = plane_layout(sl, n, ws, pm.p);
   float* part = reinterpret_cast<float*>(ws + w.part);
-  launch(planes_kernel<T>, dim3((unsigned)std::min((most + 1023) / 1024, 2048LL), n), dim3(256), 0, st, l, pm, eps);
+  launch(planes_kernel<T>, dim3((unsigned)std::min(most, 2048LL), n), dim3(256), 0, st, l, pm, eps);
   PlaneShape gram[kJobs], poly[kJobs], step[kJobs];
   PlaneJobs<GramEpi, kJobs> jg, jp;
   PlaneJobs<StepEpi, kJobs> js;
@@ -313,9 +439,9 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
     step[i] = {p.s, p.l, p.lda};
     const long long xp = (long long)p.s * p.ldx, ap = (long long)p.s * p.lda;
     jg.j[i] = {{p.x, p.ldx, xp}, {p.x, p.ldx, xp}, p.s, p.s, p.ldx, 0, 0, 0, 0, nullptr,
-               {p.a, nullptr, p.lda, ap, kAs / (kXs * kXs), 0.f}};
+               {p.a, nullptr, p.lda, p.s, ap, kAs / (kXs * kXs), 0.f}};
     jp.j[i] = {{p.a, p.lda, ap}, {p.a, p.lda, ap}, p.s, p.s, p.lda, 0, 0, 0, 0, nullptr,
-               {p.b, p.a, p.lda, ap, co[2] / kAs, co[1]}};
+               {p.b, p.a, p.lda, p.s, ap, co[2] / kAs, co[1]}};
     js.j[i] = {{p.b, p.lda, ap}, {p.x, p.ldx, xp}, p.s, p.l, p.s, 0, 0, 0, 0, nullptr,
                {p.y, p.x, xp, p.ldx, 0, 1.f / kAs, co[0], l.m[i].out, l.m[i].ldo, l.m[i].rows > l.m[i].cols,
                 l.m[i].scale, hyper}};

@@ -9,8 +9,8 @@
 // f32 matrix instructions run at 154 TFLOP/s on a large product, 16-bit ones at 1365: a third of that is 455, a
 // sixth 227, so f32 accuracy from planes is 3.0 and 1.5 times what the f32 instructions can reach.
 //
-// A tile's planes go to LDS by DMA (global_load_lds, 16 bytes a lane, one stage ahead of the products, two
-// buffers, one barrier a stage).  A t-contiguous operand lies there as rows of BK values and is read by
+// A tile's planes go to LDS by DMA (global_load_lds, 16 bytes a lane, one to three stages ahead of the
+// products, one barrier a stage).  A t-contiguous operand lies there as rows of BK values and is read by
 // ds_read_b128; a t-strided one as BK rows of its own and is read by ds_read_b64_tr_b16, which hands lane i of
 // a group of 16 column i of four rows: transposed operands cost no pass over memory.  DMA writes LDS in lane
 // order, so bank conflicts are avoided on the global side: each lane fetches the 16-byte chunk whose
@@ -146,14 +146,21 @@ template <int BM, bool SYM> __device__ __forceinline__ void plane_tile(int t, in
   }
 }
 
-template <typename T, int P, bool AT, bool BT, int BM, int BN, int BK, int WI, int WJ, bool SYM, class E, int N>
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+// One BM x BN tile, WI x WJ waves, BK values of t a stage, S stage buffers: S - 1 stages are in flight ahead.
+// The barrier that opens a new stage comes before the last row of products of the one before: they cover the
+// wait for the other waves and the reads of the next stage's first fragments, each of B's in the registers
+// of its predecessor right behind that one's last use.
+template <typename T, int P, bool AT, bool BT, int BM, int BN, int BK, int S, int WI, int WJ, bool SYM, class E, int N>
 __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> jobs) {
-  constexpr int NW = WI * WJ, WM = BM / WI, WN = BN / WJ, FM = WM / 16, FN = WN / 16;
+  constexpr int NW = WI * WJ, WM = BM / WI, WN = BN / WJ, FM = WM / 16, FN = WN / 16, H = BK / 32;
   using TA = PlaneTile<AT, BM, BK, NW>;
   using TB = PlaneTile<BT, BN, BK, NW>;
-  constexpr int STAGE = P * (TA::BYTES + TB::BYTES);
-  static_assert(2 * STAGE <= 160 * 1024, "two stages fit the LDS");
-  __shared__ __align__(16) unsigned char lds[2 * STAGE];
+  constexpr int STAGE = P * (TA::BYTES + TB::BYTES), REQ = P * (TA::Q + TB::Q);
+  static_assert(S * STAGE <= 160 * 1024 && (S - 1) * REQ < 64, "the stages fit the LDS, their requests the counter");
+  static_assert(FM >= 2, "two rows of fragments behind the barrier");
+  __shared__ __align__(16) unsigned char lds[S * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int b = xcd_order(blockIdx.x, gridDim.x), jn = 0;
   if constexpr (N > 1)
@@ -173,9 +180,11 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
   tb.init(p.b, p.J, j0, wave, lane);
   typedef __attribute__((address_space(3))) void* lvp;
   const unsigned base = (unsigned)(uintptr_t)(lvp)lds;
+  int slot_in = 0, slot = 0;  // ring positions of the next stage to request and of the one being read
   const auto issue = [&](int s) {
     const int k = k0 + s * BK;
-    const unsigned at = base + (s & 1) * STAGE;
+    const unsigned at = base + slot_in * STAGE;
+    slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
 #pragma unroll
     for (int q = 0; q < P; ++q) {
       ta.issue(p.a, k, k1 - k, q * p.a.plane, at + q * TA::BYTES, wave);
@@ -183,36 +192,77 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
     }
   };
   f32x4_m acc[FM][FN] = {};
-  if (steps > 0) issue(0);
-  for (int s = 0; s < steps; ++s) {
-    // this stage has landed for every wave, and every wave is done reading the other buffer
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  s16x8_v fb[P][FN], fa[2][P];  // B's fragments of the unit, A's first two rows of them
+  const auto read_a = [&](s16x8_v(&f)[P], int m, int h) {
+    const unsigned char* la = lds + slot * STAGE;
+#pragma unroll
+    for (int q = 0; q < P; ++q) f[q] = plane_frag<AT, BM, BK>(la + q * TA::BYTES, wi + m * 16, h, lane);
+  };
+  const auto read_b = [&](int n, int h) {
+    const unsigned char* lb = lds + slot * STAGE + P * TA::BYTES;
+#pragma unroll
+    for (int q = 0; q < P; ++q) fb[q][n] = plane_frag<BT, BN, BK>(lb + q * TB::BYTES, wj + n * 16, h, lane);
+  };
+  // small products first; operands swapped, so that a lane ends up with neighbouring columns
+  const auto row = [&](int m, const s16x8_v(&a)[P]) {
+#pragma unroll
+    for (int o = P - 1; o >= 0; --o)
+#pragma unroll
+      for (int q = 0; q <= o; ++q)
+#pragma unroll
+        for (int n = 0; n < FN; ++n) acc[m][n] = plane_mfma(fb[o - q][n], a[q], acc[m][n], T());
+  };
+  // waits until stage s + 1 (of `steps`) has landed; s + S - 1 is the last one requested
+  const auto landed = [&](int s) {
+    if (S > 2 && s + S - 1 < steps) wait_vm<(S - 2) * REQ>();
+    else wait_vm<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < steps) issue(s + 1);
-    const unsigned char* la = lds + (s & 1) * STAGE;
-    const unsigned char* lb = la + P * TA::BYTES;
+  };
+  const auto unit = [&](int s, int h) {
+    if (h == 0 && s + S - 1 < steps) issue(s + S - 1);
+    s16x8_v fr[FM][P];
 #pragma unroll
-    for (int h = 0; h < BK / 32; ++h) {
-      s16x8_v fb[P][FN];
-#pragma unroll
-      for (int q = 0; q < P; ++q)
-#pragma unroll
-        for (int n = 0; n < FN; ++n) fb[q][n] = plane_frag<BT, BN, BK>(lb + q * TB::BYTES, wj + n * 16, h, lane);
-#pragma unroll
-      for (int m = 0; m < FM; ++m) {
-        s16x8_v fa[P];
-#pragma unroll
-        for (int q = 0; q < P; ++q) fa[q] = plane_frag<AT, BM, BK>(la + q * TA::BYTES, wi + m * 16, h, lane);
-        // small products first; operands swapped, so that a lane ends up with neighbouring columns
-#pragma unroll
-        for (int o = P - 1; o >= 0; --o)
-#pragma unroll
-          for (int q = 0; q <= o; ++q)
-#pragma unroll
-            for (int n = 0; n < FN; ++n) acc[m][n] = plane_mfma(fb[o - q][n], fa[q], acc[m][n], T());
-      }
+    for (int m = 0; m < FM - 1; ++m) {
+      if (m + 2 < FM) read_a(fr[m + 2], m + 2, h);
+      if (m < 2) row(m, fa[m]);
+      else row(m, fr[m]);
     }
+    s16x8_v last[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) last[q] = FM > 2 ? fr[FM - 1][q] : fa[1][q];
+    if (h + 1 == H && s + 1 < steps) {
+      landed(s);
+      slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    // behind the last stage these read that stage again, for nothing: a branch here would cut the row apart
+    const int hn = h + 1 < H ? h + 1 : 0;
+    read_a(fa[0], 0, hn);
+    read_a(fa[1], 1, hn);
+#pragma unroll
+    for (int n = 0; n < FN; ++n) {  // the last row column by column: its fragment of B is free behind it
+#pragma unroll
+      for (int o = P - 1; o >= 0; --o)
+#pragma unroll
+        for (int q = 0; q <= o; ++q) acc[FM - 1][n] = plane_mfma(fb[o - q][n], last[q], acc[FM - 1][n], T());
+      read_b(n, hn);
+    }
+  };
+  if (steps > 0) {
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s)
+      if (s < steps) issue(s);
+    if (steps >= S - 1) wait_vm<(S - 2) * REQ>();
+    else wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read_a(fa[0], 0, 0);
+#pragma unroll
+    for (int n = 0; n < FN; ++n) read_b(n, 0);
+    read_a(fa[1], 1, 0);
+    for (int s = 0; s < steps; ++s)
+#pragma unroll
+      for (int h = 0; h < H; ++h) unit(s, h);
   }
   if (p.part) {
     float* o = p.part + ((long long)split * p.tiles + t) * (BM * BN);
@@ -250,7 +300,8 @@ __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
   int ti, tj;
   plane_tile<BM, SYM>(t, p.I, p.tj, ti, tj);
   for (int q = threadIdx.x; q < 32 * BN / 4; q += 256) {
-    const int li = sub * 32 + q / (BN / 4), lj = q % (BN / 4) * 4, i = ti * BM + li, j = tj * BN + lj;
+    // 16 lanes on 16 rows, as the products leave them: a mirrored value's neighbours are written together
+    const int li = sub * 32 + q / (BN * 4) * 16 + q % 16, lj = q / 16 % (BN / 4) * 4, i = ti * BM + li, j = tj * BN + lj;
     if (i >= p.I || j >= p.J) continue;
     const float* s = p.part + (long long)t * (BM * BN) + li * BN + lj;
     f32x4_m v = *reinterpret_cast<const f32x4_m*>(s);
@@ -271,15 +322,15 @@ struct PlanePick {
 // blocks where there are few
 template <int P> struct PlaneCfg;
 template <> struct PlaneCfg<1> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 64, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {4, 4, 4};
   static constexpr float RATE[3] = {1.f, 0.75f, 0.4f};
 };
 template <> struct PlaneCfg<2> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {2, 2, 3};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<3> {
-  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2};
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 3};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 
@@ -351,7 +402,7 @@ void plane_run(PlaneJobs<E, N>& jobs, const PlanePick& pick, float* part, hipStr
       jat += j.tiles * (BM / 32);
     }
     if (at == 0) return;
-    launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK, C::WI[c], C::WJ[c], SYM, E, N>, dim3(at),
+    launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK, C::S[c], C::WI[c], C::WJ[c], SYM, E, N>, dim3(at),
            dim3(C::WI[c] * C::WJ[c] * 64), 0, st, jobs);
     if (join) launch(plane_join_kernel<BM, BN, SYM, E, N>, dim3(jat), dim3(256), 0, st, js);
   };
