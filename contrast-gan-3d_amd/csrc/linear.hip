@@ -6,9 +6,16 @@
 //
 // The epilogue runs on the accumulators, so z, act(z) and the sum with r never pass through memory,
 // apart from z itself where a backward pass will want it.
+//
+// Which kernel a product takes (mat_route):
+//   rows <= 4, forward     gemv_kernel: a wave per output column pair streams the weight once
+//   16-bit tensors         plane_kernel (planes.h) on the tensors themselves; an operand whose rows are not
+//                          whole aligned 16-byte chunks is copied once into rows that are
+//   f32 tensors            plane_kernel on three bf16 planes where the product is large enough to pay for
+//                          the splitting, else mat_kernel (mat.h: f32 instructions, any layout)
 #include <climits>
 
-#include "mat.h"
+#include "planes.h"
 
 namespace cg {
 namespace {
@@ -51,76 +58,481 @@ void mat_run(int dt, const MatArgs& p, void* ws, hipStream_t st) {
   else mat_run_t<f16_t, AT, BT>(p, ws, st);
 }
 
-// dz = dy * act'(z) and the column sums of dz (in 32 bits, before its rounding): 64 columns x 4 rows a
-// block, `rows` rows of them; part [blockIdx.y][n].
-template <typename T>
-__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, long long lddy,
-                                                       const typename PreT<T>::type* __restrict__ pre, T* __restrict__ dz,
-                                                       float* __restrict__ part, long long rows, int n, long long chunk,
-                                                       int act, float slope) {
-  __shared__ float red[4][64];
-  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-  const long long j = (long long)blockIdx.x * 64 + c;
-  const long long i1 = std::min(rows, ((long long)blockIdx.y + 1) * chunk);
-  float s = 0.f;
-  if (j < n) {
-    for (long long i = (long long)blockIdx.y * chunk + r; i < i1; i += 4) {
-      float v = to_f(dy[i * lddy + j]);
-      if (act != CGAN3D_ACT_NONE) {
-        v *= mat_act_grad(to_f(pre[i * n + j]), act, slope);
-        dz[i * n + j] = from_f<T>(v);
+// --- products on planes ---
+constexpr int kGemvRows = 4;
+
+// Epilogue of a plane product.  NANFIX (f32 on three planes): an infinity times an empty lower plane
+// is NaN, so a NaN sum is computed again value by value, which leaves what f32 gives.
+template <typename T, bool NANFIX> struct LinEpi {
+  MatEpi e;
+  long long J;
+  int vec;  // every tensor of the epilogue takes vectors of four
+  struct Values {  // NANFIX: an operand's planes; element (i, t) at i si + t st
+    const bf16_t* p;
+    long long plane, si, st;
+    __device__ __forceinline__ float at(long long i, long long t) const {
+      const bf16_t* q = p + i * si + t * st;
+      return ((float)q[0] + (float)q[plane]) + (float)q[2 * plane];
+    }
+  };
+  Values a, b;
+  long long K;
+  __device__ __noinline__ float again(int i, int j) const {
+    float s = 0.f;
+    for (long long t = 0; t < K; ++t) s = fmaf(a.at(i, t), b.at(j, t), s);
+    return s;
+  }
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+    if constexpr (NANFIX) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < jn && v[r] != v[r]) v[r] = again(i, j + r);
+    }
+    if (jn < 4 || !vec) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < jn) mat_store<T>(e, J, i, j + r, v[r]);
+      return;
+    }
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    typedef typename PreT<T>::type preT;
+    typedef preT p4 __attribute__((ext_vector_type(4)));
+    v *= e.alpha;
+    if (e.bias) {
+      const v4 b = *reinterpret_cast<const v4*>(static_cast<const T*>(e.bias) + j);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += to_f(b[r]);
+    }
+    if (e.preact) {
+      p4 p;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        preT q;
+        mat_preact(&q, v[r]);
+        p[r] = q;
       }
-      s += v;
+      *reinterpret_cast<p4*>(static_cast<preT*>(e.preact) + i * J + j) = p;
+    }
+    if (e.act != CGAN3D_ACT_NONE) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = mat_act(v[r], e.act, e.slope);
+    }
+    if (e.residual) {
+      const v4 b = *reinterpret_cast<const v4*>(static_cast<const T*>(e.residual) + i * e.ldr + j);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += e.beta * to_f(b[r]);
+    }
+    v4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = from_f<T>(v[r]);
+    *reinterpret_cast<v4*>(static_cast<T*>(e.out) + i * e.ldo + j) = o;
+  }
+};
+
+bool vec4(const void* p, long long ld, int elt) { return !p || (reinterpret_cast<uintptr_t>(p) % (4 * elt) == 0 && ld % 4 == 0); }
+
+// an operand as planes: copied (16-bit) or split (f32) into rows of whole chunks, padding zeroed
+struct Pack {
+  const void* src;
+  long long ld, rows;
+  int cols, ldp;
+  void* dst;
+  long long first;  // chunk number of the launch at which this operand starts
+};
+struct Packs {
+  Pack p[2];
+  long long chunks;
+};
+long long up8(long long v) { return (v + 7) / 8 * 8; }
+long long up256(long long v) { return (v + 255) / 256 * 256; }
+
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(Packs ps) {
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < ps.chunks; q += gridDim.x * 256LL) {
+    const Pack& p = ps.p[q >= ps.p[1].first];
+    const long long u = q - p.first;
+    const int nc = p.ldp / 8;
+    const long long row = u / nc;
+    const int c = (int)(u - row * nc) * 8;
+    const T* s = static_cast<const T*>(p.src) + row * p.ld + c;
+    T v[8];
+    if (c + 8 <= p.cols && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
+      typedef T vt __attribute__((ext_vector_type(MatT<T>::VEC)));
+#pragma unroll
+      for (int h = 0; h < 8 / MatT<T>::VEC; ++h)
+        *reinterpret_cast<vt*>(v + h * MatT<T>::VEC) = *reinterpret_cast<const vt*>(s + h * MatT<T>::VEC);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? s[e] : from_f<T>(0.f);
+    }
+    if constexpr (sizeof(T) == 4) {
+      const long long plane = p.rows * p.ldp, o = row * p.ldp + c;
+      bf16x8_m h, m, l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bf16_t t[3];
+        split3(v[e], t);
+        h[e] = t[0];
+        m[e] = t[1];
+        l[e] = t[2];
+      }
+      bf16_t* d = static_cast<bf16_t*>(p.dst) + o;
+      *reinterpret_cast<bf16x8_m*>(d) = h;
+      *reinterpret_cast<bf16x8_m*>(d + plane) = m;
+      *reinterpret_cast<bf16x8_m*>(d + 2 * plane) = l;
+    } else {
+      typedef T v8 __attribute__((ext_vector_type(8)));
+      *reinterpret_cast<v8*>(static_cast<T*>(p.dst) + row * p.ldp + c) = *reinterpret_cast<v8*>(v);
     }
   }
-  red[r][c] = s;
+}
+
+bool chunked(const void* p, long long ld, long long cols) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0;
+}
+
+// One operand of a product: [rows, cols] with row stride ld; `strided`: its rows are summed over.
+struct Operand {
+  const void* p;
+  long long ld, rows;
+  int cols;
+  bool strided;
+  bool planes;  // p already holds planes (dz), rows of ld values
+};
+
+enum Route { ROUTE_MAT, ROUTE_PLANES };
+
+// f32: splitting both operands (4 bytes read, 6 written a value) and six 16-bit products at ~1000 TFLOP/s
+// against f32 instructions at ~80 (measured: 2048 x 1024 -> 4096, forward and backward, see DESIGN's table)
+Route mat_route(int dt, long long I, long long J, long long K) {
+  if (K == 0 || K >= 1 << 30 || I >= 1 << 30 || J >= 1 << 30) return ROUTE_MAT;
+  if (dt != CGAN3D_DT_F32) return ROUTE_PLANES;
+  const double fl = 2.0 * I * J * K, pack = 10.0 * K * (I + J);
+  return fl / 80e12 > fl / 160e12 + pack / 4e12 + 4e-6 ? ROUTE_PLANES : ROUTE_MAT;
+}
+
+long long operand_bytes(int dt, const Operand& o) {
+  if (o.planes) return 0;
+  if (dt == CGAN3D_DT_F32) return up256(o.rows * up8(o.cols) * 6);
+  return chunked(o.p, o.ld, o.cols) ? 0 : up256(o.rows * up8(o.cols) * 2);
+}
+PlanePick pick_for(int dt, long long I, long long J, long long K) {
+  const PlaneShape s = {(int)I, (int)J, (int)K};
+  return dt == CGAN3D_DT_F32 ? plane_pick<3>(&s, 1, false) : plane_pick<1>(&s, 1, false);
+}
+// workspace of one product: both operands' planes, then partial sums
+long long product_bytes(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
+  if (I == 0 || J == 0) return 0;
+  if (mat_route(dt, I, J, K) == ROUTE_MAT) return mat_ws_bytes(I, J, K);
+  return operand_bytes(dt, a) + operand_bytes(dt, b) + pick_for(dt, I, J, K).part_floats * 4;
+}
+
+template <typename T, typename PT, int P>
+void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStream_t st) {
+  char* at = static_cast<char*>(ws);
+  Packs ps = {};
+  const Operand a0 = a, b0 = b;
+  int np = 0;
+  Operand* os[2] = {&a, &b};
+  for (Operand* o : os) {
+    const long long bytes = operand_bytes(dt, *o);
+    if (!bytes) continue;
+    const int ldp = (int)up8(o->cols);
+    ps.p[np++] = {o->p, o->ld, o->rows, o->cols, ldp, at, ps.chunks};
+    ps.chunks += o->rows * (ldp / 8);
+    o->p = at;
+    o->ld = ldp;
+    at += bytes;
+  }
+  if (np == 1) ps.p[1].first = LLONG_MAX;
+  if (ps.chunks)
+    launch(pack_kernel<T>, dim3((unsigned)std::min((ps.chunks + 255) / 256, 16384LL)), dim3(256), 0, st, ps);
+  PlaneJobs<LinEpi<T, P == 3>, 1> jobs;
+  jobs.n = 1;
+  auto& j = jobs.j[0];
+  j.a = {a.p, a.ld, a.rows * a.ld};
+  j.b = {b.p, b.ld, b.rows * b.ld};
+  j.I = (int)m.I;
+  j.J = (int)m.J;
+  j.K = (int)m.K;
+  j.e.e = m.e;
+  j.e.J = m.J;
+  j.e.vec = vec4(m.e.bias, 4, sizeof(T)) && vec4(m.e.residual, m.e.ldr, sizeof(T)) && vec4(m.e.out, m.e.ldo, sizeof(T)) &&
+            vec4(m.e.preact, m.J, sizeof(T));
+  if constexpr (P == 3) {
+    j.e.a = {static_cast<const bf16_t*>(a.p), a.rows * a.ld, a.strided ? 1 : a.ld, a.strided ? a.ld : 1};
+    j.e.b = {static_cast<const bf16_t*>(b.p), b.rows * b.ld, b.strided ? 1 : b.ld, b.strided ? b.ld : 1};
+    j.e.K = m.K;
+  }
+  const PlanePick pick = pick_for(dt, m.I, m.J, m.K);
+  if (a0.strided) plane_run<PT, P, true, true, false>(jobs, pick, reinterpret_cast<float*>(at), st);
+  else if (b0.strided) plane_run<PT, P, false, true, false>(jobs, pick, reinterpret_cast<float*>(at), st);
+  else plane_run<PT, P, false, false, false>(jobs, pick, reinterpret_cast<float*>(at), st);
+}
+
+// C = A B^T with m's epilogue; m.a / m.b: the operands as the tensors they are
+void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void* ws, hipStream_t st) {
+  if (m.I == 0 || m.J == 0) return;
+  if (mat_route(dt, m.I, m.J, m.K) == ROUTE_MAT) {
+    if (a.strided) mat_run<true, true>(dt, m, ws, st);
+    else if (b.strided) mat_run<false, true>(dt, m, ws, st);
+    else mat_run<false, false>(dt, m, ws, st);
+  } else if (dt == CGAN3D_DT_F32) {
+    planes_run<float, bf16_t, 3>(dt, a, b, m, ws, st);
+  } else if (dt == CGAN3D_DT_BF16) {
+    planes_run<bf16_t, bf16_t, 1>(dt, a, b, m, ws, st);
+  } else {
+    planes_run<f16_t, f16_t, 1>(dt, a, b, m, ws, st);
+  }
+}
+
+// --- a few rows: the weight is read once, 16 bytes a lane, and nothing else matters ---
+// A wave takes R = 2 columns of y; KW waves of the block share the summed axis (1, or 4 where there are few
+// columns).  Measured: see DESIGN's table.
+template <typename T, int M, int KW>
+__global__ __launch_bounds__(256) void gemv_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
+                                                   long long ldw, int n, int k, int vec, MatEpi e) {
+  constexpr int V = MatT<T>::VEC, R = 2;
+  typedef T vecT __attribute__((ext_vector_type(V)));
+  __shared__ float red[4][M * R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % KW;
+  const int j0 = (blockIdx.x * (4 / KW) + wave / KW) * R;
+  float acc[M][R] = {};
+  if (j0 < n) {
+    const T* wr[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) wr[r] = w + std::min(j0 + r, n - 1) * ldw;
+    int t = (part * 64 + lane) * V;
+    if (vec) {
+#pragma unroll 4
+      for (; t + V <= k; t += KW * 64 * V) {
+        vecT xv[M], wv[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) wv[r] = *reinterpret_cast<const vecT*>(wr[r] + t);
+#pragma unroll
+        for (int m = 0; m < M; ++m) xv[m] = *reinterpret_cast<const vecT*>(x + m * ldx + t);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int q = 0; q < V; ++q) acc[m][r] = fmaf(to_f(xv[m][q]), to_f(wv[r][q]), acc[m][r]);
+      }
+    }
+    // unaligned rows, and the last values of aligned ones
+    for (; t < k; t += KW * 64 * V)
+      for (int q = 0; q < V && t + q < k; ++q)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[m][r] = fmaf(to_f(x[m * ldx + t + q]), to_f(wr[r][t + q]), acc[m][r]);
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[m][r] = wave_sum(acc[m][r]);
+  if constexpr (KW > 1) {
+    if (lane == 0)
+#pragma unroll
+      for (int q = 0; q < M * R; ++q) red[wave][q] = acc[q / R][q % R];
+    __syncthreads();
+    if (wave == 0 && lane < M * R && j0 + lane % R < n)
+      mat_store<T>(e, n, lane / R, j0 + lane % R, (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+  } else {
+#pragma unroll
+    for (int q = 0; q < M * R; ++q)
+      if (lane == q && j0 + q % R < n) mat_store<T>(e, n, q / R, j0 + q % R, acc[q / R][q % R]);
+  }
+}
+
+template <typename T, int M> void gemv_run_m(const MatArgs& p, hipStream_t st) {
+  const T* x = static_cast<const T*>(p.a);
+  const T* w = static_cast<const T*>(p.b);
+  const int V = MatT<T>::VEC, n = (int)p.J, k = (int)p.K;
+  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
+                  (M == 1 || p.lda % V == 0) && (n == 1 || p.ldb % V == 0);
+  // two columns a wave: below 8 waves a CU the summed axis is shared by four waves
+  if (n / 2 >= 8 * cu_count())
+    launch(gemv_kernel<T, M, 1>, dim3((n + 7) / 8), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, vec, p.e);
+  else
+    launch(gemv_kernel<T, M, 4>, dim3((n + 1) / 2), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, vec, p.e);
+}
+template <typename T> void gemv_run(const MatArgs& p, hipStream_t st) {
+  if (p.I == 1) gemv_run_m<T, 1>(p, st);
+  else if (p.I == 2) gemv_run_m<T, 2>(p, st);
+  else if (p.I == 3) gemv_run_m<T, 3>(p, st);
+  else gemv_run_m<T, 4>(p, st);
+}
+
+// --- dz = dy * act'(z), and its column sums ---
+// CT threads of a block along the columns (V values each), the rest along the rows; column sums in 32 bits, of dz
+// before its rounding, into part [blockIdx.y][n].  dz goes to rows of ldz values whose padding is zeroed:
+// as it is, or (PL3) split into three planes.
+template <typename T, bool PL3>
+__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, long long lddy,
+                                                       const typename PreT<T>::type* __restrict__ pre, void* __restrict__ dzv,
+                                                       int ldz, float* __restrict__ part, long long rows, int n,
+                                                       long long chunk, int act, float slope, int ct, int vec) {
+  constexpr int V = MatT<T>::VEC;
+  typedef typename PreT<T>::type preT;
+  typedef T vecT __attribute__((ext_vector_type(V)));
+  typedef preT vecP __attribute__((ext_vector_type(V)));
+  __shared__ float red[256 * V];
+  const int c = threadIdx.x % ct, r = threadIdx.x / ct, rt = 256 / ct;
+  const int j = (blockIdx.x * ct + c) * V;
+  const long long i1 = std::min(rows, ((long long)blockIdx.y + 1) * chunk);
+  float s[V] = {};
+  if (j < n || (dzv && j < ldz)) {
+    for (long long i = (long long)blockIdx.y * chunk + r; i < i1; i += rt) {
+      float v[V];
+      if (vec && j + V <= n) {
+        const vecT y = *reinterpret_cast<const vecT*>(dy + i * lddy + j);
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = to_f(y[q]);
+        if (act != CGAN3D_ACT_NONE) {
+          const vecP z = *reinterpret_cast<const vecP*>(pre + i * n + j);
+#pragma unroll
+          for (int q = 0; q < V; ++q) v[q] *= mat_act_grad(to_f(z[q]), act, slope);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          v[q] = 0.f;
+          if (j + q < n) {
+            v[q] = to_f(dy[i * lddy + j + q]);
+            if (act != CGAN3D_ACT_NONE) v[q] *= mat_act_grad(to_f(pre[i * n + j + q]), act, slope);
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < V; ++q) s[q] += v[q];
+      if (!dzv) continue;
+      if constexpr (PL3) {
+        bf16x4_m h, m, l;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          bf16_t t[3];
+          split3(v[q], t);
+          h[q] = t[0];
+          m[q] = t[1];
+          l[q] = t[2];
+        }
+        bf16_t* d = static_cast<bf16_t*>(dzv) + i * ldz + j;
+        *reinterpret_cast<bf16x4_m*>(d) = h;
+        *reinterpret_cast<bf16x4_m*>(d + rows * ldz) = m;
+        *reinterpret_cast<bf16x4_m*>(d + 2 * rows * ldz) = l;
+      } else {
+        vecT o;
+#pragma unroll
+        for (int q = 0; q < V; ++q) o[q] = from_f<T>(v[q]);
+        *reinterpret_cast<vecT*>(static_cast<T*>(dzv) + i * ldz + j) = o;
+      }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int q = 0; q < V; ++q) red[(r * V + q) * ct + c] = s[q];
   __syncthreads();
-  if (r == 0 && j < n && part) part[(long long)blockIdx.y * n + j] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  for (int u = threadIdx.x; u < ct * V; u += 256) {
+    float a = 0.f;
+    for (int w = 0; w < rt; ++w) a += red[w * V * ct + u];
+    const int col = (blockIdx.x * ct + u % ct) * V + u / ct;
+    if (col < n) part[(long long)blockIdx.y * n + col] = a;
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict__ part, int nb, int n, T* __restrict__ db) {
-  const long long j = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
+  // 16 columns a block, 16 threads on each, added in a fixed order
+  __shared__ double red[16][16];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const long long j = (long long)blockIdx.x * 16 + c;
   double s = 0.;
-  for (int b = 0; b < nb; ++b) s += part[(long long)b * n + j];
-  db[j] = from_f<T>((float)s);
+  if (j < n)
+    for (int b = r; b < nb; b += 16) s += part[(long long)b * n + j];
+  red[r][c] = s;
+  __syncthreads();
+  if (r == 0 && j < n) {
+    for (int q = 1; q < 16; ++q) s += red[q][c];
+    db[j] = from_f<T>((float)s);
+  }
 }
 
-long long act_chunk(long long rows, int n) {
-  const long long cols = (n + 63) / 64;
-  const long long want = std::max(1LL, 8LL * cu_count() / cols);
-  return std::max(16LL, (rows + want - 1) / want);
+struct ActGrid {
+  int ct, bx;
+  long long chunk, nb;
+};
+ActGrid act_grid(const cgan3d_linear_args* a) {
+  const int v = a->dtype == CGAN3D_DT_F32 ? 4 : 8;
+  ActGrid g;
+  const long long width = up8(a->n);
+  g.ct = 1;
+  while (g.ct < 32 && g.ct * v < width) g.ct *= 2;
+  g.bx = (int)((width + g.ct * v - 1) / (g.ct * v));
+  const long long want = std::max(1LL, 8LL * cu_count() / std::max(1, g.bx));
+  g.chunk = std::max((long long)(256 / g.ct), (a->rows + want - 1) / want);
+  g.nb = (a->rows + g.chunk - 1) / g.chunk;
+  return g;
 }
 
-template <typename T>
-void act_grad_run(const cgan3d_linear_args* a, T* dz, float* part, hipStream_t st) {
-  const long long chunk = act_chunk(a->rows, a->n), nb = (a->rows + chunk - 1) / chunk;
-  if (nb > 0 && a->n > 0)
-    launch(act_grad_kernel<T>, dim3((a->n + 63) / 64, (unsigned)nb), dim3(256), 0, st, static_cast<const T*>(a->dy),
-           (long long)a->lddy, static_cast<const typename PreT<T>::type*>(a->preact), dz, part, (long long)a->rows,
-           a->n, chunk, a->act, a->slope);
+// dz: null where dy itself serves (no activation, rows that the products can read)
+template <typename T, bool PL3>
+void act_grad_run(const cgan3d_linear_args* a, void* dz, int ldz, float* part, hipStream_t st) {
+  const ActGrid g = act_grid(a);
+  const int vec = reinterpret_cast<uintptr_t>(a->dy) % 16 == 0 && a->lddy % MatT<T>::VEC == 0 &&
+                  (a->act == CGAN3D_ACT_NONE || (reinterpret_cast<uintptr_t>(a->preact) % 16 == 0 && a->n % MatT<T>::VEC == 0));
+  if (g.nb > 0 && a->n > 0)
+    launch(act_grad_kernel<T, PL3>, dim3(g.bx, (unsigned)g.nb), dim3(256), 0, st, static_cast<const T*>(a->dy),
+           (long long)a->lddy, static_cast<const typename PreT<T>::type*>(a->preact), dz, ldz, part, (long long)a->rows,
+           a->n, g.chunk, a->act, a->slope, g.ct, vec);
   if (a->dbias && a->n > 0)
-    launch(bias_join_kernel<T>, dim3((a->n + 255) / 256), dim3(256), 0, st, (const float*)part, (int)nb, a->n,
+    launch(bias_join_kernel<T>, dim3((a->n + 15) / 16), dim3(256), 0, st, (const float*)part, (int)g.nb, a->n,
            static_cast<T*>(a->dbias));
 }
 
-long long up256(long long v) { return (v + 255) / 256 * 256; }
-
-struct Bwd {  // workspace layout of the backward pass
+struct Bwd {  // the backward pass: dz, and where things lie in its workspace
+  bool has_dz, planes3;
+  int ldz;
   long long dz, part, mat, total;
+  Operand za, zb, x, w;  // dz summed over columns (dx) and over rows (dw)
 };
 Bwd bwd_layout(const cgan3d_linear_args* a) {
-  Bwd w;
-  w.dz = 0;
-  long long at = a->act != CGAN3D_ACT_NONE ? up256(a->rows * a->n * dt_bytes(a->dtype)) : 0;
+  Bwd w = {};
+  const int dt = a->dtype;
+  // both products take dz in one form: planes if either is better off with them
+  const bool rx = a->dx && mat_route(dt, a->rows, a->k, a->n) == ROUTE_PLANES && a->rows && a->k;
+  const bool rw = a->dw && mat_route(dt, a->n, a->k, a->rows) == ROUTE_PLANES && a->n && a->k;
+  w.planes3 = dt == CGAN3D_DT_F32 && rx && rw;
+  const bool direct = a->act == CGAN3D_ACT_NONE && !w.planes3 && (dt == CGAN3D_DT_F32 || chunked(a->dy, a->lddy, a->n));
+  w.has_dz = !direct && (a->dx || a->dw);
+  w.ldz = (int)up8(a->n);
+  long long at = w.has_dz ? up256(a->rows * w.ldz * (w.planes3 ? 6 : dt_bytes(dt))) : 0;
   w.part = at;
-  const long long chunk = act_chunk(a->rows, a->n);
-  if (a->dbias) at += up256((a->rows + chunk - 1) / chunk * a->n * 4);
+  if (a->dbias) at += up256(act_grid(a).nb * a->n * 4);
   w.mat = at;
-  const long long m1 = a->dx ? mat_ws_bytes(a->rows, a->k, a->n) : 0, m2 = a->dw ? mat_ws_bytes(a->n, a->k, a->rows) : 0;
+  const bool pl = w.planes3 || (dt != CGAN3D_DT_F32);
+  w.za = {a->dy, a->lddy, a->rows, a->n, false, pl};
+  if (w.has_dz) w.za.ld = w.ldz;
+  w.zb = w.za;
+  w.zb.strided = true;
+  w.x = {a->x, a->ldx, a->rows, a->k, true, false};
+  w.w = {a->w, a->ldw, a->n, a->k, true, false};
+  const long long m1 = a->dx ? product_bytes(dt, w.za, w.w, a->rows, a->k, a->n) : 0;
+  const long long m2 = a->dw ? product_bytes(dt, w.zb, w.x, a->n, a->k, a->rows) : 0;
   w.total = at + std::max(m1, m2);  // the two products run one after the other
   return w;
+}
+
+// the forward product's operands, and its workspace
+void fwd_operands(const cgan3d_linear_args* a, Operand* x, Operand* w) {
+  *x = {a->x, a->ldx, a->rows, a->k, false, false};
+  *w = {a->w, a->ldw, a->n, a->k, false, false};
+}
+long long fwd_bytes(const cgan3d_linear_args* a) {
+  if (a->rows <= kGemvRows) return 0;
+  Operand x, w;
+  fwd_operands(a, &x, &w);
+  return product_bytes(a->dtype, x, w, a->rows, a->n, a->k);
 }
 
 const char* lin_check(const cgan3d_linear_args* a, bool bwd) {
@@ -174,13 +586,13 @@ extern "C" int64_t cgan3d_linear_fwd_ws_bytes(const cgan3d_linear_args* a) {
     set_error("cgan3d_linear_fwd_ws_bytes: %s", e);
     return -1;
   }
-  return mat_ws_bytes(a->rows, a->n, a->k);
+  return fwd_bytes(a);
 }
 
 extern "C" int cgan3d_linear_fwd(const cgan3d_linear_args* a, void* ws, int64_t ws_bytes, void* stream) try {
   const char* e = lin_check(a, false);
   CG_CHECK_ARG(!e, "cgan3d_linear_fwd: %s", e);
-  const long long need = mat_ws_bytes(a->rows, a->n, a->k);
+  const long long need = fwd_bytes(a);
   CG_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
                "cgan3d_linear_fwd: workspace of %lld bytes (16-byte aligned) needed, got %lld", need, (long long)ws_bytes);
   const int b = dt_bytes(a->dtype), pb = a->dtype == CGAN3D_DT_F32 ? 4 : 2;
@@ -195,7 +607,17 @@ extern "C" int cgan3d_linear_fwd(const cgan3d_linear_args* a, void* ws, int64_t 
   p.b = a->w; p.ldb = a->ldw;
   p.I = a->rows; p.J = a->n; p.K = a->k;
   p.e = {a->bias, a->residual, a->ldr, a->preact, a->y, a->ldy, 1.f, 1.f, a->act, a->slope};
-  mat_run<false, false>(a->dtype, p, ws, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (a->rows == 0 || a->n == 0) return CGAN3D_OK;
+  if (a->rows <= kGemvRows) {
+    if (a->dtype == CGAN3D_DT_F32) gemv_run<float>(p, st);
+    else if (a->dtype == CGAN3D_DT_BF16) gemv_run<bf16_t>(p, st);
+    else gemv_run<f16_t>(p, st);
+  } else {
+    Operand x0, w0;
+    fwd_operands(a, &x0, &w0);
+    product(a->dtype, x0, w0, p, ws, st);
+  }
   CG_LAUNCH_CHECK("cgan3d_linear_fwd");
   return CGAN3D_OK;
 } catch (...) {
@@ -230,31 +652,35 @@ extern "C" int cgan3d_linear_bwd(const cgan3d_linear_args* a, void* ws, int64_t 
   }
   hipStream_t st = (hipStream_t)stream;
   char* base = static_cast<char*>(ws);
-  const bool act = a->act != CGAN3D_ACT_NONE;
-  void* dz = act ? base + l.dz : nullptr;
+  void* dz = l.has_dz ? base + l.dz : nullptr;
   float* part = a->dbias ? reinterpret_cast<float*>(base + l.part) : nullptr;
-  if (a->dbias || (act && (a->dx || a->dw))) {
-    if (a->dtype == CGAN3D_DT_F32) act_grad_run<float>(a, (float*)dz, part, st);
-    else if (a->dtype == CGAN3D_DT_BF16) act_grad_run<bf16_t>(a, (bf16_t*)dz, part, st);
-    else act_grad_run<f16_t>(a, (f16_t*)dz, part, st);
+  if (a->dbias || l.has_dz) {
+    if (l.planes3) act_grad_run<float, true>(a, dz, l.ldz, part, st);
+    else if (a->dtype == CGAN3D_DT_F32) act_grad_run<float, false>(a, dz, l.ldz, part, st);
+    else if (a->dtype == CGAN3D_DT_BF16) act_grad_run<bf16_t, false>(a, dz, l.ldz, part, st);
+    else act_grad_run<f16_t, false>(a, dz, l.ldz, part, st);
   }
   MatArgs p = {};
-  p.a = act ? dz : a->dy;
-  p.lda = act ? a->n : a->lddy;
+  p.a = l.has_dz ? dz : a->dy;
+  p.lda = l.has_dz ? l.ldz : a->lddy;
   p.e.alpha = 1.f;
   if (a->dx) {
     MatArgs q = p;
+    Operand z = l.za;
+    z.p = p.a;
     q.b = a->w; q.ldb = a->ldw;
     q.I = a->rows; q.J = a->k; q.K = a->n;
     q.e.out = a->dx; q.e.ldo = a->lddx;
-    mat_run<false, true>(a->dtype, q, base + l.mat, st);
+    product(a->dtype, z, l.w, q, base + l.mat, st);
   }
   if (a->dw) {
     MatArgs q = p;
+    Operand z = l.zb;
+    z.p = p.a;
     q.b = a->x; q.ldb = a->ldx;
     q.I = a->n; q.J = a->k; q.K = a->rows;
     q.e.out = a->dw; q.e.ldo = a->k;
-    mat_run<true, true>(a->dtype, q, base + l.mat, st);
+    product(a->dtype, z, l.x, q, base + l.mat, st);
   }
   CG_LAUNCH_CHECK("cgan3d_linear_bwd");
   return CGAN3D_OK;
