@@ -64,6 +64,7 @@ constexpr int kGemvRows = 4;
 // Epilogue of a plane product.  NANFIX (f32 on three planes): an infinity times an empty lower plane
 // is NaN, so a NaN sum is computed again value by value, which leaves what f32 gives.
 template <typename T, bool NANFIX> struct LinEpi {
+  static constexpr bool STAGED = true;
   MatEpi e;
   long long J;
   int vec;  // every tensor of the epilogue takes vectors of four
@@ -82,50 +83,67 @@ template <typename T, bool NANFIX> struct LinEpi {
     for (long long t = 0; t < K; ++t) s = fmaf(a.at(i, t), b.at(j, t), s);
     return s;
   }
-  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+  // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store, so that they are in
+  // flight together
+  template <int STEP>
+  __device__ __forceinline__ void put4(int i, int j, f32x4_m* v, int I, int jn) const {
     if constexpr (NANFIX) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < jn && v[r] != v[r]) v[r] = again(i, j + r);
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (i + u * STEP < I && r < jn && v[u][r] != v[u][r]) v[u][r] = again(i + u * STEP, j + r);
     }
     if (jn < 4 || !vec) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < jn) mat_store<T>(e, J, i, j + r, v[r]);
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (i + u * STEP < I && r < jn) mat_store<T>(e, J, i + u * STEP, j + r, v[u][r]);
       return;
     }
     typedef T v4 __attribute__((ext_vector_type(4)));
     typedef typename PreT<T>::type preT;
     typedef preT p4 __attribute__((ext_vector_type(4)));
-    v *= e.alpha;
-    if (e.bias) {
-      const v4 b = *reinterpret_cast<const v4*>(static_cast<const T*>(e.bias) + j);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += to_f(b[r]);
-    }
-    if (e.preact) {
-      p4 p;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        preT q;
-        mat_preact(&q, v[r]);
-        p[r] = q;
-      }
-      *reinterpret_cast<p4*>(static_cast<preT*>(e.preact) + i * J + j) = p;
-    }
-    if (e.act != CGAN3D_ACT_NONE) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = mat_act(v[r], e.act, e.slope);
-    }
+    v4 res[4], bias;
+    if (e.bias) bias = *reinterpret_cast<const v4*>(static_cast<const T*>(e.bias) + j);
     if (e.residual) {
-      const v4 b = *reinterpret_cast<const v4*>(static_cast<const T*>(e.residual) + i * e.ldr + j);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += e.beta * to_f(b[r]);
+      for (int u = 0; u < 4; ++u)
+        res[u] = *reinterpret_cast<const v4*>(static_cast<const T*>(e.residual) + min(i + u * STEP, I - 1) * e.ldr + j);
     }
-    v4 o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = from_f<T>(v[r]);
-    *reinterpret_cast<v4*>(static_cast<T*>(e.out) + i * e.ldo + j) = o;
+    for (int u = 0; u < 4; ++u) {
+      v[u] *= e.alpha;
+      if (e.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[u][r] += to_f(bias[r]);
+      }
+      if (e.preact && i + u * STEP < I) {
+        p4 p;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          preT q;
+          mat_preact(&q, v[u][r]);
+          p[r] = q;
+        }
+        *reinterpret_cast<p4*>(static_cast<preT*>(e.preact) + (i + u * STEP) * J + j) = p;
+      }
+    }
+    mat_act16<T>(reinterpret_cast<float*>(v), e.act, e.slope);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i + u * STEP >= I) continue;
+      v4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = from_f<T>(e.residual ? v[u][r] + e.beta * to_f(res[u][r]) : v[u][r]);
+      *reinterpret_cast<v4*>(static_cast<T*>(e.out) + (i + u * STEP) * e.ldo + j) = o;
+    }
+  }
+  // the joined sums, a row at a time
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+    f32x4_m w[4] = {v};
+    put4<1>(i, j, w, i + 1, jn);
   }
 };
 
@@ -392,7 +410,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
         if (act != CGAN3D_ACT_NONE) {
           const vecP z = *reinterpret_cast<const vecP*>(pre + i * n + j);
 #pragma unroll
-          for (int q = 0; q < V; ++q) v[q] *= mat_act_grad(to_f(z[q]), act, slope);
+          for (int q = 0; q < V; ++q) v[q] *= mat_act_grad<sizeof(T) == 2>(to_f(z[q]), act, slope);
         }
       } else {
 #pragma unroll
@@ -400,7 +418,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
           v[q] = 0.f;
           if (j + q < n) {
             v[q] = to_f(dy[i * lddy + j + q]);
-            if (act != CGAN3D_ACT_NONE) v[q] *= mat_act_grad(to_f(pre[i * n + j + q]), act, slope);
+            if (act != CGAN3D_ACT_NONE) v[q] *= mat_act_grad<sizeof(T) == 2>(to_f(pre[i * n + j + q]), act, slope);
           }
         }
       }

@@ -172,6 +172,7 @@ constexpr float kXs = 4096.f, kAs = 1024.f;
 
 // A = X X^T (beta 0) or B = b A + c A A, from sums in the operands' scales to planes in A's
 struct GramEpi {
+  static constexpr bool STAGED = false;
   f16_t* out;
   const f16_t* in;  // A's planes
   int ld, n;        // row stride, side
@@ -250,6 +251,7 @@ struct GramEpi {
 
 // X <- a X + B X: to planes, or where it is the last step to the result / the parameter
 struct StepEpi {
+  static constexpr bool STAGED = false;
   f16_t* out;
   const f16_t* in;  // X's planes
   long long plane;

@@ -50,7 +50,7 @@ template <class E, int N> struct PlaneJobs {
 // neighbouring rows, which then lie in 16 different 16-byte columns of the 256-byte bank space.  t-strided
 // rows: a wave reads 32 bytes of rows 8 g + 4 h + (0..3), g = 0..3: the eight rows of a half wave get eight
 // different 32-byte columns (rows of 256 bytes or more; of 128 bytes: four, and the row's own parity).
-template <int CH> __device__ __forceinline__ int sw_kc(int r) { return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
+template <int CH> __device__ __forceinline__ int sw_kc(int r) { return CH == 8 ? (r >> 1) & 7 : -(r >> 2) & 3; }
 template <int CH> __device__ __forceinline__ int sw_ks(int k) {
   return CH >= 16 ? 2 * ((k & 3) + 4 * ((k >> 3) & 1)) : 2 * (((k >> 1) & 1) + 2 * ((k >> 3) & 1));
 }
@@ -146,6 +146,7 @@ template <int BM, bool SYM> __device__ __forceinline__ void plane_tile(int t, in
   }
 }
 
+template <int N> __device__ __forceinline__ void wait_vm_only() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
 // One BM x BN tile, WI x WJ waves, BK values of t a stage, S stage buffers: S - 1 stages are in flight ahead.
@@ -192,19 +193,24 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
     }
   };
   f32x4_m acc[FM][FN] = {};
-  s16x8_v fb[P][FN], fa[2][P];  // B's fragments of the unit, A's first two rows of them
-  const auto read_a = [&](s16x8_v(&f)[P], int m, int h) {
-    const unsigned char* la = lds + slot * STAGE;
+  const auto wait_stage = [&](bool all) {  // all but the requests of the S - 2 stages behind
+    if (S > 2 && !all) wait_vm<(S - 2) * REQ>();
+    else wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  const auto read_a = [&](s16x8_v(&f)[P], int at, int m, int h) {
+    const unsigned char* la = lds + at * STAGE;
 #pragma unroll
     for (int q = 0; q < P; ++q) f[q] = plane_frag<AT, BM, BK>(la + q * TA::BYTES, wi + m * 16, h, lane);
   };
-  const auto read_b = [&](int n, int h) {
-    const unsigned char* lb = lds + slot * STAGE + P * TA::BYTES;
+  const auto read_b = [&](s16x8_v(&f)[P][FN], int at, int n, int h) {
+    const unsigned char* lb = lds + at * STAGE + P * TA::BYTES;
 #pragma unroll
-    for (int q = 0; q < P; ++q) fb[q][n] = plane_frag<BT, BN, BK>(lb + q * TB::BYTES, wj + n * 16, h, lane);
+    for (int q = 0; q < P; ++q) f[q][n] = plane_frag<BT, BN, BK>(lb + q * TB::BYTES, wj + n * 16, h, lane);
   };
   // small products first; operands swapped, so that a lane ends up with neighbouring columns
-  const auto row = [&](int m, const s16x8_v(&a)[P]) {
+  const auto row = [&](int m, const s16x8_v(&a)[P], const s16x8_v(&fb)[P][FN]) {
 #pragma unroll
     for (int o = P - 1; o >= 0; --o)
 #pragma unroll
@@ -212,57 +218,89 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
 #pragma unroll
         for (int n = 0; n < FN; ++n) acc[m][n] = plane_mfma(fb[o - q][n], a[q], acc[m][n], T());
   };
-  // waits until stage s + 1 (of `steps`) has landed; s + S - 1 is the last one requested
-  const auto landed = [&](int s) {
-    if (S > 2 && s + S - 1 < steps) wait_vm<(S - 2) * REQ>();
-    else wait_vm<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  const auto unit = [&](int s, int h) {
-    if (h == 0 && s + S - 1 < steps) issue(s + S - 1);
-    s16x8_v fr[FM][P];
-#pragma unroll
-    for (int m = 0; m < FM - 1; ++m) {
-      if (m + 2 < FM) read_a(fr[m + 2], m + 2, h);
-      if (m < 2) row(m, fa[m]);
-      else row(m, fr[m]);
-    }
-    s16x8_v last[P];
-#pragma unroll
-    for (int q = 0; q < P; ++q) last[q] = FM > 2 ? fr[FM - 1][q] : fa[1][q];
-    if (h + 1 == H && s + 1 < steps) {
-      landed(s);
+  if constexpr (P == 1) {
+    // One product a fragment pair: a stage's products are too few to hide the reads behind its barrier.  A whole
+    // stage of fragments is read a stage ahead: A's each into the registers of the row that has just used
+    // them, B's into a second set.  The barrier of stage s finds s + 1 landed and s - 1 read by every wave.
+    // Stages behind the last are requested and computed too, from the zero page (up to a whole pair): branches
+    // would cost more than they save.
+    static_assert(H == 1 && S >= 4, "stages: one being read late, one read, one landing, one requested");
+    s16x8_v fa[FM][1], fb[2][1][FN];
+    const auto stage = [&](int s, auto par) {
+      constexpr int c = decltype(par)::value;
+      wait_vm_only<(S - 3) * REQ>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      issue(s + S - 1);
       slot = slot + 1 == S ? 0 : slot + 1;
-    }
-    // behind the last stage these read that stage again, for nothing: a branch here would cut the row apart
-    const int hn = h + 1 < H ? h + 1 : 0;
-    read_a(fa[0], 0, hn);
-    read_a(fa[1], 1, hn);
 #pragma unroll
-    for (int n = 0; n < FN; ++n) {  // the last row column by column: its fragment of B is free behind it
+      for (int m = 0; m < FM; ++m) {
+        row(m, fa[m], fb[c]);
+        if (m < FN) read_b(fb[c ^ 1], slot, m, 0);
+        read_a(fa[m], slot, m, 0);
+      }
+    };
 #pragma unroll
-      for (int o = P - 1; o >= 0; --o)
-#pragma unroll
-        for (int q = 0; q <= o; ++q) acc[FM - 1][n] = plane_mfma(fb[o - q][n], last[q], acc[FM - 1][n], T());
-      read_b(n, hn);
-    }
-  };
-  if (steps > 0) {
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s)
-      if (s < steps) issue(s);
-    if (steps >= S - 1) wait_vm<(S - 2) * REQ>();
-    else wait_vm<0>();
+    for (int s = 0; s < S - 1; ++s) issue(s);
+    wait_vm_only<(S - 2) * REQ>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read_a(fa[0], 0, 0);
 #pragma unroll
-    for (int n = 0; n < FN; ++n) read_b(n, 0);
-    read_a(fa[1], 1, 0);
-    for (int s = 0; s < steps; ++s)
+    for (int n = 0; n < FN; ++n) read_b(fb[0], 0, n, 0);
 #pragma unroll
-      for (int h = 0; h < H; ++h) unit(s, h);
+    for (int m = 0; m < FM; ++m) read_a(fa[m], 0, m, 0);
+    int s = 0;
+#pragma clang loop unroll(disable)
+    do {
+      stage(s, std::integral_constant<int, 0>());
+      stage(s + 1, std::integral_constant<int, 1>());
+      s += 2;
+    } while (s < steps);
+    wait_vm<0>();  // no request outlives the block
+  } else {
+    s16x8_v fb[P][FN], fa[2][P];  // B's fragments of the unit, A's first two rows of them
+    const auto unit = [&](int s, int h) {
+      if (h == 0 && s + S - 1 < steps) issue(s + S - 1);
+      s16x8_v fr[FM][P];
+#pragma unroll
+      for (int m = 0; m < FM - 1; ++m) {
+        if (m + 2 < FM) read_a(fr[m + 2], slot, m + 2, h);
+        if (m < 2) row(m, fa[m], fb);
+        else row(m, fr[m], fb);
+      }
+      s16x8_v last[P];
+#pragma unroll
+      for (int q = 0; q < P; ++q) last[q] = FM > 2 ? fr[FM - 1][q] : fa[1][q];
+      if (h + 1 == H && s + 1 < steps) {
+        wait_stage(s + S - 1 >= steps);
+        slot = slot + 1 == S ? 0 : slot + 1;
+      }
+      // behind the last stage these read that stage again, for nothing: a branch here would cut the row apart
+      const int hn = h + 1 < H ? h + 1 : 0;
+      read_a(fa[0], slot, 0, hn);
+      read_a(fa[1], slot, 1, hn);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {  // the last row column by column: its fragment of B is free behind it
+#pragma unroll
+        for (int o = P - 1; o >= 0; --o)
+#pragma unroll
+          for (int q = 0; q <= o; ++q) acc[FM - 1][n] = plane_mfma(fb[o - q][n], last[q], acc[FM - 1][n], T());
+        read_b(fb, slot, n, hn);
+      }
+    };
+    if (steps > 0) {
+#pragma unroll
+      for (int s = 0; s < S - 1; ++s)
+        if (s < steps) issue(s);
+      wait_stage(steps < S - 1);
+      read_a(fa[0], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) read_b(fb, 0, n, 0);
+      read_a(fa[1], 0, 1, 0);
+      for (int s = 0; s < steps; ++s)
+#pragma unroll
+        for (int h = 0; h < H; ++h) unit(s, h);
+    }
   }
   if (p.part) {
     float* o = p.part + ((long long)split * p.tiles + t) * (BM * BN);
@@ -273,14 +311,44 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
         *reinterpret_cast<f32x4_m*>(o + (wi + m * 16 + (lane & 15)) * BN + wj + n * 16 + (lane >> 4) * 4) = acc[m][n];
     return;
   }
+  if constexpr (E::STAGED) {
+    // through LDS, a wave's own part of it, so that lanes go along the rows of the output: the epilogue's tensors
+    // are read and written in whole lines, and its code is there once per pass and not once per fragment
+    constexpr int MB = FM < 4 ? FM : 4, LD = WN + 4, LPR = WN / 4, IT = MB * 16 / (64 / LPR);
+    static_assert(NW * MB * 16 * LD * 4 <= S * STAGE && FM % MB == 0 && IT % 4 == 0, "a pass fits the stages' LDS");
+    float* my = reinterpret_cast<float*>(lds) + wave * (MB * 16 * LD);
+    const int lr = lane / LPR, j = j0 + wj + lane % LPR * 4;
+    __syncthreads();  // the last stage's fragments are read
 #pragma unroll
-  for (int m = 0; m < FM; ++m) {
-    const int i = i0 + wi + m * 16 + (lane & 15);
-    if (i < p.I) {
+    for (int mb = 0; mb < FM; mb += MB) {
 #pragma unroll
-      for (int n = 0; n < FN; ++n) {
-        const int j = j0 + wj + n * 16 + (lane >> 4) * 4;
-        if (j < p.J) p.e.put(i, j, acc[m][n], p.J - j, SYM && ti != tj);
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < FN; ++n)
+          *reinterpret_cast<f32x4_m*>(my + (m * 16 + (lane & 15)) * LD + n * 16 + (lane >> 4) * 4) = acc[mb + m][n];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j < p.J) {
+#pragma clang loop unroll(disable)
+        for (int it = 0; it < IT; it += 4) {
+          const int r = it * (64 / LPR) + lr;
+          f32x4_m v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f32x4_m*>(my + (r + u * (64 / LPR)) * LD + lane % LPR * 4);
+          p.e.template put4<64 / LPR>(i0 + wi + mb * 16 + r, j, v, p.I, p.J - j);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      const int i = i0 + wi + m * 16 + (lane & 15);
+      if (i < p.I) {
+#pragma unroll
+        for (int n = 0; n < FN; ++n) {
+          const int j = j0 + wj + n * 16 + (lane >> 4) * 4;
+          if (j < p.J) p.e.put(i, j, acc[m][n], p.J - j, SYM && ti != tj);
+        }
       }
     }
   }
@@ -322,7 +390,7 @@ struct PlanePick {
 // blocks where there are few
 template <int P> struct PlaneCfg;
 template <> struct PlaneCfg<1> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {4, 4, 4};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 5};
   static constexpr float RATE[3] = {1.f, 0.75f, 0.4f};
 };
 template <> struct PlaneCfg<2> {
