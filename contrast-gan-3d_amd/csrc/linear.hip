@@ -140,6 +140,8 @@ template <typename T, bool NANFIX> struct LinEpi {
       *reinterpret_cast<v4*>(static_cast<T*>(e.out) + (i + u * STEP) * e.ldo + j) = o;
     }
   }
+  __device__ __forceinline__ bool turned() const { return false; }
+  __device__ __forceinline__ void put_turned(int, int, f32x4_m, int) const {}
   // the joined sums, a row at a time
   __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
     f32x4_m w[4] = {v};
@@ -236,7 +238,7 @@ long long operand_bytes(int dt, const Operand& o) {
 }
 PlanePick pick_for(int dt, long long I, long long J, long long K) {
   const PlaneShape s = {(int)I, (int)J, (int)K};
-  return dt == CGAN3D_DT_F32 ? plane_pick<3>(&s, 1, false) : plane_pick<1>(&s, 1, false);
+  return dt == CGAN3D_DT_F32 ? plane_pick<3, false>(&s, 1) : plane_pick<1, false>(&s, 1);
 }
 // workspace of one product: both operands' planes, then partial sums
 long long product_bytes(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {

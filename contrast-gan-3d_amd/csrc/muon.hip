@@ -251,7 +251,7 @@ struct GramEpi {
 
 // X <- a X + B X: to planes, or where it is the last step to the result / the parameter
 struct StepEpi {
-  static constexpr bool STAGED = false;
+  static constexpr bool STAGED = true;
   f16_t* out;
   const f16_t* in;  // X's planes
   long long plane;
@@ -263,17 +263,13 @@ struct StepEpi {
   int tall;
   float scale;
   const float* hyper;
-  template <typename T> __device__ __forceinline__ void store(int i, int j, f32x4_m x, int jn) const {
-    T* p = static_cast<T*>(res);
-    if (tall) {  // 16 lanes write 16 neighbours
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < jn) p[(j + r) * ldr + i] = (T)x[r];
-      return;
-    }
-    p += i * ldr + j;
+
+  __device__ __forceinline__ bool turned() const { return tall && mode; }
+
+  // four values at p, neighbours in memory, n of them
+  template <typename T> static __device__ __forceinline__ void store(T* p, f32x4_m x, int n) {
     typedef T v4 __attribute__((ext_vector_type(4)));
-    if (jn >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0) {
+    if (n >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0) {
       v4 o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[r] = (T)x[r];
@@ -281,47 +277,70 @@ struct StepEpi {
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (r < jn) p[r] = (T)x[r];
+        if (r < n) p[r] = (T)x[r];
     }
   }
-  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
-    const long long o = (long long)i * ld + j;  // rows of whole 32s: four columns are always there to read
-    const f16x4_m a = *reinterpret_cast<const f16x4_m*>(in + o), c = *reinterpret_cast<const f16x4_m*>(in + plane + o);
-    f32x4_m x;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = alpha * v[r] + beta * ((float)a[r] + (float)c[r]);
-    if (mode == 0) {
-      f16x4_m h, l;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        f16_t s[2];
-        split2(r < jn ? x[r] : 0.f, s);  // the padding stays zero
-        h[r] = s[0];
-        l[r] = s[1];
-      }
-      *reinterpret_cast<f16x4_m*>(out + o) = h;
-      *reinterpret_cast<f16x4_m*>(out + plane + o) = l;
-      return;
-    }
+  // the last step's values x at offset d of the result or the parameter, n of them
+  __device__ __forceinline__ void finish(long long d, f32x4_m x, int n) const {
     x *= 1.f / kXs;
     if (mode == 1 + CGAN3D_DT_F32) {
-      store<float>(i, j, x, jn);
+      store(static_cast<float*>(res) + d, x, n);
     } else if (mode == 1 + CGAN3D_DT_BF16) {
-      store<bf16_t>(i, j, x, jn);
+      store(static_cast<bf16_t*>(res) + d, x, n);
     } else if (mode == 1 + CGAN3D_DT_F16) {
-      store<f16_t>(i, j, x, jn);
+      store(static_cast<f16_t*>(res) + d, x, n);
     } else {
-      float* p = static_cast<float*>(res);
+      float* p = static_cast<float*>(res) + d;
       const float lr = hyper[H_LR], clip = hyper[H_CLIP], keep = 1.f - lr * hyper[H_WD], rate = lr * scale;
+      f32x4_m w;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if (r >= jn) break;
-        const long long d = tall ? (j + r) * ldr + i : i * ldr + j + r;
-        float w = p[d] * keep - rate * x[r];
-        if (clip > 0.f) w = fminf(fmaxf(w, -clip), clip);
-        p[d] = w;
+        w[r] = r < n ? p[r] * keep - rate * x[r] : 0.f;
+        if (clip > 0.f) w[r] = fminf(fmaxf(w[r], -clip), clip);
+      }
+      store(p, w, n);
+    }
+  }
+  // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store
+  template <int STEP> __device__ __forceinline__ void put4(int i, int j, f32x4_m* v, int I, int jn) const {
+    f16x4_m a[4], c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long o = (long long)min(i + u * STEP, I - 1) * ld + j;  // rows of whole 32s: four columns are there
+      a[u] = *reinterpret_cast<const f16x4_m*>(in + o);
+      c[u] = *reinterpret_cast<const f16x4_m*>(in + plane + o);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[u][r] = alpha * v[u][r] + beta * ((float)a[u][r] + (float)c[u][r]);
+      if (i + u * STEP >= I || turned()) continue;
+      if (mode == 0) {
+        f16x4_m h, l;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f16_t s[2];
+          split2(r < jn ? v[u][r] : 0.f, s);  // the padding stays zero
+          h[r] = s[0];
+          l[r] = s[1];
+        }
+        const long long o = (long long)(i + u * STEP) * ld + j;
+        *reinterpret_cast<f16x4_m*>(out + o) = h;
+        *reinterpret_cast<f16x4_m*>(out + plane + o) = l;
+      } else {
+        finish((i + u * STEP) * ldr + j, v[u], jn);
       }
     }
+  }
+  // column j of the result, rows i .. i + 3 of the iterate
+  __device__ __forceinline__ void put_turned(int i, int j, f32x4_m v, int in_) const { finish(j * ldr + i, v, in_); }
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+    f32x4_m w[4] = {v};
+    put4<1>(i, j, w, i + 1, jn);
+    if (turned())
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < jn) finish((j + r) * ldr + i, f32x4_m{w[0][r], 0.f, 0.f, 0.f}, 1);
   }
 };
 
@@ -409,8 +428,8 @@ PlaneLayout plane_layout(const int (*sl)[2], int n, char* ws, PlaneMat* out) {
     step[i] = {s, l, lda};
   }
   w.part = w.bytes;
-  const long long f = std::max({plane_pick<2>(gram, n, true).part_floats, plane_pick<2>(poly, n, true).part_floats,
-                                plane_pick<2>(step, n, false).part_floats});
+  const long long f = std::max({plane_pick<2, true>(gram, n).part_floats, plane_pick<2, true>(poly, n).part_floats,
+                                plane_pick<2, false>(step, n).part_floats});
   w.bytes += up256(f * 4);
   return w;
 }
@@ -448,7 +467,7 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
                {p.y, p.x, xp, p.ldx, 0, 1.f / kAs, co[0], l.m[i].out, l.m[i].ldo, l.m[i].rows > l.m[i].cols,
                 l.m[i].scale, hyper}};
   }
-  const PlanePick pg = plane_pick<2>(gram, n, true), pp = plane_pick<2>(poly, n, true), ps = plane_pick<2>(step, n, false);
+  const PlanePick pg = plane_pick<2, true>(gram, n), pp = plane_pick<2, true>(poly, n), ps = plane_pick<2, false>(step, n);
   for (int k = 0; k < steps; ++k) {
     plane_run<f16_t, 2, false, false, true>(jg, pg, part, st);
     plane_run<f16_t, 2, false, false, true>(jp, pp, part, st);

@@ -153,7 +153,7 @@ template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_wai
 // The barrier that opens a new stage comes before the last row of products of the one before: they cover the
 // wait for the other waves and the reads of the next stage's first fragments, each of B's in the registers
 // of its predecessor right behind that one's last use.
-template <typename T, int P, bool AT, bool BT, int BM, int BN, int BK, int S, int WI, int WJ, bool SYM, class E, int N>
+template <typename T, int P, bool AT, bool BT, int BM, int BN, int BK, int S, int WI, int WJ, bool AHEAD, bool SYM, class E, int N>
 __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> jobs) {
   constexpr int NW = WI * WJ, WM = BM / WI, WN = BN / WJ, FM = WM / 16, FN = WN / 16, H = BK / 32;
   using TA = PlaneTile<AT, BM, BK, NW>;
@@ -218,14 +218,14 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
 #pragma unroll
         for (int n = 0; n < FN; ++n) acc[m][n] = plane_mfma(fb[o - q][n], a[q], acc[m][n], T());
   };
-  if constexpr (P == 1) {
-    // One product a fragment pair: a stage's products are too few to hide the reads behind its barrier.  A whole
-    // stage of fragments is read a stage ahead: A's each into the registers of the row that has just used
-    // them, B's into a second set.  The barrier of stage s finds s + 1 landed and s - 1 read by every wave.
+  if constexpr (AHEAD) {
+    // A whole stage of fragments is read a stage ahead: A's each into the registers of the row that has just used
+    // them, B's into a second set.  The barrier of stage s finds s + 1 landed and s - 1 read by every wave, and
+    // the products behind it need nothing that is not in registers.
     // Stages behind the last are requested and computed too, from the zero page (up to a whole pair): branches
     // would cost more than they save.
-    static_assert(H == 1 && S >= 4, "stages: one being read late, one read, one landing, one requested");
-    s16x8_v fa[FM][1], fb[2][1][FN];
+    static_assert(H == 1 && S >= 3, "stages: one read late, one being read, one landing");
+    s16x8_v fa[FM][P], fb[2][P][FN];
     const auto stage = [&](int s, auto par) {
       constexpr int c = decltype(par)::value;
       wait_vm_only<(S - 3) * REQ>();
@@ -237,6 +237,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
       for (int m = 0; m < FM; ++m) {
         row(m, fa[m], fb[c]);
         if (m < FN) read_b(fb[c ^ 1], slot, m, 0);
+        if (FN > FM && m + FM < FN) read_b(fb[c ^ 1], slot, m + FM, 0);
         read_a(fa[m], slot, m, 0);
       }
     };
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
   if constexpr (E::STAGED) {
     // through LDS, a wave's own part of it, so that lanes go along the rows of the output: the epilogue's tensors
     // are read and written in whole lines, and its code is there once per pass and not once per fragment
-    constexpr int MB = FM < 4 ? FM : 4, LD = WN + 4, LPR = WN / 4, IT = MB * 16 / (64 / LPR);
+    constexpr int LD = WN + 4, MB = FM >= 4 && NW * 64 * LD * 4 <= S * STAGE ? 4 : 2, LPR = WN / 4, IT = MB * 16 / (64 / LPR);
     static_assert(NW * MB * 16 * LD * 4 <= S * STAGE && FM % MB == 0 && IT % 4 == 0, "a pass fits the stages' LDS");
     float* my = reinterpret_cast<float*>(lds) + wave * (MB * 16 * LD);
     const int lr = lane / LPR, j = j0 + wj + lane % LPR * 4;
@@ -335,6 +336,24 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
 #pragma unroll
           for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f32x4_m*>(my + (r + u * (64 / LPR)) * LD + lane % LPR * 4);
           p.e.template put4<64 / LPR>(i0 + wi + mb * 16 + r, j, v, p.I, p.J - j);
+          if (p.e.turned()) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) *reinterpret_cast<f32x4_m*>(my + (r + u * (64 / LPR)) * LD + lane % LPR * 4) = v[u];
+          }
+        }
+      }
+      if (p.e.turned()) {  // a transposed output: lanes along its rows, which are the tile's columns
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        constexpr int LPC = MB * 4;  // lanes per column, four rows each
+        const int r = lane % LPC * 4, i = i0 + wi + mb * 16 + r;
+        if (i < p.I) {
+#pragma clang loop unroll(disable)
+          for (int c = lane / LPC; c < WN; c += 64 / LPC) {
+            f32x4_m v;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = my[(r + u) * LD + c];
+            if (j0 + wj + c < p.J) p.e.put_turned(i, j0 + wj + c, v, p.I - i);
+          }
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -388,17 +407,25 @@ struct PlanePick {
 };
 // tile configurations by planes: 0 the largest (8 waves, one block a CU), 1 and 2 smaller ones that give more
 // blocks where there are few
-template <int P> struct PlaneCfg;
-template <> struct PlaneCfg<1> {
+template <int P, bool SYM = false> struct PlaneCfg;
+template <> struct PlaneCfg<1, false> {
   static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 5};
+  static constexpr bool AHEAD[3] = {true, true, true};
   static constexpr float RATE[3] = {1.f, 0.75f, 0.4f};
 };
-template <> struct PlaneCfg<2> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {2, 2, 3};
+template <> struct PlaneCfg<2, false> {
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {3, 2, 3};
+  static constexpr bool AHEAD[3] = {true, false, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
-template <> struct PlaneCfg<3> {
+template <> struct PlaneCfg<2, true> {
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {2, 2, 3};
+  static constexpr bool AHEAD[3] = {false, false, true};
+  static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
+};
+template <> struct PlaneCfg<3, false> {
   static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 3};
+  static constexpr bool AHEAD[3] = {false, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 
@@ -411,8 +438,8 @@ inline long long plane_tiles(const PlaneShape& s, int bm, int bn, bool sym) {
 // with: the blocks that the fullest CU gets, at the rate a CU reaches with that tile (PlaneCfg::RATE), 64
 // t-values' worth of start and end per block, and the joining of partial sums (written and read once, a
 // launch of its own).
-template <int P> PlanePick plane_pick(const PlaneShape* s, int n, bool sym) {
-  using C = PlaneCfg<P>;
+template <int P, bool sym> PlanePick plane_pick(const PlaneShape* s, int n) {
+  using C = PlaneCfg<P, sym>;
   const double cus = cu_count(), rate = 1.1e15 / (P * (P + 1) / 2) / 2 / cus;  // products of a CU per second
   PlanePick best;
   double tb = 1e30;
@@ -449,7 +476,7 @@ template <int P> PlanePick plane_pick(const PlaneShape* s, int n, bool sym) {
 // Fills in tiles, splits, partial sums and block numbers (a, b, I, J, K and e are the caller's), and launches.
 template <typename T, int P, bool AT, bool BT, bool SYM, class E, int N>
 void plane_run(PlaneJobs<E, N>& jobs, const PlanePick& pick, float* part, hipStream_t st) {
-  using C = PlaneCfg<P>;
+  using C = PlaneCfg<P, SYM>;
   const auto go = [&](auto cfg) {
     constexpr int c = decltype(cfg)::value, BM = C::BM[c], BN = C::BN[c];
     int at = 0, jat = 0;
@@ -470,7 +497,7 @@ void plane_run(PlaneJobs<E, N>& jobs, const PlanePick& pick, float* part, hipStr
       jat += j.tiles * (BM / 32);
     }
     if (at == 0) return;
-    launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK, C::S[c], C::WI[c], C::WJ[c], SYM, E, N>, dim3(at),
+    launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK, C::S[c], C::WI[c], C::WJ[c], C::AHEAD[c], SYM, E, N>, dim3(at),
            dim3(C::WI[c] * C::WJ[c] * 64), 0, st, jobs);
     if (join) launch(plane_join_kernel<BM, BN, SYM, E, N>, dim3(jat), dim3(256), 0, st, js);
   };
