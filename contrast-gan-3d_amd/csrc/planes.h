@@ -414,13 +414,13 @@ template <> struct PlaneCfg<1, false> {
   static constexpr float RATE[3] = {1.f, 0.75f, 0.4f};
 };
 template <> struct PlaneCfg<2, false> {
-  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {3, 2, 3};
-  static constexpr bool AHEAD[3] = {true, false, true};
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {3, 3, 3};
+  static constexpr bool AHEAD[3] = {true, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<2, true> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {2, 2, 3};
-  static constexpr bool AHEAD[3] = {false, false, true};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 3};
+  static constexpr bool AHEAD[3] = {false, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<3, false> {
