@@ -484,6 +484,355 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
   }
 }
 
+// --- matrices with a short side of up to 64: the whole step in one launch ---
+// A block owns a slab of X, 128 columns of the long side (several in turn where there are more than kMaxSlabs), and
+// keeps it in LDS through a step; what the blocks of a matrix share is the 64 x 64 Gram matrix, whose partial
+// sums pass through memory between launches:
+//   launch 0:  G -> planes (and the momentum update), partial G G^T
+//   launch k:  A = sum of the partials, B = b A + c A A (every block for itself: 2 x 64^3), X <- a X + B X,
+//              partial X X^T for the next launch; the last one writes the result or the parameter
+// so five steps are six launches for up to kSlabMats matrices of any shapes, where the general products take
+// nineteen.  G's planes are scaled by the power of two of the slab's largest value, and the norm is the trace of
+// the partial Gram matrices, in 64 bits: no pass of its own.  Vectors' Adam rides on launch 0.
+constexpr int kSlabMats = 28, kMaxSlabs = 48, kSlabBytes = 64 * 128 * 4;
+
+struct SlabMat {
+  const void* g;    // G, or the gradient
+  void* out;        // the result, or the parameter
+  float* mom;       // muon: momentum (vectors: first moment)
+  float* sq;        // muon, vectors: second moment
+  long long ldg, ldo;
+  int rows, cols;   // rows 0: a vector of `count` values
+  float scale;
+  int nslab, sub;   // blocks, and slabs of 128 columns a block takes
+  long long count;
+  f16_t* x;         // planes, [slab][2][64][128], LDS order
+  float* part;      // [2][nslab][64 * 64]
+  float* expo;      // [nslab]: G = planes * 2^expo
+};
+struct SlabList {
+  int n, tick;  // tick: the last launch advances the step counter
+  int start[kSlabMats + 1];
+  SlabMat m[kSlabMats];
+};
+
+// place of 16-byte chunk c of row r: conflict-free for fragments along the row, two lanes a bank across it
+__device__ __forceinline__ int slab_at(int r, int c) { return r * 16 + (c ^ (r & 15)); }
+
+// 16 x 16 tiles (ti, tj) and (ti, tj + 1) of M M^T over 32 W columns, M's planes in rows of CH chunks
+template <int CH, int W>
+__device__ __forceinline__ void gram_tiles(const f16_t* m, int plane, int ti, int tj, int lane, f32x4_m (&acc)[2]) {
+  const auto frag = [&](int p, int row, int k) {
+    const int r = row * 16 + (lane & 15), c = k * 4 + (lane >> 4);
+    return *reinterpret_cast<const s16x8_v*>(m + p * plane + (CH == 16 ? slab_at(r, c) : r * CH + (c ^ sw_kc<8>(r))) * 8);
+  };
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    const s16x8_v a0 = frag(0, ti, k), a1 = frag(1, ti, k);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const s16x8_v b0 = frag(0, tj + u, k), b1 = frag(1, tj + u, k);
+      acc[u] = plane_mfma(b1, a0, acc[u], f16_t());
+      acc[u] = plane_mfma(b0, a1, acc[u], f16_t());
+      acc[u] = plane_mfma(b0, a0, acc[u], f16_t());
+    }
+  }
+}
+
+// PHASE 0: launch 0, 1: a step that is not the last, 2: the last
+template <typename T, int PHASE>
+__global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, float cb, float cc, float eps,
+                                                   float* __restrict__ hyper) {
+  __shared__ __align__(16) f16_t X[2 * 64 * 128];
+  __shared__ __align__(16) f16_t Y[2 * 64 * 128];
+  __shared__ __align__(16) f16_t A[2 * 64 * 64];
+  __shared__ __align__(16) f16_t B[2 * 64 * 64];
+  __shared__ double redd[8];
+  __shared__ float redf[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int mi = 0;
+  while (mi + 1 < l.n && (int)blockIdx.x >= l.start[mi + 1]) ++mi;
+  const SlabMat& m = l.m[mi];
+  const int slab = blockIdx.x - l.start[mi];
+  if (PHASE == 2 && hyper && l.tick && blockIdx.x == 0 && tid == 0) hyper[H_STEP] += 1.f;  // nothing of this launch reads it
+  if (m.rows == 0) {
+    if (PHASE == 0) {
+      const float h[6] = {hyper[H_VLR], hyper[H_VB1], hyper[H_VB2], hyper[H_VEPS], 0.f, hyper[H_CLIP]};
+      const AdamK ak = adam_k(h, hyper[H_STEP] + 1.f);
+      for (long long q = slab * 512LL + tid; q < m.count; q += m.nslab * 512LL)
+        adam_elem(ak, static_cast<float*>(m.out), static_cast<const float*>(m.g), m.mom, m.sq, q);
+    }
+    return;
+  }
+  const bool tall = m.rows > m.cols;
+  const int s = min(m.rows, m.cols), len = max(m.rows, m.cols);
+  f32x4_m gram[2] = {};
+  const int gi = wave >> 1, gj = (wave & 1) * 2;  // this wave's two tiles of a 64 x 64 matrix
+  f16_t* state = m.x + (long long)slab * m.sub * (2 * 64 * 128);
+
+  if constexpr (PHASE == 0) {
+    const float mu = hyper ? hyper[H_MU] : 0.f;
+    const bool nest = hyper && hyper[H_NESTEROV] != 0.f;
+    const T* g = static_cast<const T*>(m.g);
+    float v[16];
+    const auto load = [&](int b, bool keep) {
+      const int t0 = (slab * m.sub + b) * 128;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int q = u * 512 + tid, i = tall ? q % 64 : q / 128, t = t0 + (tall ? q / 64 : q % 128);
+        v[u] = 0.f;
+        if (i < s && t < len) {
+          const long long o = tall ? t * m.ldg + i : i * m.ldg + t;
+          v[u] = to_f(g[o]);
+          if (hyper) {
+            float w = m.mom[o];
+            w += (1.f - mu) * (v[u] - w);
+            if (keep) m.mom[o] = w;
+            v[u] = nest ? v[u] + mu * (w - v[u]) : w;
+          }
+        }
+      }
+    };
+    float big = 0.f;
+    for (int b = 0; b < m.sub; ++b) {
+      load(b, m.sub == 1);
+#pragma unroll
+      for (int u = 0; u < 16; ++u) big = fmaxf(big, fabsf(v[u]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+    if (lane == 0) redf[wave] = big;
+    __syncthreads();
+    big = redf[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) big = fmaxf(big, redf[w]);
+    // values below 2^12; nothing to scale by where all are zero or some are not finite
+    const int e = big > 0.f && big < __builtin_inff() ? ilogbf(big) + 1 - 12 : 0;
+    if (tid == 0) m.expo[slab] = (float)e;
+    for (int b = 0; b < m.sub; ++b) {
+      if (m.sub > 1) load(b, true);
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int q = u * 512 + tid, i = tall ? q % 64 : q / 128, t = tall ? q / 64 : q % 128;
+        f16_t p[2];
+        split2(ldexpf(v[u], -e), p);
+        const int o = slab_at(i, t >> 3) * 8 + (t & 7);
+        Y[o] = p[0];
+        Y[64 * 128 + o] = p[1];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        reinterpret_cast<s16x8_v*>(state + (long long)b * (2 * 64 * 128))[u * 512 + tid] = reinterpret_cast<s16x8_v*>(Y)[u * 512 + tid];
+      gram_tiles<16, 4>(Y, 64 * 128, gi, gj, lane, gram);
+      __syncthreads();
+    }
+  } else {
+    s16x8_v xr[4];  // the slab is on its way while the Gram matrix is put together
+#pragma unroll
+    for (int u = 0; u < 4; ++u) xr[u] = reinterpret_cast<const s16x8_v*>(state)[u * 512 + tid];
+    // A: a thread adds eight neighbours of a row over the slabs, in their order
+    const float* part = m.part + (long long)((k - 1) & 1) * m.nslab * 4096 + tid * 8;
+    const int ri = tid >> 3, rj = (tid & 7) * 8;
+    float sum[8];
+    float alpha = 1.f / kAs, beta = ca;
+    if (k == 1) {
+      double d[8] = {};
+#pragma unroll 2
+      for (int z = 0; z < m.nslab; ++z) {
+        const double f = ldexp(1.0, 2 * (int)m.expo[z]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4_m p = *reinterpret_cast<const f32x4_m*>(part + (long long)z * 4096 + h * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) d[h * 4 + r] += f * p[r];
+        }
+      }
+      double tr = 0.;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (rj + r == ri) tr = d[r];
+      tr = wave_sum_d(tr);
+      if (lane == 0) redd[wave] = tr;
+      __syncthreads();
+      tr = 0.;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) tr += redd[w];
+      const double norm = sqrt(tr) + (double)eps;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sum[r] = (float)(d[r] / (norm * norm));
+      // from G's planes to X's; a slab of zeros may have any factor but an infinite one
+      const float r0 = (float)fmin(ldexp(1.0, (int)m.expo[slab]) / norm * kXs, 1e38);
+      alpha *= r0;
+      beta *= r0;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sum[r] = 0.f;
+#pragma unroll 4
+      for (int z = 0; z < m.nslab; ++z) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4_m p = *reinterpret_cast<const f32x4_m*>(part + (long long)z * 4096 + h * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[h * 4 + r] += p[r];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sum[r] *= 1.f / (kXs * kXs);
+    }
+    {
+      f16x8_m hi, lo;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        f16_t p[2];
+        split2(sum[r] * kAs, p);
+        hi[r] = p[0];
+        lo[r] = p[1];
+      }
+      const int o = (ri * 8 + ((tid & 7) ^ sw_kc<8>(ri))) * 8;
+      *reinterpret_cast<f16x8_m*>(A + o) = hi;
+      *reinterpret_cast<f16x8_m*>(A + 64 * 64 + o) = lo;
+    }
+    __syncthreads();
+    f32x4_m sqr[2] = {};
+    gram_tiles<8, 2>(A, 64 * 64, gi, gj, lane, sqr);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = gi * 16 + (lane & 15), j = (gj + u) * 16 + (lane >> 4) * 4;
+      const int o = (i * 8 + ((j >> 3) ^ sw_kc<8>(i))) * 8 + (j & 7);
+      const f16x4_m h = *reinterpret_cast<const f16x4_m*>(A + o), lw = *reinterpret_cast<const f16x4_m*>(A + 64 * 64 + o);
+      f16x4_m oh, ol;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f16_t p[2];
+        split2(cc / kAs * sqr[u][r] + cb * ((float)h[r] + (float)lw[r]), p);
+        oh[r] = p[0];
+        ol[r] = p[1];
+      }
+      *reinterpret_cast<f16x4_m*>(B + o) = oh;
+      *reinterpret_cast<f16x4_m*>(B + 64 * 64 + o) = ol;
+    }
+    for (int b = 0; b < m.sub; ++b) {
+      if (b > 0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) xr[u] = reinterpret_cast<const s16x8_v*>(state + (long long)b * (2 * 64 * 128))[u * 512 + tid];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) reinterpret_cast<s16x8_v*>(X)[u * 512 + tid] = xr[u];
+      __syncthreads();
+      // a wave: 16 columns, all 64 rows
+      f32x4_m acc[4] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s16x8_v fx[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int kr = h * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2), c = wave * 2 + ((lane & 3) >> 1);
+          typedef __attribute__((address_space(3))) s16x4_v* lp;
+          const f16_t* base = X + p * 64 * 128 + (lane & 1) * 4;
+          const s16x4_v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(base + slab_at(kr, c) * 8));
+          const s16x4_v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(base + slab_at(kr + 4, c) * 8));
+          fx[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = q * 16 + (lane & 15), o = (r * 8 + ((h * 4 + (lane >> 4)) ^ sw_kc<8>(r))) * 8;
+          const s16x8_v b0 = *reinterpret_cast<const s16x8_v*>(B + o), b1 = *reinterpret_cast<const s16x8_v*>(B + 64 * 64 + o);
+          acc[q] = plane_mfma(fx[1], b0, acc[q], f16_t());
+          acc[q] = plane_mfma(fx[0], b1, acc[q], f16_t());
+          acc[q] = plane_mfma(fx[0], b0, acc[q], f16_t());
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = q * 16 + (lane & 15), t = wave * 16 + (lane >> 4) * 4;
+        const int o = slab_at(i, t >> 3) * 8 + (t & 7);
+        const f16x4_m h = *reinterpret_cast<const f16x4_m*>(X + o), lw = *reinterpret_cast<const f16x4_m*>(X + 64 * 128 + o);
+        f32x4_m x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = alpha * acc[q][r] + beta * ((float)h[r] + (float)lw[r]);
+        if constexpr (PHASE == 1) {
+          f16x4_m oh, ol;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f16_t p[2];
+            split2(x[r], p);
+            oh[r] = p[0];
+            ol[r] = p[1];
+          }
+          *reinterpret_cast<f16x4_m*>(Y + o) = oh;
+          *reinterpret_cast<f16x4_m*>(Y + 64 * 128 + o) = ol;
+        } else {  // f32, rows of 32 chunks
+          *reinterpret_cast<f32x4_m*>(reinterpret_cast<float*>(Y) + (i * 32 + ((t >> 2) ^ (i & 15))) * 4) = x;
+        }
+      }
+      __syncthreads();
+      if constexpr (PHASE == 1) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          reinterpret_cast<s16x8_v*>(state + (long long)b * (2 * 64 * 128))[u * 512 + tid] = reinterpret_cast<s16x8_v*>(Y)[u * 512 + tid];
+        gram_tiles<16, 4>(Y, 64 * 128, gi, gj, lane, gram);
+        __syncthreads();
+      } else {
+        const int t0 = (slab * m.sub + b) * 128;
+        const float lr = hyper ? hyper[H_LR] : 0.f, clip = hyper ? hyper[H_CLIP] : 0.f;
+        const float keep = hyper ? 1.f - lr * hyper[H_WD] : 0.f, rate = lr * m.scale;
+        const float* y = reinterpret_cast<const float*>(Y);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int q = u * 512 + tid, i = tall ? q % 64 : q / 128, t = tall ? q / 64 : q % 128;
+          if (i >= s || t0 + t >= len) continue;
+          const float x = y[(i * 32 + ((t >> 2) ^ (i & 15))) * 4 + (t & 3)] * (1.f / kXs);
+          const long long o = tall ? (t0 + t) * m.ldo + i : i * m.ldo + t0 + t;
+          if (hyper) {
+            float* p = static_cast<float*>(m.out);
+            float w = p[o] * keep - rate * x;
+            if (clip > 0.f) w = fminf(fmaxf(w, -clip), clip);
+            p[o] = w;
+          } else {
+            static_cast<T*>(m.out)[o] = from_f<T>(x);
+          }
+        }
+        __syncthreads();
+      }
+    }
+  }
+  if constexpr (PHASE != 2) {
+    float* part = m.part + ((long long)(k & 1) * m.nslab + slab) * 4096;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      *reinterpret_cast<f32x4_m*>(part + (gi * 16 + (lane & 15)) * 64 + (gj + u) * 16 + (lane >> 4) * 4) = gram[u];
+  }
+}
+
+bool slab_takes(long long rows, long long cols) { return std::min(rows, cols) <= 64; }
+
+// blocks of a matrix, and its part of the workspace from `ws` on
+long long slab_place(SlabMat& m, char* ws) {
+  const int len = std::max(m.rows, m.cols), n128 = (len + 127) / 128;
+  m.sub = (n128 + kMaxSlabs - 1) / kMaxSlabs;
+  m.nslab = (n128 + m.sub - 1) / m.sub;
+  const long long xb = (long long)m.nslab * m.sub * kSlabBytes, pb = 2LL * m.nslab * 4096 * 4;
+  m.x = reinterpret_cast<f16_t*>(ws);
+  m.part = reinterpret_cast<float*>(ws + xb);
+  m.expo = reinterpret_cast<float*>(ws + xb + pb);
+  return xb + pb + up256(m.nslab * 4);
+}
+
+// five launches and one per step; `hyper`: the Muon step of the list (f32)
+template <typename T>
+void slab_run(SlabList& l, int steps, const float* co, float eps, float* hyper, hipStream_t st) {
+  int at = 0;
+  for (int i = 0; i < l.n; ++i) {
+    l.start[i] = at;
+    at += l.m[i].nslab;
+  }
+  launch(slab_kernel<T, 0>, dim3(at), dim3(512), 0, st, l, 0, co[0], co[1], co[2], eps, hyper);
+  for (int k = 1; k < steps; ++k)
+    launch(slab_kernel<T, 1>, dim3(at), dim3(512), 0, st, l, k, co[0], co[1], co[2], eps, hyper);
+  launch(slab_kernel<T, 2>, dim3(at), dim3(512), 0, st, l, steps, co[0], co[1], co[2], eps, hyper);
+}
+
 // Whether iterates that start within |X| <= 1 stay where the planes hold them: |X| < 2^16 / kXs, |A| and |B|
 // (largest entry <= largest singular value) < 2^16 / kAs
 bool planes_hold(int steps, const float* co) {
@@ -535,7 +884,7 @@ template <class F> long long plane_bytes(int n, F rc) {
   for (int i = 0; i <= n; ++i) {
     long long r = 0, c = 0;
     if (i < n) rc(i, r, c);
-    if (r * c > 0) {
+    if (r * c > 0 && !slab_takes(r, c)) {
       sl[at][0] = (int)std::min(r, c);
       sl[at][1] = (int)std::max(r, c);
       ++at;
@@ -544,6 +893,24 @@ template <class F> long long plane_bytes(int n, F rc) {
       most = std::max(most, plane_layout(sl, at, nullptr, nullptr).bytes);
       at = 0;
     }
+  }
+  return most;
+}
+
+// the same of the largest group of kSlabMats matrices with a short side for slab_kernel
+template <class F> long long slab_bytes(int n, F rc) {
+  long long most = 0, sum = 0;
+  int at = 0;
+  for (int i = 0; i < n; ++i) {
+    long long r = 0, c = 0;
+    rc(i, r, c);
+    if (r * c == 0 || !slab_takes(r, c)) continue;
+    SlabMat m;
+    m.rows = (int)r;
+    m.cols = (int)c;
+    sum += slab_place(m, nullptr);
+    most = std::max(most, sum);
+    if (++at == kSlabMats) at = 0, sum = 0;
   }
   return most;
 }
@@ -600,7 +967,8 @@ const char* mats_check(const cgan3d_ortho_mat* m, int n, int dt) {
 Layout ortho_layout(const cgan3d_ortho_mat* m, int n) {
   Layout w = {};
   for (int i = 0; i < n; ++i) size_mat(w, m[i].rows, m[i].cols);
-  place(w, n, 0, plane_bytes(n, [&](int i, long long& r, long long& c) { r = m[i].rows; c = m[i].cols; }));
+  const auto rc = [&](int i, long long& r, long long& c) { r = m[i].rows; c = m[i].cols; };
+  place(w, n, 0, std::max(plane_bytes(n, rc), slab_bytes(n, rc)));
   return w;
 }
 
@@ -608,6 +976,24 @@ template <typename T>
 void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, char* ws, int steps, const float* co,
                float eps, hipStream_t st) {
   const bool planes = planes_hold(steps, co);
+  if (planes) {
+    SlabList sl = {};
+    long long used = 0;
+    for (int i = 0; i < n; ++i) {
+      const cgan3d_ortho_mat& q = mats[i];
+      if ((long long)q.rows * q.cols > 0 && slab_takes(q.rows, q.cols)) {
+        SlabMat& m = sl.m[sl.n++];
+        m = {};
+        m.g = q.g; m.out = q.out; m.ldg = q.ldg; m.ldo = q.ldo; m.rows = q.rows; m.cols = q.cols;
+        used += slab_place(m, ws + w.x + used);
+      }
+      if (sl.n == kSlabMats || (i == n - 1 && sl.n > 0)) {
+        slab_run<T>(sl, steps, co, eps, nullptr, st);
+        sl.n = 0;
+        used = 0;
+      }
+    }
+  }
   MatList l;
   int at = 0;
   const auto flush = [&]() {
@@ -625,7 +1011,7 @@ void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, cha
   };
   for (int i = 0; i < n; ++i) {
     const cgan3d_ortho_mat& q = mats[i];
-    if ((long long)q.rows * q.cols == 0) continue;
+    if ((long long)q.rows * q.cols == 0 || (planes && slab_takes(q.rows, q.cols))) continue;
     l.m[at++] = {q.g, q.out, q.ldg, q.ldo, q.rows, q.cols, 1.f, reinterpret_cast<float*>(ws + w.x),
                  reinterpret_cast<double*>(ws + w.part) + (long long)i * kNormBlocks};
     if (at == (planes ? kJobs : 1)) flush();
@@ -655,7 +1041,8 @@ Layout muon_layout(const cgan3d_muon_seg* s, int n) {
       u += up256(s[i].rows * s[i].cols * 4);
       ++nm;
     }
-  place(w, nm, u, plane_bytes(n, [&](int i, long long& r, long long& c) { r = s[i].rows; c = s[i].cols; }));
+  const auto rc = [&](int i, long long& r, long long& c) { r = s[i].rows; c = s[i].cols; };
+  place(w, nm, u, std::max(plane_bytes(n, rc), slab_bytes(n, rc)));
   return w;
 }
 
@@ -719,6 +1106,14 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   char* base = static_cast<char*>(ws);
   float* u = reinterpret_cast<float*>(base + w.u);
   double* part = reinterpret_cast<double*>(base + w.part);
+  const bool planes = planes_hold(steps, coefficients);
+  // segment i: a matrix of slab_kernel, another one, or a vector; vectors ride along with the first list of the
+  // former as long as there is room
+  const auto is_slab = [&](int i) { return planes && segs[i].rows > 0 && segs[i].cols > 0 && slab_takes(segs[i].rows, segs[i].cols); };
+  int slabs = 0;
+  for (int i = 0; i < n; ++i) slabs += is_slab(i);
+  int room = slabs > 0 ? kSlabMats - std::min(slabs, kSlabMats) : 0;
+  const int rides = room;
   long long uo = 0;
   int nm = 0, at = 0;
   SegList l;
@@ -730,21 +1125,24 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   };
   for (int i = 0; i < n; ++i) {
     const long long total = segs[i].rows > 0 ? segs[i].rows * segs[i].cols : segs[i].cols;
+    if (!total || is_slab(i)) continue;
     if (segs[i].rows > 0) {
       l.mat[at] = nm++;
       l.u[at] = uo / 4;
       uo += up256(total * 4);
     } else {
+      if (room > 0) {
+        --room;
+        continue;
+      }
       l.mat[at] = -1;
     }
-    if (!total) continue;
     l.s[at] = segs[i];
     if (++at == kList) flush();
   }
   flush();
   uo = 0;
   nm = 0;
-  const bool planes = planes_hold(steps, coefficients);
   MatList q;
   int qn = 0;
   const auto run = [&]() {
@@ -760,16 +1158,45 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
     qn = 0;
   };
   for (int i = 0; i < n; ++i) {
-    if (segs[i].rows == 0) continue;
     const long long total = segs[i].rows * segs[i].cols;
+    if (segs[i].rows == 0 || !total || is_slab(i)) continue;
     q.m[qn] = {u + uo / 4, param + segs[i].offset, segs[i].cols, segs[i].cols, (int)segs[i].rows, (int)segs[i].cols,
                segs[i].lr_scale, reinterpret_cast<float*>(base + w.x), part + (long long)nm * kNormBlocks};
     ++nm;
     uo += up256(total * 4);
-    if (total && ++qn == (planes ? kJobs : 1)) run();
+    if (++qn == (planes ? kJobs : 1)) run();
   }
   run();
-  launch(muon_tick_kernel, dim3(1), dim3(1), 0, st, hyper);
+  SlabList sl = {};
+  long long used = 0;
+  int left = slabs, ride = rides;
+  for (int i = 0; i < n && left > 0; ++i) {
+    if (!is_slab(i)) continue;
+    SlabMat& m = sl.m[sl.n++];
+    m = {};
+    m.g = grad + segs[i].offset; m.out = param + segs[i].offset; m.mom = momentum + segs[i].offset;
+    m.rows = (int)segs[i].rows; m.cols = (int)segs[i].cols;
+    m.ldg = m.ldo = m.cols;
+    m.scale = segs[i].lr_scale;
+    used += slab_place(m, base + w.x + used);
+    if (--left > 0 && sl.n < kSlabMats) continue;
+    for (int v = 0; v < n && ride > 0; ++v) {
+      if (segs[v].rows > 0 || segs[v].cols == 0) continue;
+      SlabMat& x = sl.m[sl.n++];
+      x = {};
+      x.g = grad + segs[v].offset; x.out = param + segs[v].offset; x.mom = momentum + segs[v].offset;
+      x.sq = exp_avg_sq + segs[v].offset;
+      x.count = segs[v].cols;
+      x.nslab = (int)std::max(1LL, std::min((x.count + 4095) / 4096, 256LL));
+      --ride;
+    }
+    ride = 0;
+    sl.tick = left == 0;
+    slab_run<float>(sl, steps, coefficients, eps, hyper, st);
+    sl.n = 0;
+    used = 0;
+  }
+  if (slabs == 0) launch(muon_tick_kernel, dim3(1), dim3(1), 0, st, hyper);
   CG_LAUNCH_CHECK("cgan3d_muon_step");
   return CGAN3D_OK;
 } catch (...) {
