@@ -485,8 +485,8 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
 }
 
 // --- matrices with a short side of up to 64: the whole step in one launch ---
-// A block owns a slab of X, 128 columns of the long side (several in turn where there are more than kMaxSlabs), and
-// keeps it in LDS through a step; what the blocks of a matrix share is the 64 x 64 Gram matrix, whose partial
+// A block owns a slab of X, kCols columns of the long side (several in turn where there are more than kMaxSlabs),
+// and keeps it in LDS through a step; what the blocks of a matrix share is the 64 x 64 Gram matrix, whose partial
 // sums pass through memory between launches:
 //   launch 0:  G -> planes (and the momentum update), partial G G^T
 //   launch k:  A = sum of the partials, B = b A + c A A (every block for itself: 2 x 64^3), X <- a X + B X,
@@ -494,7 +494,9 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
 // so five steps are six launches for up to kSlabMats matrices of any shapes, where the general products take
 // nineteen.  G's planes are scaled by the power of two of the slab's largest value, and the norm is the trace of
 // the partial Gram matrices, in 64 bits: no pass of its own.  Vectors' Adam rides on launch 0.
-constexpr int kSlabMats = 28, kMaxSlabs = 48, kSlabBytes = 64 * 128 * 4;
+constexpr int kSlabMats = 28, kMaxSlabs = 32, kBatch = 16, kCols = 256, kSlab = 64 * kCols;
+constexpr int kSlabThreads = 4 * kCols, kSlabWaves = kSlabThreads / 64;  // a wave: 16 columns, and one tile of a 64 x 64 matrix
+static_assert(kSlabWaves == 16, "a wave for each tile of the Gram matrix");
 
 struct SlabMat {
   const void* g;    // G, or the gradient
@@ -504,9 +506,10 @@ struct SlabMat {
   long long ldg, ldo;
   int rows, cols;   // rows 0: a vector of `count` values
   float scale;
-  int nslab, sub;   // blocks, and slabs of 128 columns a block takes
+  int nslab, sub;   // blocks, and slabs a block takes
+  int vec_g, vec_o; // rows of G (and the momentum) / of the result start at multiples of four aligned values
   long long count;
-  f16_t* x;         // planes, [slab][2][64][128], LDS order
+  f16_t* x;         // planes, [slab][2][64][kCols], LDS order
   float* part;      // [2][nslab][64 * 64]
   float* expo;      // [nslab]: G = planes * 2^expo
 };
@@ -517,41 +520,77 @@ struct SlabList {
 };
 
 // place of 16-byte chunk c of row r: conflict-free for fragments along the row, two lanes a bank across it
-__device__ __forceinline__ int slab_at(int r, int c) { return r * 16 + (c ^ (r & 15)); }
+__device__ __forceinline__ int slab_at(int r, int c) { return r * (kCols / 8) + (c ^ (r & 15)); }
 
-// 16 x 16 tiles (ti, tj) and (ti, tj + 1) of M M^T over 32 W columns, M's planes in rows of CH chunks
-template <int CH, int W>
-__device__ __forceinline__ void gram_tiles(const f16_t* m, int plane, int ti, int tj, int lane, f32x4_m (&acc)[2]) {
+// 16 x 16 tile (ti, tj) of M M^T over 32 W columns; M's planes: a slab's (SLAB), or of 64 x 64 in rows of 8 chunks
+template <bool SLAB, int W>
+__device__ __forceinline__ void gram_tile(const f16_t* m, int plane, int ti, int tj, int lane, f32x4_m& acc) {
   const auto frag = [&](int p, int row, int k) {
     const int r = row * 16 + (lane & 15), c = k * 4 + (lane >> 4);
-    return *reinterpret_cast<const s16x8_v*>(m + p * plane + (CH == 16 ? slab_at(r, c) : r * CH + (c ^ sw_kc<8>(r))) * 8);
+    return *reinterpret_cast<const s16x8_v*>(m + p * plane + (SLAB ? slab_at(r, c) : r * 8 + (c ^ sw_kc<8>(r))) * 8);
   };
+  f32x4_m c1 = {}, c2 = {};  // chains of their own
 #pragma unroll
   for (int k = 0; k < W; ++k) {
-    const s16x8_v a0 = frag(0, ti, k), a1 = frag(1, ti, k);
+    const s16x8_v a0 = frag(0, ti, k), a1 = frag(1, ti, k), b0 = frag(0, tj, k), b1 = frag(1, tj, k);
+    c1 = plane_mfma(b1, a0, c1, f16_t());
+    c2 = plane_mfma(b0, a1, c2, f16_t());
+    acc = plane_mfma(b0, a0, acc, f16_t());
+  }
+  acc += c1 + c2;
+}
+
+// a thread's four neighbours u of a slab (row, and column within it): along the long side, or a tall matrix's short one
+__device__ __forceinline__ int slab_i(bool tall, int u, int tid) {
+  const int q = u * kSlabThreads + tid;
+  return tall ? q % 16 * 4 : q / (kCols / 4);
+}
+__device__ __forceinline__ int slab_t(bool tall, int u, int tid) {
+  const int q = u * kSlabThreads + tid;
+  return tall ? q / 16 : q % (kCols / 4) * 4;
+}
+// n of four neighbours (more than four: all); vec: they are aligned where all four are there
+template <typename T> __device__ __forceinline__ f32x4_m load4(const T* p, int n, int vec) {
+  f32x4_m v = {0.f, 0.f, 0.f, 0.f};
+  if (n >= 4 && vec) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    const v4 x = *reinterpret_cast<const v4*>(p);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const s16x8_v b0 = frag(0, tj + u, k), b1 = frag(1, tj + u, k);
-      acc[u] = plane_mfma(b1, a0, acc[u], f16_t());
-      acc[u] = plane_mfma(b0, a1, acc[u], f16_t());
-      acc[u] = plane_mfma(b0, a0, acc[u], f16_t());
-    }
+    for (int r = 0; r < 4; ++r) v[r] = to_f(x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) v[r] = to_f(p[r]);
+  }
+  return v;
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, f32x4_m v, int n, int vec) {
+  if (n >= 4 && vec) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    v4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = from_f<T>(v[r]);
+    *reinterpret_cast<v4*>(p) = x;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) p[r] = from_f<T>(v[r]);
   }
 }
 
 // PHASE 0: launch 0, 1: a step that is not the last, 2: the last
 template <typename T, int PHASE>
-__global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, float cb, float cc, float eps,
+__global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, float ca, float cb, float cc, float eps,
                                                    float* __restrict__ hyper) {
-  __shared__ __align__(16) f16_t X[2 * 64 * 128];
-  __shared__ __align__(16) f16_t Y[2 * 64 * 128];
+  __shared__ __align__(16) f16_t X[2 * kSlab];  // a wave's columns are its own: the step's result replaces them
   __shared__ __align__(16) f16_t A[2 * 64 * 64];
   __shared__ __align__(16) f16_t B[2 * 64 * 64];
-  __shared__ double redd[8];
-  __shared__ float redf[8];
+  __shared__ double redd[kSlabWaves];
+  __shared__ float redf[kSlabWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int mi = 0;
-  while (mi + 1 < l.n && (int)blockIdx.x >= l.start[mi + 1]) ++mi;
+  // this block's matrix: every lane looks at one start (the arguments are far away: one trip, not one per entry)
+  const unsigned long long before = __ballot(lane < l.n && (int)blockIdx.x >= l.start[min(lane, kSlabMats)]);
+  const int mi = __builtin_amdgcn_readfirstlane(__popcll(before) - 1);
   const SlabMat& m = l.m[mi];
   const int slab = blockIdx.x - l.start[mi];
   if (PHASE == 2 && hyper && l.tick && blockIdx.x == 0 && tid == 0) hyper[H_STEP] += 1.f;  // nothing of this launch reads it
@@ -559,155 +598,171 @@ __global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, 
     if (PHASE == 0) {
       const float h[6] = {hyper[H_VLR], hyper[H_VB1], hyper[H_VB2], hyper[H_VEPS], 0.f, hyper[H_CLIP]};
       const AdamK ak = adam_k(h, hyper[H_STEP] + 1.f);
-      for (long long q = slab * 512LL + tid; q < m.count; q += m.nslab * 512LL)
+      for (long long q = slab * (long long)kSlabThreads + tid; q < m.count; q += m.nslab * (long long)kSlabThreads)
         adam_elem(ak, static_cast<float*>(m.out), static_cast<const float*>(m.g), m.mom, m.sq, q);
     }
     return;
   }
   const bool tall = m.rows > m.cols;
   const int s = min(m.rows, m.cols), len = max(m.rows, m.cols);
-  f32x4_m gram[2] = {};
-  const int gi = wave >> 1, gj = (wave & 1) * 2;  // this wave's two tiles of a 64 x 64 matrix
-  f16_t* state = m.x + (long long)slab * m.sub * (2 * 64 * 128);
+  f32x4_m gram = {};
+  const int gi = wave >> 2, gj = wave & 3;  // this wave's tile of a 64 x 64 matrix
+  f16_t* state = m.x + (long long)slab * m.sub * (2 * kSlab);
 
   if constexpr (PHASE == 0) {
     const float mu = hyper ? hyper[H_MU] : 0.f;
     const bool nest = hyper && hyper[H_NESTEROV] != 0.f;
     const T* g = static_cast<const T*>(m.g);
-    float v[16];
+    // a thread: four neighbours in memory, four times; every load before the first store
+    f32x4_m v[4];
     const auto load = [&](int b, bool keep) {
-      const int t0 = (slab * m.sub + b) * 128;
+      const int t0 = (slab * m.sub + b) * kCols;
+      f32x4_m w[4];
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const int q = u * 512 + tid, i = tall ? q % 64 : q / 128, t = t0 + (tall ? q / 64 : q % 128);
-        v[u] = 0.f;
-        if (i < s && t < len) {
-          const long long o = tall ? t * m.ldg + i : i * m.ldg + t;
-          v[u] = to_f(g[o]);
-          if (hyper) {
-            float w = m.mom[o];
-            w += (1.f - mu) * (v[u] - w);
-            if (keep) m.mom[o] = w;
-            v[u] = nest ? v[u] + mu * (w - v[u]) : w;
-          }
-        }
+      for (int u = 0; u < 4; ++u) {
+        const int i = slab_i(tall, u, tid), t = t0 + slab_t(tall, u, tid);
+        const int n = i < s && t < len ? (tall ? s - i : len - t) : 0;
+        const long long o = tall ? t * m.ldg + i : i * m.ldg + t;
+        v[u] = load4<T>(g + o, n, m.vec_g);
+        w[u] = hyper ? load4<float>(m.mom + o, n, m.vec_g) : f32x4_m{0.f, 0.f, 0.f, 0.f};
+      }
+      if (!hyper) return;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = slab_i(tall, u, tid), t = t0 + slab_t(tall, u, tid);
+        const int n = i < s && t < len ? (tall ? s - i : len - t) : 0;
+        w[u] += (1.f - mu) * (v[u] - w[u]);
+        v[u] = nest ? v[u] + mu * (w[u] - v[u]) : w[u];
+        if (keep) store4<float>(m.mom + (tall ? t * m.ldg + i : i * m.ldg + t), w[u], n, m.vec_g);
       }
     };
     float big = 0.f;
     for (int b = 0; b < m.sub; ++b) {
       load(b, m.sub == 1);
 #pragma unroll
-      for (int u = 0; u < 16; ++u) big = fmaxf(big, fabsf(v[u]));
+      for (int u = 0; u < 16; ++u) big = fmaxf(big, fabsf(v[u >> 2][u & 3]));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
     if (lane == 0) redf[wave] = big;
-    __syncthreads();
+    lds_barrier();
     big = redf[0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) big = fmaxf(big, redf[w]);
+    for (int w = 1; w < kSlabWaves; ++w) big = fmaxf(big, redf[w]);
     // values below 2^12; nothing to scale by where all are zero or some are not finite
     const int e = big > 0.f && big < __builtin_inff() ? ilogbf(big) + 1 - 12 : 0;
     if (tid == 0) m.expo[slab] = (float)e;
     for (int b = 0; b < m.sub; ++b) {
       if (m.sub > 1) load(b, true);
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const int q = u * 512 + tid, i = tall ? q % 64 : q / 128, t = tall ? q / 64 : q % 128;
-        f16_t p[2];
-        split2(ldexpf(v[u], -e), p);
-        const int o = slab_at(i, t >> 3) * 8 + (t & 7);
-        Y[o] = p[0];
-        Y[64 * 128 + o] = p[1];
+      for (int u = 0; u < 4; ++u) {
+        const int i = slab_i(tall, u, tid), t = slab_t(tall, u, tid);
+        f16x4_m hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f16_t p[2];
+          split2(ldexpf(v[u][r], -e), p);
+          hi[r] = p[0];
+          lo[r] = p[1];
+        }
+        if (tall) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int o = slab_at(i + r, t >> 3) * 8 + (t & 7);
+            X[o] = hi[r];
+            X[kSlab + o] = lo[r];
+          }
+        } else {
+          const int o = slab_at(i, t >> 3) * 8 + (t & 7);
+          *reinterpret_cast<f16x4_m*>(X + o) = hi;
+          *reinterpret_cast<f16x4_m*>(X + kSlab + o) = lo;
+        }
       }
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        reinterpret_cast<s16x8_v*>(state + (long long)b * (2 * 64 * 128))[u * 512 + tid] = reinterpret_cast<s16x8_v*>(Y)[u * 512 + tid];
-      gram_tiles<16, 4>(Y, 64 * 128, gi, gj, lane, gram);
-      __syncthreads();
+        reinterpret_cast<s16x8_v*>(state + (long long)b * (2 * kSlab))[u * kSlabThreads + tid] = reinterpret_cast<s16x8_v*>(X)[u * kSlabThreads + tid];
+      if (gi >= gj) gram_tile<true, kCols / 32>(X, kSlab, gi, gj, lane, gram);
+      lds_barrier();
     }
   } else {
     s16x8_v xr[4];  // the slab is on its way while the Gram matrix is put together
 #pragma unroll
-    for (int u = 0; u < 4; ++u) xr[u] = reinterpret_cast<const s16x8_v*>(state)[u * 512 + tid];
-    // A: a thread adds eight neighbours of a row over the slabs, in their order
-    const float* part = m.part + (long long)((k - 1) & 1) * m.nslab * 4096 + tid * 8;
-    const int ri = tid >> 3, rj = (tid & 7) * 8;
-    float sum[8];
+    for (int u = 0; u < 4; ++u) xr[u] = reinterpret_cast<const s16x8_v*>(state)[u * kSlabThreads + tid];
+    // A: a thread adds four neighbours of a row over the slabs, in their order.  What lies beyond the short side is
+    // zero and is not read; the loads of kBatch slabs are in flight together
+    const float* part = m.part + (long long)((k - 1) & 1) * m.nslab * 4096 + tid * 4;
+    const int ri = tid >> 4, rj = (tid & 15) * 4;
+    const bool some = ri < s && rj < s;
+    f32x4_m sum = {};
     float alpha = 1.f / kAs, beta = ca;
+    const auto slabs = [&](auto f) {
+      for (int z0 = 0; z0 < m.nslab; z0 += kBatch) {
+        f32x4_m p[kBatch];
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z) {
+          p[z] = f32x4_m{0.f, 0.f, 0.f, 0.f};
+          if (some && z0 + z < m.nslab) p[z] = *reinterpret_cast<const f32x4_m*>(part + (long long)(z0 + z) * 4096);
+        }
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z) f(min(z0 + z, m.nslab - 1), p[z]);
+      }
+    };
     if (k == 1) {
-      double d[8] = {};
-#pragma unroll 2
-      for (int z = 0; z < m.nslab; ++z) {
+      double d[4] = {};
+      slabs([&](int z, const f32x4_m& p) {
         const double f = ldexp(1.0, 2 * (int)m.expo[z]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4_m p = *reinterpret_cast<const f32x4_m*>(part + (long long)z * 4096 + h * 4);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) d[h * 4 + r] += f * p[r];
-        }
-      }
+        for (int r = 0; r < 4; ++r) d[r] += f * p[r];
+      });
       double tr = 0.;
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
+      for (int r = 0; r < 4; ++r)
         if (rj + r == ri) tr = d[r];
       tr = wave_sum_d(tr);
       if (lane == 0) redd[wave] = tr;
-      __syncthreads();
+      lds_barrier();
       tr = 0.;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) tr += redd[w];
-      const double norm = sqrt(tr) + (double)eps;
+      for (int w = 0; w < kSlabWaves; ++w) tr += redd[w];
+      const double norm = sqrt(tr) + (double)eps, inv = 1. / (norm * norm);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) sum[r] = (float)(d[r] / (norm * norm));
+      for (int r = 0; r < 4; ++r) sum[r] = (float)(d[r] * inv);
       // from G's planes to X's; a slab of zeros may have any factor but an infinite one
       const float r0 = (float)fmin(ldexp(1.0, (int)m.expo[slab]) / norm * kXs, 1e38);
       alpha *= r0;
       beta *= r0;
     } else {
-#pragma unroll
-      for (int r = 0; r < 8; ++r) sum[r] = 0.f;
-#pragma unroll 4
-      for (int z = 0; z < m.nslab; ++z) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4_m p = *reinterpret_cast<const f32x4_m*>(part + (long long)z * 4096 + h * 4);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sum[h * 4 + r] += p[r];
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) sum[r] *= 1.f / (kXs * kXs);
+      slabs([&](int, const f32x4_m& p) { sum += p; });
+      sum *= 1.f / (kXs * kXs);
     }
     {
-      f16x8_m hi, lo;
+      f16x4_m hi, lo;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        f16_t p[2];
-        split2(sum[r] * kAs, p);
-        hi[r] = p[0];
-        lo[r] = p[1];
+      for (int r = 0; r < 4; ++r) {
+        f16_t q[2];
+        split2(sum[r] * kAs, q);
+        hi[r] = q[0];
+        lo[r] = q[1];
       }
-      const int o = (ri * 8 + ((tid & 7) ^ sw_kc<8>(ri))) * 8;
-      *reinterpret_cast<f16x8_m*>(A + o) = hi;
-      *reinterpret_cast<f16x8_m*>(A + 64 * 64 + o) = lo;
+      const int o = (ri * 8 + ((rj >> 3) ^ sw_kc<8>(ri))) * 8 + (rj & 7);
+      *reinterpret_cast<f16x4_m*>(A + o) = hi;
+      *reinterpret_cast<f16x4_m*>(A + 64 * 64 + o) = lo;
     }
-    __syncthreads();
-    f32x4_m sqr[2] = {};
-    gram_tiles<8, 2>(A, 64 * 64, gi, gj, lane, sqr);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int i = gi * 16 + (lane & 15), j = (gj + u) * 16 + (lane >> 4) * 4;
+    lds_barrier();
+    f32x4_m sqr = {};
+    gram_tile<false, 2>(A, 64 * 64, gi, gj, lane, sqr);
+    {
+      const int i = gi * 16 + (lane & 15), j = gj * 16 + (lane >> 4) * 4;
       const int o = (i * 8 + ((j >> 3) ^ sw_kc<8>(i))) * 8 + (j & 7);
       const f16x4_m h = *reinterpret_cast<const f16x4_m*>(A + o), lw = *reinterpret_cast<const f16x4_m*>(A + 64 * 64 + o);
       f16x4_m oh, ol;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        f16_t p[2];
-        split2(cc / kAs * sqr[u][r] + cb * ((float)h[r] + (float)lw[r]), p);
-        oh[r] = p[0];
-        ol[r] = p[1];
+        f16_t q[2];
+        split2(cc / kAs * sqr[r] + cb * ((float)h[r] + (float)lw[r]), q);
+        oh[r] = q[0];
+        ol[r] = q[1];
       }
       *reinterpret_cast<f16x4_m*>(B + o) = oh;
       *reinterpret_cast<f16x4_m*>(B + 64 * 64 + o) = ol;
@@ -715,11 +770,11 @@ __global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, 
     for (int b = 0; b < m.sub; ++b) {
       if (b > 0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) xr[u] = reinterpret_cast<const s16x8_v*>(state + (long long)b * (2 * 64 * 128))[u * 512 + tid];
+        for (int u = 0; u < 4; ++u) xr[u] = reinterpret_cast<const s16x8_v*>(state + (long long)b * (2 * kSlab))[u * kSlabThreads + tid];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) reinterpret_cast<s16x8_v*>(X)[u * 512 + tid] = xr[u];
-      __syncthreads();
+      for (int u = 0; u < 4; ++u) reinterpret_cast<s16x8_v*>(X)[u * kSlabThreads + tid] = xr[u];
+      lds_barrier();
       // a wave: 16 columns, all 64 rows
       f32x4_m acc[4] = {};
 #pragma unroll
@@ -729,7 +784,7 @@ __global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, 
         for (int p = 0; p < 2; ++p) {
           const int kr = h * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2), c = wave * 2 + ((lane & 3) >> 1);
           typedef __attribute__((address_space(3))) s16x4_v* lp;
-          const f16_t* base = X + p * 64 * 128 + (lane & 1) * 4;
+          const f16_t* base = X + p * kSlab + (lane & 1) * 4;
           const s16x4_v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(base + slab_at(kr, c) * 8));
           const s16x4_v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(base + slab_at(kr + 4, c) * 8));
           fx[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -747,7 +802,7 @@ __global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, 
       for (int q = 0; q < 4; ++q) {
         const int i = q * 16 + (lane & 15), t = wave * 16 + (lane >> 4) * 4;
         const int o = slab_at(i, t >> 3) * 8 + (t & 7);
-        const f16x4_m h = *reinterpret_cast<const f16x4_m*>(X + o), lw = *reinterpret_cast<const f16x4_m*>(X + 64 * 128 + o);
+        const f16x4_m h = *reinterpret_cast<const f16x4_m*>(X + o), lw = *reinterpret_cast<const f16x4_m*>(X + kSlab + o);
         f32x4_m x;
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = alpha * acc[q][r] + beta * ((float)h[r] + (float)lw[r]);
@@ -760,59 +815,85 @@ __global__ __launch_bounds__(512) void slab_kernel(SlabList l, int k, float ca, 
             oh[r] = p[0];
             ol[r] = p[1];
           }
-          *reinterpret_cast<f16x4_m*>(Y + o) = oh;
-          *reinterpret_cast<f16x4_m*>(Y + 64 * 128 + o) = ol;
-        } else {  // f32, rows of 32 chunks
-          *reinterpret_cast<f32x4_m*>(reinterpret_cast<float*>(Y) + (i * 32 + ((t >> 2) ^ (i & 15))) * 4) = x;
+          *reinterpret_cast<f16x4_m*>(X + o) = oh;
+          *reinterpret_cast<f16x4_m*>(X + kSlab + o) = ol;
+        } else {  // the two planes' places hold one f32: its high half and its low half
+          f16x4_m oh, ol;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const unsigned w = __float_as_uint(x[r] * (1.f / kXs));
+            oh[r] = __builtin_bit_cast(f16_t, (unsigned short)(w >> 16));
+            ol[r] = __builtin_bit_cast(f16_t, (unsigned short)w);
+          }
+          *reinterpret_cast<f16x4_m*>(X + o) = oh;
+          *reinterpret_cast<f16x4_m*>(X + kSlab + o) = ol;
         }
       }
-      __syncthreads();
+      lds_barrier();
       if constexpr (PHASE == 1) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          reinterpret_cast<s16x8_v*>(state + (long long)b * (2 * 64 * 128))[u * 512 + tid] = reinterpret_cast<s16x8_v*>(Y)[u * 512 + tid];
-        gram_tiles<16, 4>(Y, 64 * 128, gi, gj, lane, gram);
-        __syncthreads();
+          reinterpret_cast<s16x8_v*>(state + (long long)b * (2 * kSlab))[u * kSlabThreads + tid] = reinterpret_cast<s16x8_v*>(X)[u * kSlabThreads + tid];
+        if (gi >= gj) gram_tile<true, kCols / 32>(X, kSlab, gi, gj, lane, gram);
+        lds_barrier();
       } else {
-        const int t0 = (slab * m.sub + b) * 128;
+        const int t0 = (slab * m.sub + b) * kCols;
         const float lr = hyper ? hyper[H_LR] : 0.f, clip = hyper ? hyper[H_CLIP] : 0.f;
         const float keep = hyper ? 1.f - lr * hyper[H_WD] : 0.f, rate = lr * m.scale;
-        const float* y = reinterpret_cast<const float*>(Y);
+        f32x4_m w[4];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) {
-          const int q = u * 512 + tid, i = tall ? q % 64 : q / 128, t = tall ? q / 64 : q % 128;
-          if (i >= s || t0 + t >= len) continue;
-          const float x = y[(i * 32 + ((t >> 2) ^ (i & 15))) * 4 + (t & 3)] * (1.f / kXs);
+        for (int u = 0; u < 4; ++u) {
+          const int i = slab_i(tall, u, tid), t = t0 + slab_t(tall, u, tid);
+          const int n = hyper && i < s && t < len ? (tall ? s - i : len - t) : 0;
+          w[u] = load4<float>(static_cast<const float*>(m.out) + (tall ? t * m.ldo + i : i * m.ldo + t), n, m.vec_o);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = slab_i(tall, u, tid), t = slab_t(tall, u, tid);
+          const int n = i < s && t0 + t < len ? (tall ? s - i : len - t0 - t) : 0;
           const long long o = tall ? (t0 + t) * m.ldo + i : i * m.ldo + t0 + t;
+          f32x4_m x;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = tall ? slab_at(i + r, t >> 3) * 8 + (t & 7) : slab_at(i, t >> 3) * 8 + (t & 7) + r;
+            x[r] = __uint_as_float((unsigned)__builtin_bit_cast(unsigned short, X[at]) << 16 |
+                                   __builtin_bit_cast(unsigned short, X[kSlab + at]));
+          }
           if (hyper) {
-            float* p = static_cast<float*>(m.out);
-            float w = p[o] * keep - rate * x;
-            if (clip > 0.f) w = fminf(fmaxf(w, -clip), clip);
-            p[o] = w;
+            x = w[u] * keep - rate * x;
+            if (clip > 0.f)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) x[r] = fminf(fmaxf(x[r], -clip), clip);
+            store4<float>(static_cast<float*>(m.out) + o, x, n, m.vec_o);
           } else {
-            static_cast<T*>(m.out)[o] = from_f<T>(x);
+            store4<T>(static_cast<T*>(m.out) + o, x, n, m.vec_o);
           }
         }
-        __syncthreads();
+        lds_barrier();
       }
     }
   }
   if constexpr (PHASE != 2) {
+    if (gi < gj) return;  // the upper triangle is the lower one's mirror
     float* part = m.part + ((long long)(k & 1) * m.nslab + slab) * 4096;
+    const int i = gi * 16 + (lane & 15), j = gj * 16 + (lane >> 4) * 4;
+    *reinterpret_cast<f32x4_m*>(part + i * 64 + j) = gram;
+    if (gi > gj)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      *reinterpret_cast<f32x4_m*>(part + (gi * 16 + (lane & 15)) * 64 + (gj + u) * 16 + (lane >> 4) * 4) = gram[u];
+      for (int r = 0; r < 4; ++r) part[(j + r) * 64 + i] = gram[r];
   }
 }
 
 bool slab_takes(long long rows, long long cols) { return std::min(rows, cols) <= 64; }
 
 // blocks of a matrix, and its part of the workspace from `ws` on
-long long slab_place(SlabMat& m, char* ws) {
-  const int len = std::max(m.rows, m.cols), n128 = (len + 127) / 128;
-  m.sub = (n128 + kMaxSlabs - 1) / kMaxSlabs;
-  m.nslab = (n128 + m.sub - 1) / m.sub;
-  const long long xb = (long long)m.nslab * m.sub * kSlabBytes, pb = 2LL * m.nslab * 4096 * 4;
+long long slab_place(SlabMat& m, char* ws, int elt) {
+  const int len = std::max(m.rows, m.cols), all = (len + kCols - 1) / kCols;
+  m.sub = (all + kMaxSlabs - 1) / kMaxSlabs;
+  m.nslab = (all + m.sub - 1) / m.sub;
+  const long long xb = (long long)m.nslab * m.sub * kSlab * 4, pb = 2LL * m.nslab * 4096 * 4;
+  m.vec_g = m.ldg % 4 == 0 && reinterpret_cast<uintptr_t>(m.g) % (4 * elt) == 0 && reinterpret_cast<uintptr_t>(m.mom) % 16 == 0;
+  m.vec_o = m.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(m.out) % (4 * elt) == 0;
   m.x = reinterpret_cast<f16_t*>(ws);
   m.part = reinterpret_cast<float*>(ws + xb);
   m.expo = reinterpret_cast<float*>(ws + xb + pb);
@@ -827,10 +908,10 @@ void slab_run(SlabList& l, int steps, const float* co, float eps, float* hyper, 
     l.start[i] = at;
     at += l.m[i].nslab;
   }
-  launch(slab_kernel<T, 0>, dim3(at), dim3(512), 0, st, l, 0, co[0], co[1], co[2], eps, hyper);
+  launch(slab_kernel<T, 0>, dim3(at), dim3(kSlabThreads), 0, st, l, 0, co[0], co[1], co[2], eps, hyper);
   for (int k = 1; k < steps; ++k)
-    launch(slab_kernel<T, 1>, dim3(at), dim3(512), 0, st, l, k, co[0], co[1], co[2], eps, hyper);
-  launch(slab_kernel<T, 2>, dim3(at), dim3(512), 0, st, l, steps, co[0], co[1], co[2], eps, hyper);
+    launch(slab_kernel<T, 1>, dim3(at), dim3(kSlabThreads), 0, st, l, k, co[0], co[1], co[2], eps, hyper);
+  launch(slab_kernel<T, 2>, dim3(at), dim3(kSlabThreads), 0, st, l, steps, co[0], co[1], co[2], eps, hyper);
 }
 
 // Whether iterates that start within |X| <= 1 stay where the planes hold them: |X| < 2^16 / kXs, |A| and |B|
@@ -905,10 +986,10 @@ template <class F> long long slab_bytes(int n, F rc) {
     long long r = 0, c = 0;
     rc(i, r, c);
     if (r * c == 0 || !slab_takes(r, c)) continue;
-    SlabMat m;
+    SlabMat m = {};
     m.rows = (int)r;
     m.cols = (int)c;
-    sum += slab_place(m, nullptr);
+    sum += slab_place(m, nullptr, 4);
     most = std::max(most, sum);
     if (++at == kSlabMats) at = 0, sum = 0;
   }
@@ -985,7 +1066,7 @@ void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, cha
         SlabMat& m = sl.m[sl.n++];
         m = {};
         m.g = q.g; m.out = q.out; m.ldg = q.ldg; m.ldo = q.ldo; m.rows = q.rows; m.cols = q.cols;
-        used += slab_place(m, ws + w.x + used);
+        used += slab_place(m, ws + w.x + used, sizeof(T));
       }
       if (sl.n == kSlabMats || (i == n - 1 && sl.n > 0)) {
         slab_run<T>(sl, steps, co, eps, nullptr, st);
@@ -1178,7 +1259,7 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
     m.rows = (int)segs[i].rows; m.cols = (int)segs[i].cols;
     m.ldg = m.ldo = m.cols;
     m.scale = segs[i].lr_scale;
-    used += slab_place(m, base + w.x + used);
+    used += slab_place(m, base + w.x + used, 4);
     if (--left > 0 && sl.n < kSlabMats) continue;
     for (int v = 0; v < n && ride > 0; ++v) {
       if (segs[v].rows > 0 || segs[v].cols == 0) continue;
