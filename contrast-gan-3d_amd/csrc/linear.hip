@@ -9,6 +9,7 @@
 //
 // Which kernel a product takes (mat_route):
 //   rows <= 4, forward     gemv_kernel: a wave per output column pair streams the weight once
+//   k, n <= 64              rows_fwd_kernel, rows_bwd_kernel: every row's values are read and written once
 //   16-bit tensors         plane_kernel (planes.h) on the tensors themselves; an operand whose rows are not
 //                          whole aligned 16-byte chunks is copied once into rows that are
 //   f32 tensors            plane_kernel on three bf16 planes where the product is large enough to pay for
@@ -384,6 +385,311 @@ template <typename T> void gemv_run(const MatArgs& p, hipStream_t st) {
   else gemv_run_m<T, 4>(p, st);
 }
 
+// --- few channels (k, n <= 64): every row's values are read and written once ---
+// Forward: a wave takes 16 rows at a time, x straight from memory into fragments, the whole weight in registers; no
+// LDS, no barrier.  Bound by memory.
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, int vec, T (&v)[8]) {
+  if (n >= 8 && vec) {
+    typedef T vt __attribute__((ext_vector_type(MatT<T>::VEC)));
+#pragma unroll
+    for (int h = 0; h < 8 / MatT<T>::VEC; ++h)
+      *reinterpret_cast<vt*>(v + h * MatT<T>::VEC) = *reinterpret_cast<const vt*>(p + h * MatT<T>::VEC);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : from_f<T>(0.f);
+  }
+}
+
+template <typename T, int NT, int KS>
+__global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
+                                                       long long ldw, long long rows, int n, int k, int vecx, int vece,
+                                                       MatEpi e) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  typedef typename PreT<T>::type preT;
+  typedef preT p4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
+  __align__(16) T fw[NT][KS][8];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int j = t * 16 + row, c = s * 32 + g * 8;
+      load8(w + (long long)min(j, n - 1) * ldw + c, j < n ? k - c : 0, 0, fw[t][s]);
+    }
+  v4 bias[NT] = {};
+  if (e.bias)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (t * 16 + g * 4 + r < n) bias[t][r] = static_cast<const T*>(e.bias)[t * 16 + g * 4 + r];
+  const long long groups = (rows + 15) / 16, step = (long long)gridDim.x * 4;
+  for (long long q = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); q < groups; q += step) {
+    const long long i = q * 16 + row;
+    const bool in = i < rows;
+    __align__(16) T fx[KS][8];
+    v4 res[NT];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) load8(x + i * ldx + s * 32 + g * 8, in ? k - (s * 32 + g * 8) : 0, vecx, fx[s]);
+    if (e.residual && vece && in)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (t * 16 + g * 4 < n) res[t] = *reinterpret_cast<const v4*>(static_cast<const T*>(e.residual) + i * e.ldr + t * 16 + g * 4);
+    f32x4_m acc[NT] = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = mfma_8(fw[t][s], fx[s], acc[t]);
+    if (!in) continue;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int j = t * 16 + g * 4;
+      if (j >= n) continue;
+      f32x4_m v = acc[t];
+      if (!vece) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (j + r < n) mat_store<T>(e, n, i, j + r, v[r]);
+        continue;
+      }
+      if (e.bias)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += to_f(bias[t][r]);
+      if (e.preact) {
+        p4 p;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          preT z;
+          mat_preact(&z, v[r]);
+          p[r] = z;
+        }
+        *reinterpret_cast<p4*>(static_cast<preT*>(e.preact) + i * n + j) = p;
+      }
+      v4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[r] = mat_act<sizeof(T) == 2>(v[r], e.act, e.slope);
+        o[r] = from_f<T>(e.residual ? v[r] + to_f(res[t][r]) : v[r]);
+      }
+      *reinterpret_cast<v4*>(static_cast<T*>(e.out) + i * e.ldo + j) = o;
+    }
+  }
+}
+
+// Backward: one pass over dy, z and x writes dx and keeps dW and db in registers; a block takes tiles of 64 rows in
+// turn and leaves one partial sum of each.  dz is used as its own type would hold it, for db before that.
+constexpr int kRowsBlocks = 512;
+template <typename T, int NT, int KT>
+__global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy, long long lddy,
+                                                       const typename PreT<T>::type* __restrict__ pre,
+                                                       const T* __restrict__ x, long long ldx, const T* __restrict__ w,
+                                                       long long ldw, T* __restrict__ dx, long long lddx,
+                                                       float* __restrict__ part, long long rows, int n, int k, int act,
+                                                       float slope, int vecy, int vecx, int vecd, int want_w) {
+  constexpr int NP = NT * 16, KP = KT * 16, PAD = MatT<T>::PAD, NS = (NP + 31) / 32 * 32;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  typedef typename PreT<T>::type preT;
+  typedef preT p4 __attribute__((ext_vector_type(4)));
+  __shared__ __align__(16) T dz[64 * (NS + PAD)];   // [row][n]
+  __shared__ __align__(16) T dzt[NP * (64 + PAD)];  // [n][row]
+  __shared__ __align__(16) T xt[KP * (64 + PAD)];   // [k][row]
+  __shared__ __align__(16) T wt[KP * (NS + PAD)];   // [k][n]
+  __shared__ float red[256 * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, g = lane >> 4;
+  for (int q = tid; q < KP * NS; q += 256) {
+    const int c = q % KP, j = q / KP;
+    wt[c * (NS + PAD) + j] = dx && c < k && j < n ? w[(long long)j * ldw + c] : from_f<T>(0.f);
+  }
+  if constexpr (NS > NP)
+    for (int q = tid; q < 64 * (NS - NP); q += 256) dz[q / (NS - NP) * (NS + PAD) + NP + q % (NS - NP)] = from_f<T>(0.f);
+  f32x4_m aw[KT] = {};
+  f32x4_m sb = {};
+  for (long long r0 = blockIdx.x * 64LL; r0 < rows; r0 += gridDim.x * 64LL) {
+    constexpr int NC = NP / 4, KC = KP / 4, UN = 64 * NC / 256, UK = 64 * KC / 256;  // chunks of four a row, a thread
+    v4 vy[UN], vx[UK];
+    p4 vz[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int q = u * 256 + tid, j = q % NC * 4;
+      const long long i = r0 + q / NC;
+      vy[u] = v4{};
+      vz[u] = p4{};
+      if (i < rows && j < n) {
+        if (vecy) {
+          vy[u] = *reinterpret_cast<const v4*>(dy + i * lddy + j);
+          if (act != CGAN3D_ACT_NONE) vz[u] = *reinterpret_cast<const p4*>(pre + i * n + j);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j + r < n) {
+              vy[u][r] = dy[i * lddy + j + r];
+              if (act != CGAN3D_ACT_NONE) vz[u][r] = pre[i * n + j + r];
+            }
+        }
+      }
+    }
+    if (want_w) {
+#pragma unroll
+      for (int u = 0; u < UK; ++u) {
+        const int q = u * 256 + tid, c = q % KC * 4;
+        const long long i = r0 + q / KC;
+        vx[u] = v4{};
+        if (i < rows && c < k) {
+          if (vecx) vx[u] = *reinterpret_cast<const v4*>(x + i * ldx + c);
+          else
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (c + r < k) vx[u][r] = x[i * ldx + c + r];
+        }
+      }
+    }
+    __syncthreads();  // the previous tile's fragments are read
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int q = u * 256 + tid, j = q % NC * 4, i = q / NC;
+      v4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = to_f(vy[u][r]);
+        if (act != CGAN3D_ACT_NONE) v *= mat_act_grad<sizeof(T) == 2>(to_f(vz[u][r]), act, slope);
+        sb[r] += v;
+        o[r] = from_f<T>(v);
+        dzt[(j + r) * (64 + PAD) + i] = o[r];
+      }
+      *reinterpret_cast<v4*>(&dz[i * (NS + PAD) + j]) = o;
+    }
+    if (want_w) {
+#pragma unroll
+      for (int u = 0; u < UK; ++u) {
+        const int q = u * 256 + tid, c = q % KC * 4, i = q / KC;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) xt[(c + r) * (64 + PAD) + i] = vx[u][r];
+      }
+    }
+    __syncthreads();
+    if (dx) {  // a wave: 16 rows, every column
+      f32x4_m ax[KT] = {};
+#pragma unroll
+      for (int s = 0; s < NS / 32; ++s)
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+          ax[t] = mfma_8(&wt[(t * 16 + row) * (NS + PAD) + s * 32 + g * 8], &dz[(wave * 16 + row) * (NS + PAD) + s * 32 + g * 8], ax[t]);
+      const long long i = r0 + wave * 16 + row;
+      if (i < rows)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const int c = t * 16 + g * 4;
+          if (c >= k) continue;
+          v4 o;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] = from_f<T>(ax[t][r]);
+          if (vecd) *reinterpret_cast<v4*>(dx + i * lddx + c) = o;
+          else
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (c + r < k) dx[i * lddx + c + r] = o[r];
+        }
+    }
+    if (want_w && wave < NT) {  // a wave: 16 rows of dW
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+          aw[t] = mfma_8(&xt[(t * 16 + row) * (64 + PAD) + s * 32 + g * 8], &dzt[(wave * 16 + row) * (64 + PAD) + s * 32 + g * 8], aw[t]);
+    }
+  }
+  // partial sums: [block][n k + n]
+  if (!part) return;
+  float* o = part + (long long)blockIdx.x * (n * k + n);
+  if (want_w && wave < NT) {
+    const int j = wave * 16 + row;
+    if (j < n)
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t * 16 + g * 4 + r < k) o[j * k + t * 16 + g * 4 + r] = aw[t][r];
+  }
+  constexpr int NC = NP / 4;
+  *reinterpret_cast<f32x4_m*>(red + tid * 4) = sb;
+  __syncthreads();
+  if (tid < NP && tid < n) {
+    float s = 0.f;
+    for (int q = tid / 4; q < 256; q += NC) s += red[q * 4 + tid % 4];
+    o[n * k + tid] = s;
+  }
+}
+
+// out[c] = sum of part[b][c] over nb rows of `width`, 16 columns a block, 64 threads on each, added in a fixed order; the
+// columns from n k on are db's
+template <typename T>
+__global__ __launch_bounds__(1024) void rows_join_kernel(const float* __restrict__ part, int nb, int width, int nk,
+                                                         T* __restrict__ dw, T* __restrict__ db) {
+  __shared__ float red[64][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  float s = 0.f;
+  if (col < width)
+#pragma unroll 8
+    for (int b = r; b < nb; b += 64) s += part[(long long)b * width + col];
+  red[r][c] = s;
+  __syncthreads();
+  if (r == 0 && col < width) {
+    double a = 0.;
+    for (int q = 0; q < 64; ++q) a += red[q][c];
+    if (col < nk) {
+      if (dw) dw[col] = from_f<T>((float)a);
+    } else if (db) {
+      db[col - nk] = from_f<T>((float)a);
+    }
+  }
+}
+
+bool few_channels(long long n, long long k) { return n > 0 && k > 0 && n <= 64 && k <= 64; }
+// one pass pays where the rows fill the card; below, the products' launches are as good
+bool rows_bwd_takes(const cgan3d_linear_args* a) { return few_channels(a->n, a->k) && a->rows >= 64 && (a->dx || a->dw); }
+int rows_blocks(const cgan3d_linear_args* a) { return (int)std::min<long long>((a->rows + 63) / 64, kRowsBlocks); }
+
+template <typename T, int NT> void rows_fwd_nt(const MatArgs& p, int vecx, int vece, hipStream_t st) {
+  const T* x = static_cast<const T*>(p.a);
+  const T* w = static_cast<const T*>(p.b);
+  // four waves a block; enough blocks to fill the card, each wave going on from there
+  const unsigned blocks = (unsigned)std::min((p.I + 63) / 64, 8LL * cu_count());
+  if (p.K <= 32) launch(rows_fwd_kernel<T, NT, 1>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vece, p.e);
+  else launch(rows_fwd_kernel<T, NT, 2>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vece, p.e);
+}
+template <typename T> void rows_fwd_run(const MatArgs& p, hipStream_t st) {
+  const int vecx = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % MatT<T>::VEC == 0;
+  const int vece = p.J % 4 == 0 && vec4(p.e.residual, p.e.ldr, sizeof(T)) && vec4(p.e.out, p.e.ldo, sizeof(T)) &&
+                   vec4(p.e.preact, p.J, sizeof(T));
+  if (p.J <= 16) rows_fwd_nt<T, 1>(p, vecx, vece, st);
+  else if (p.J <= 32) rows_fwd_nt<T, 2>(p, vecx, vece, st);
+  else rows_fwd_nt<T, 4>(p, vecx, vece, st);
+}
+
+template <typename T, int NT, int KT> void rows_bwd_nk(const cgan3d_linear_args* a, float* part, hipStream_t st) {
+  typedef typename PreT<T>::type preT;
+  const int b = sizeof(T);
+  const int vecy = a->n % 4 == 0 && vec4(a->dy, a->lddy, b) && vec4(a->act != CGAN3D_ACT_NONE ? a->preact : nullptr, a->n, b);
+  const int vecx = a->k % 4 == 0 && vec4(a->x, a->ldx, b), vecd = a->k % 4 == 0 && vec4(a->dx, a->lddx, b);
+  launch(rows_bwd_kernel<T, NT, KT>, dim3(rows_blocks(a)), dim3(256), 0, st, static_cast<const T*>(a->dy), (long long)a->lddy,
+         static_cast<const preT*>(a->preact), static_cast<const T*>(a->x), (long long)a->ldx, static_cast<const T*>(a->w),
+         (long long)a->ldw, static_cast<T*>(a->dx), (long long)a->lddx, part, (long long)a->rows, a->n, a->k, a->act,
+         a->slope, vecy, vecx, vecd, a->dw != nullptr ? 1 : 0);
+}
+template <typename T> void rows_bwd_run(const cgan3d_linear_args* a, void* ws, hipStream_t st) {
+  float* part = a->dw || a->dbias ? static_cast<float*>(ws) : nullptr;
+  const int nt = a->n <= 16 ? 1 : a->n <= 32 ? 2 : 4, kt = a->k <= 16 ? 1 : a->k <= 32 ? 2 : 4;
+#define CG_ROWS(N, K) \
+  if (nt == N && kt == K) rows_bwd_nk<T, N, K>(a, part, st);
+  CG_ROWS(1, 1) CG_ROWS(1, 2) CG_ROWS(1, 4) CG_ROWS(2, 1) CG_ROWS(2, 2) CG_ROWS(2, 4) CG_ROWS(4, 1) CG_ROWS(4, 2) CG_ROWS(4, 4)
+#undef CG_ROWS
+  if (part) {
+    const int width = a->n * a->k + a->n;
+    launch(rows_join_kernel<T>, dim3((width + 15) / 16), dim3(1024), 0, st, (const float*)part, rows_blocks(a), width,
+           a->n * a->k, static_cast<T*>(a->dw), static_cast<T*>(a->dbias));
+  }
+}
+
 // --- dz = dy * act'(z), and its column sums ---
 // CT threads of a block along the columns (V values each), the rest along the rows; column sums in 32 bits, of dz
 // before its rounding, into part [blockIdx.y][n].  dz goes to rows of ldz values whose padding is zeroed:
@@ -519,6 +825,10 @@ struct Bwd {  // the backward pass: dz, and where things lie in its workspace
 Bwd bwd_layout(const cgan3d_linear_args* a) {
   Bwd w = {};
   const int dt = a->dtype;
+  if (rows_bwd_takes(a)) {
+    w.total = a->dw || a->dbias ? (long long)rows_blocks(a) * (a->n * a->k + a->n) * 4 : 0;
+    return w;
+  }
   // both products take dz in one form: planes if either is better off with them
   const bool rx = a->dx && mat_route(dt, a->rows, a->k, a->n) == ROUTE_PLANES && a->rows && a->k;
   const bool rw = a->dw && mat_route(dt, a->n, a->k, a->rows) == ROUTE_PLANES && a->n && a->k;
@@ -549,7 +859,7 @@ void fwd_operands(const cgan3d_linear_args* a, Operand* x, Operand* w) {
   *w = {a->w, a->ldw, a->n, a->k, false, false};
 }
 long long fwd_bytes(const cgan3d_linear_args* a) {
-  if (a->rows <= kGemvRows) return 0;
+  if (a->rows <= kGemvRows || few_channels(a->n, a->k)) return 0;
   Operand x, w;
   fwd_operands(a, &x, &w);
   return product_bytes(a->dtype, x, w, a->rows, a->n, a->k);
@@ -633,6 +943,10 @@ extern "C" int cgan3d_linear_fwd(const cgan3d_linear_args* a, void* ws, int64_t 
     if (a->dtype == CGAN3D_DT_F32) gemv_run<float>(p, st);
     else if (a->dtype == CGAN3D_DT_BF16) gemv_run<bf16_t>(p, st);
     else gemv_run<f16_t>(p, st);
+  } else if (few_channels(a->n, a->k)) {
+    if (a->dtype == CGAN3D_DT_F32) rows_fwd_run<float>(p, st);
+    else if (a->dtype == CGAN3D_DT_BF16) rows_fwd_run<bf16_t>(p, st);
+    else rows_fwd_run<f16_t>(p, st);
   } else {
     Operand x0, w0;
     fwd_operands(a, &x0, &w0);
@@ -672,6 +986,13 @@ extern "C" int cgan3d_linear_bwd(const cgan3d_linear_args* a, void* ws, int64_t 
   }
   hipStream_t st = (hipStream_t)stream;
   char* base = static_cast<char*>(ws);
+  if (rows_bwd_takes(a)) {
+    if (a->dtype == CGAN3D_DT_F32) rows_bwd_run<float>(a, ws, st);
+    else if (a->dtype == CGAN3D_DT_BF16) rows_bwd_run<bf16_t>(a, ws, st);
+    else rows_bwd_run<f16_t>(a, ws, st);
+    CG_LAUNCH_CHECK("cgan3d_linear_bwd");
+    return CGAN3D_OK;
+  }
   void* dz = l.has_dz ? base + l.dz : nullptr;
   float* part = a->dbias ? reinterpret_cast<float*>(base + l.part) : nullptr;
   if (a->dbias || l.has_dz) {
