@@ -36,8 +36,10 @@ def _rows(t: Tensor, cols: int) -> Tensor:
     """``t`` [..., cols] as a matrix with contiguous rows (a view wherever its strides allow one)."""
     if t.dim() != 2:
         t = t.reshape(math.prod(t.shape[:-1]), cols)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
-        t = t.contiguous()
+    if not t.is_contiguous():
+        s = t.stride()
+        if (cols > 1 and s[1] != 1) or (t.shape[0] > 1 and s[0] < cols):
+            t = t.contiguous()
     return t
 
 
@@ -53,19 +55,19 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
         raise ValueError(f"fused_linear: residual {tuple(residual.shape)} is not of the result's shape "
                          f"{(*x.shape[:-1], weight.shape[0])}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _LinearFn.apply(x, weight, bias, residual, act, slope)
     return _forward(x, weight, bias, residual, act, slope, None)
 
 
 def _forward(x, weight, bias, residual, act, slope, preact):
     n, k = weight.shape
-    x2 = _rows(x.detach(), k)
-    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    ops.linear(x2, _rows(weight.detach(), k), y.view(x2.shape[0], n),
-               bias=bias.detach().contiguous() if bias is not None else None,
-               residual=_rows(residual.detach(), n) if residual is not None else None, act=act, slope=slope,
-               preact=preact)
+    x2 = _rows(x, k)
+    y = x.new_empty((*x.shape[:-1], n))
+    ops.linear(x2, _rows(weight, k), y if y.dim() == 2 else y.view(x2.shape[0], n),
+               bias if bias is None or bias.is_contiguous() else bias.contiguous(),
+               residual if residual is None else _rows(residual, n), act, slope, preact)
     return y
 
 
@@ -74,7 +76,8 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act, slope):
         preact = None
         if act != L.ACT_NONE and any(ctx.needs_input_grad[:3]):
-            preact = torch.empty((math.prod(x.shape[:-1]), weight.shape[0]), dtype=ops.linear_preact_dtype(x.dtype), device=x.device)
+            preact = torch.empty((math.prod(x.shape[:-1]), weight.shape[0]), dtype=ops.linear_preact_dtype(x.dtype),
+                                 device=x.device)
         y = _forward(x, weight, bias, residual, act, slope, preact)
         ctx.act, ctx.slope = act, slope
         ctx.save_for_backward(x, weight, preact)
@@ -87,14 +90,13 @@ class _LinearFn(torch.autograd.Function):
         x, weight, preact = ctx.saved_tensors
         n, k = weight.shape
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if nx else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if nw else None
-        db = torch.empty(n, dtype=x.dtype, device=x.device) if nb else None
+        dx = x.new_empty(x.shape) if nx else None
+        dw = x.new_empty((n, k)) if nw else None
+        db = x.new_empty(n) if nb else None
         if nx or nw or nb:
-            x2 = _rows(x.detach(), k)
-            ops.linear_backward(_rows(grad_out, n), x2, _rows(weight.detach(), k),
-                                dx=dx.view(x2.shape) if nx else None, dw=dw, dbias=db, act=ctx.act, slope=ctx.slope,
-                                preact=preact)
+            x2 = _rows(x, k)
+            ops.linear_backward(_rows(grad_out, n), x2, _rows(weight, k),
+                                dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db, ctx.act, ctx.slope, preact)
         return dx, dw, db, grad_out if nr else None, None, None
 
 

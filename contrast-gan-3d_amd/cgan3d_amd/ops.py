@@ -1443,25 +1443,32 @@ def patch_normalize(out: torch.Tensor, weight: torch.Tensor):
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # a s + b s^3 + c s^5 of one Newton-Schulz step
 
 
-def _matrix(t, rows, cols, what, dtype, device):
+def _matrix(t, rows, cols, who, name, dtype, device):
     """Row stride of a [rows, cols] operand whose rows are contiguous (a padded or sliced row stride is
-    fine); anything else is refused."""
-    if t.dtype != dtype:
-        raise TypeError(f"{what}: dtype {t.dtype} != {dtype}")
+    fine); anything else is refused.  (These run on every call of a small layer: plain comparisons, and
+    texts only where something is wrong.)"""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is dtype and len(shape) == 2 and shape[0] == rows and shape[1] == cols and t.device == device:
+        ld = stride[0] if rows > 1 else cols or 1
+        if (cols <= 1 or stride[1] == 1) and ld >= cols:
+            return ld
+        raise ValueError(f"{who} {name}: rows must be contiguous and apart (strides {stride})")
+    if t.dtype is not dtype:
+        raise TypeError(f"{who} {name}: dtype {t.dtype} != {dtype}")
     if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, the other operands are on {device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{what}: shape {tuple(t.shape)} != {(rows, cols)}")
-    ld = t.stride(0) if rows > 1 else max(cols, 1)
-    if (cols > 1 and t.stride(1) != 1) or ld < cols:
-        raise ValueError(f"{what}: rows must be contiguous and apart (strides {t.stride()})")
-    return ld
+        raise ValueError(f"{who} {name}: on {t.device}, the other operands are on {device}")
+    raise ValueError(f"{who} {name}: shape {tuple(shape)} != {(rows, cols)}")
 
 
-def _flat(t, n, what, dtype, device):
+def _flat(t, n, who, name, dtype, device):
+    """Address of a contiguous operand of n values."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{who} {name}: dtype {t.dtype} != {dtype}")
     if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, the other operands are on {device}")
-    _need(t, n, what, dtype=dtype)
+        raise ValueError(f"{who} {name}: on {t.device}, the other operands are on {device}")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{who} {name}: {n} contiguous values needed, got shape {tuple(t.shape)}, strides {t.stride()}")
+    return t.data_ptr()
 
 
 def _dt(t, what):
@@ -1489,10 +1496,13 @@ def _workspace(ws, need, what, device):
 
 def _launch_on(device, name, *args):
     """``_launch`` on ``device``'s current stream, whichever device is current."""
-    if DRY_RUN or device.index is None or device.index == torch.cuda.current_device():
-        return _launch(name, *args)
+    if DRY_RUN:
+        return 0
+    i = device.index
+    if i is None or i == torch.cuda.current_device():
+        return getattr(L.lib(), name)(*args, L.stream())
     with torch.cuda.device(device):
-        return _launch(name, *args)
+        return getattr(L.lib(), name)(*args, L.stream())
 
 
 LINEAR_ACTS = (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU, L.ACT_TANH, L.ACT_GELU, L.ACT_SILU)
@@ -1503,65 +1513,64 @@ def linear_preact_dtype(dtype):
     return torch.float32 if dtype == torch.float32 else torch.float16
 
 
-def _linear_args(x, w, act, slope, what):
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError(f"{what}: x and w must be matrices, got {tuple(x.shape)} and {tuple(w.shape)}")
+def _linear_sizes(x, w, act, who):
+    """(rows, k, n, dtype code, row strides of x and w)."""
     if act not in LINEAR_ACTS:
-        raise ValueError(f"{what}: activation code {act} (none, relu, lrelu, tanh, gelu or silu)")
-    a = L.LinearArgs()
-    a.dtype = _dt(x, f"{what} x")
-    a.rows, a.k = x.shape
-    a.n = w.shape[0]
-    a.act, a.slope = act, slope
-    a.x, a.ldx = x.data_ptr(), _matrix(x, a.rows, a.k, f"{what} x", x.dtype, x.device)
-    a.w, a.ldw = w.data_ptr(), _matrix(w, a.n, a.k, f"{what} w", x.dtype, x.device)
-    return a
+        raise ValueError(f"{who}: activation code {act} (none, relu, lrelu, tanh, gelu or silu)")
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"{who}: x and w must be matrices, got {tuple(x.shape)} and {tuple(w.shape)}")
+    dt, dev = _dt(x, who), x.device
+    (rows, k), n = x.shape, w.shape[0]
+    return rows, k, n, dt, _matrix(x, rows, k, who, "x", x.dtype, dev), _matrix(w, n, k, who, "w", x.dtype, dev)
 
 
 def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
     """``y = act(x w^T + bias) + residual`` (cgan3d_linear_fwd): x [rows, k], w [n, k], bias [n], residual
     and y [rows, n], all of one dtype (f32, bf16 or f16), rows strided as they like.  ``preact`` [rows, n]
     (``linear_preact_dtype``) receives x w^T + bias for ``linear_backward``.  y may be the residual."""
-    a = _linear_args(x, w, act, slope, "linear")
-    dev = x.device
-    a.y, a.ldy = y.data_ptr(), _matrix(y, a.rows, a.n, "linear y", x.dtype, dev)
-    if bias is not None:
-        _flat(bias, a.n, "linear bias", x.dtype, dev)
-        a.bias = bias.data_ptr()
-    if residual is not None:
-        a.residual, a.ldr = residual.data_ptr(), _matrix(residual, a.rows, a.n, "linear residual", x.dtype, dev)
-    if preact is not None:
-        _flat(preact, a.rows * a.n, "linear preact", linear_preact_dtype(x.dtype), dev)
-        a.preact = preact.data_ptr()
+    rows, k, n, dt, ldx, ldw = _linear_sizes(x, w, act, "linear")
+    t, dev = x.dtype, x.device
+    a = L.LinearArgs(
+        rows, k, n, dt, act, slope, x.data_ptr(), ldx, w.data_ptr(), ldw,
+        None if bias is None else _flat(bias, n, "linear", "bias", t, dev),
+        None if residual is None else residual.data_ptr(),
+        0 if residual is None else _matrix(residual, rows, n, "linear", "residual", t, dev),
+        y.data_ptr(), _matrix(y, rows, n, "linear", "y", t, dev),
+        None if preact is None else _flat(preact, rows * n, "linear", "preact", linear_preact_dtype(t), dev))
     ref = ctypes.byref(a)
-    ws = _workspace(ws, int(L.load().cgan3d_linear_fwd_ws_bytes(ref)), "linear", dev)
-    check(_launch_on(dev, "cgan3d_linear_fwd", ref, ptr(ws), 0 if ws is None else ws.numel()), "linear")
+    ws = _workspace(ws, L.load().cgan3d_linear_fwd_ws_bytes(ref), "linear", dev)
+    if ws is None:
+        rc = _launch_on(dev, "cgan3d_linear_fwd", ref, None, 0)
+    else:
+        rc = _launch_on(dev, "cgan3d_linear_fwd", ref, ws.data_ptr(), ws.numel())
+    check(rc, "linear")
 
 
 def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
     """Gradients of ``linear`` (cgan3d_linear_bwd) into those of ``dx`` [rows, k], ``dw`` [n, k] and
     ``dbias`` [n] that are given (overwritten); ``preact`` is the forward call's (not needed without an
     activation).  The residual's gradient is dy itself."""
-    a = _linear_args(x, w, act, slope, "linear_backward")
-    dev = x.device
-    a.dy, a.lddy = dy.data_ptr(), _matrix(dy, a.rows, a.n, "linear_backward dy", x.dtype, dev)
-    if act != L.ACT_NONE:
-        if preact is None:
-            raise ValueError("linear_backward: the activation's gradient needs the forward call's preact")
-        _flat(preact, a.rows * a.n, "linear_backward preact", linear_preact_dtype(x.dtype), dev)
-        a.preact = preact.data_ptr()
-    if dx is not None:
-        a.dx, a.lddx = dx.data_ptr(), _matrix(dx, a.rows, a.k, "linear_backward dx", x.dtype, dev)
+    rows, k, n, dt, ldx, ldw = _linear_sizes(x, w, act, "linear_backward")
+    t, dev = x.dtype, x.device
+    if act != L.ACT_NONE and preact is None:
+        raise ValueError("linear_backward: the activation's gradient needs the forward call's preact")
     if dw is not None:
-        _matrix(dw, a.n, a.k, "linear_backward dw", x.dtype, dev)
-        _flat(dw, a.n * a.k, "linear_backward dw", x.dtype, dev)
-        a.dw = dw.data_ptr()
-    if dbias is not None:
-        _flat(dbias, a.n, "linear_backward dbias", x.dtype, dev)
-        a.dbias = dbias.data_ptr()
+        _matrix(dw, n, k, "linear_backward", "dw", t, dev)
+    a = L.LinearArgs(
+        rows, k, n, dt, act, slope, x.data_ptr(), ldx, w.data_ptr(), ldw, None, None, 0, None, 0,
+        None if act == L.ACT_NONE else _flat(preact, rows * n, "linear_backward", "preact", linear_preact_dtype(t), dev),
+        dy.data_ptr(), _matrix(dy, rows, n, "linear_backward", "dy", t, dev),
+        None if dx is None else dx.data_ptr(),
+        0 if dx is None else _matrix(dx, rows, k, "linear_backward", "dx", t, dev),
+        None if dw is None else _flat(dw, n * k, "linear_backward", "dw", t, dev),
+        None if dbias is None else _flat(dbias, n, "linear_backward", "dbias", t, dev))
     ref = ctypes.byref(a)
-    ws = _workspace(ws, int(L.load().cgan3d_linear_bwd_ws_bytes(ref)), "linear_backward", dev)
-    check(_launch_on(dev, "cgan3d_linear_bwd", ref, ptr(ws), 0 if ws is None else ws.numel()), "linear_backward")
+    ws = _workspace(ws, L.load().cgan3d_linear_bwd_ws_bytes(ref), "linear_backward", dev)
+    if ws is None:
+        rc = _launch_on(dev, "cgan3d_linear_bwd", ref, None, 0)
+    else:
+        rc = _launch_on(dev, "cgan3d_linear_bwd", ref, ws.data_ptr(), ws.numel())
+    check(rc, "linear_backward")
 
 
 def _ns_args(steps, coefficients, eps, what):
@@ -1642,9 +1651,11 @@ def muon_step(param, grad, momentum, exp_avg_sq, segs: MuonSegments, hyper, step
     include/cgan3d.h."""
     dev = param.device
     _dt(param, "muon_step param")
-    for t, nm in ((param, "param"), (grad, "grad"), (momentum, "momentum"), (exp_avg_sq, "exp_avg_sq")):
-        _flat(t, segs.numel, f"muon_step {nm}", torch.float32, dev)
-    _flat(hyper, 10, "muon_step hyper", torch.float32, dev)
+    at = [_flat(t, segs.numel, "muon_step", nm, torch.float32, dev)
+          for t, nm in ((param, "param"), (grad, "grad"), (momentum, "momentum"), (exp_avg_sq, "exp_avg_sq"))]
+    if len(set(at)) < 4 and segs.numel:
+        raise ValueError("muon_step: param, grad, momentum and exp_avg_sq must be four tensors")
+    _flat(hyper, 10, "muon_step", "hyper", torch.float32, dev)
     steps, co, eps = _ns_args(steps, coefficients, eps, "muon_step")
     ws = _workspace(ws, segs.ws_bytes(), "muon_step", dev)
     check(_launch_on(dev, "cgan3d_muon_step", ptr(param), ptr(grad), ptr(momentum), ptr(exp_avg_sq), segs.c, segs.n,
