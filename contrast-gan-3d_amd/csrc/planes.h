@@ -46,6 +46,13 @@ template <class E, int N> struct PlaneJobs {
   PlaneJob<E> j[N];
 };
 
+// The job of block b: a lane looks at each start, since a trip to the arguments costs about half a microsecond.
+template <class E, int N> __device__ __forceinline__ int plane_job(const PlaneJobs<E, N>& jobs, int b) {
+  if constexpr (N == 1) return 0;
+  const int lane = threadIdx.x & 63;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < jobs.n && b >= jobs.start[min(lane, N)])) - 1);
+}
+
 // XOR of a chunk's place by its row.  t-contiguous rows of 64 or 128 bytes: 16 lanes read one chunk of 16
 // neighbouring rows, which then lie in 16 different 16-byte columns of the 256-byte bank space.  t-strided
 // rows: a wave reads 32 bytes of rows 8 g + 4 h + (0..3), g = 0..3: the eight rows of a half wave get eight
@@ -163,9 +170,8 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
   static_assert(FM >= 2, "two rows of fragments behind the barrier");
   __shared__ __align__(16) unsigned char lds[S * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int b = xcd_order(blockIdx.x, gridDim.x), jn = 0;
-  if constexpr (N > 1)
-    while (jn + 1 < jobs.n && b >= jobs.start[jn + 1]) ++jn;
+  int b = xcd_order(blockIdx.x, gridDim.x);
+  const int jn = plane_job(jobs, b);
   const PlaneJob<E>& p = jobs.j[jn];
   b -= jobs.start[jn];
   const int split = b / p.tiles, t = b - split * p.tiles;
@@ -377,9 +383,8 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
 template <int BM, int BN, bool SYM, class E, int N>
 __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
   constexpr int SUB = BM / 32;
-  int b = blockIdx.x, jn = 0;
-  if constexpr (N > 1)
-    while (jn + 1 < jobs.n && b >= jobs.start[jn + 1]) ++jn;
+  int b = blockIdx.x;
+  const int jn = plane_job(jobs, b);
   const PlaneJob<E>& p = jobs.j[jn];
   b -= jobs.start[jn];
   if (!p.part) return;
@@ -409,22 +414,22 @@ struct PlanePick {
 // blocks where there are few
 template <int P, bool SYM = false> struct PlaneCfg;
 template <> struct PlaneCfg<1, false> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 5};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 8};
   static constexpr bool AHEAD[3] = {true, true, true};
   static constexpr float RATE[3] = {1.f, 0.75f, 0.4f};
 };
 template <> struct PlaneCfg<2, false> {
-  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {3, 3, 3};
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {3, 4, 5};
   static constexpr bool AHEAD[3] = {true, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<2, true> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 3};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 4, 5};
   static constexpr bool AHEAD[3] = {false, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<3, false> {
-  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 3};
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 4};
   static constexpr bool AHEAD[3] = {false, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
