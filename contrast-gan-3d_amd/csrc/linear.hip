@@ -84,6 +84,60 @@ template <typename T, bool NANFIX> struct LinEpi {
     for (long long t = 0; t < K; ++t) s = fmaf(a.at(i, t), b.at(j, t), s);
     return s;
   }
+  // V: all four columns are there and every tensor takes them as one vector
+  template <int STEP, bool V> __device__ __forceinline__ void put4_as(int i, int j, f32x4_m* v, int I, int jn) const {
+    typedef typename PreT<T>::type preT;
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    // as they are until they are needed; columns that are not there: the last one again, without a branch (a
+    // load under a branch is waited for by itself)
+    const auto fetch = [&](const T* row) {
+      v4 x;
+      if (V) return *reinterpret_cast<const v4*>(row + j);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = row[j + min(r, jn - 1)];
+      return x;
+    };
+    v4 res[4], bias;
+    if (e.bias) bias = fetch(static_cast<const T*>(e.bias));
+    if (e.residual) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) res[u] = fetch(static_cast<const T*>(e.residual) + min(i + u * STEP, I - 1) * e.ldr);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v[u] *= e.alpha;
+      if (e.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[u][r] += to_f(bias[r]);
+      }
+      if (e.preact && i + u * STEP < I) {
+        typedef preT p4 __attribute__((ext_vector_type(4)));
+        preT* o = static_cast<preT*>(e.preact) + (i + u * STEP) * J + j;
+        p4 p;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          preT q;
+          mat_preact(&q, v[u][r]);
+          p[r] = q;
+        }
+        if (V) *reinterpret_cast<p4*>(o) = p;
+        else
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < jn) o[r] = p[r];
+      }
+    }
+    mat_act16<T>(reinterpret_cast<float*>(v), e.act, e.slope);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i + u * STEP >= I) continue;
+      if (e.residual) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[u][r] += e.beta * to_f(res[u][r]);
+      }
+      store4(static_cast<T*>(e.out) + (i + u * STEP) * e.ldo + j, v[u], jn, V);
+    }
+  }
   // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store, so that they are in
   // flight together
   template <int STEP>
@@ -95,51 +149,8 @@ template <typename T, bool NANFIX> struct LinEpi {
         for (int r = 0; r < 4; ++r)
           if (i + u * STEP < I && r < jn && v[u][r] != v[u][r]) v[u][r] = again(i + u * STEP, j + r);
     }
-    if (jn < 4 || !vec) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (i + u * STEP < I && r < jn) mat_store<T>(e, J, i + u * STEP, j + r, v[u][r]);
-      return;
-    }
-    typedef T v4 __attribute__((ext_vector_type(4)));
-    typedef typename PreT<T>::type preT;
-    typedef preT p4 __attribute__((ext_vector_type(4)));
-    v4 res[4], bias;
-    if (e.bias) bias = *reinterpret_cast<const v4*>(static_cast<const T*>(e.bias) + j);
-    if (e.residual) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        res[u] = *reinterpret_cast<const v4*>(static_cast<const T*>(e.residual) + min(i + u * STEP, I - 1) * e.ldr + j);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      v[u] *= e.alpha;
-      if (e.bias) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[u][r] += to_f(bias[r]);
-      }
-      if (e.preact && i + u * STEP < I) {
-        p4 p;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          preT q;
-          mat_preact(&q, v[u][r]);
-          p[r] = q;
-        }
-        *reinterpret_cast<p4*>(static_cast<preT*>(e.preact) + (i + u * STEP) * J + j) = p;
-      }
-    }
-    mat_act16<T>(reinterpret_cast<float*>(v), e.act, e.slope);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (i + u * STEP >= I) continue;
-      v4 o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = from_f<T>(e.residual ? v[u][r] + e.beta * to_f(res[u][r]) : v[u][r]);
-      *reinterpret_cast<v4*>(static_cast<T*>(e.out) + (i + u * STEP) * e.ldo + j) = o;
-    }
+    if (jn >= 4 && vec) put4_as<STEP, true>(i, j, v, I, 4);
+    else put4_as<STEP, false>(i, j, v, I, jn);
   }
   __device__ __forceinline__ bool turned() const { return false; }
   __device__ __forceinline__ void put_turned(int, int, f32x4_m, int) const {}
@@ -402,8 +413,8 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int n, i
 
 template <typename T, int NT, int KS>
 __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
-                                                       long long ldw, long long rows, int n, int k, int vecx, int vece,
-                                                       MatEpi e) {
+                                                       long long ldw, long long rows, int n, int k, int vecx, int vecw,
+                                                       int vece, MatEpi e) {
   typedef T v4 __attribute__((ext_vector_type(4)));
   typedef typename PreT<T>::type preT;
   typedef preT p4 __attribute__((ext_vector_type(4)));
@@ -414,7 +425,7 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int j = t * 16 + row, c = s * 32 + g * 8;
-      load8(w + (long long)min(j, n - 1) * ldw + c, j < n ? k - c : 0, 0, fw[t][s]);
+      load8(w + (long long)min(j, n - 1) * ldw + c, j < n ? k - c : 0, vecw, fw[t][s]);
     }
   v4 bias[NT] = {};
   if (e.bias)
@@ -652,10 +663,11 @@ int rows_blocks(const cgan3d_linear_args* a) { return (int)std::min<long long>((
 template <typename T, int NT> void rows_fwd_nt(const MatArgs& p, int vecx, int vece, hipStream_t st) {
   const T* x = static_cast<const T*>(p.a);
   const T* w = static_cast<const T*>(p.b);
+  const int vecw = reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.ldb % MatT<T>::VEC == 0;
   // four waves a block; enough blocks to fill the card, each wave going on from there
   const unsigned blocks = (unsigned)std::min((p.I + 63) / 64, 8LL * cu_count());
-  if (p.K <= 32) launch(rows_fwd_kernel<T, NT, 1>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vece, p.e);
-  else launch(rows_fwd_kernel<T, NT, 2>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vece, p.e);
+  if (p.K <= 32) launch(rows_fwd_kernel<T, NT, 1>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vecw, vece, p.e);
+  else launch(rows_fwd_kernel<T, NT, 2>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vecw, vece, p.e);
 }
 template <typename T> void rows_fwd_run(const MatArgs& p, hipStream_t st) {
   const int vecx = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % MatT<T>::VEC == 0;

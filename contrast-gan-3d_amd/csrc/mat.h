@@ -50,6 +50,35 @@ __device__ __forceinline__ f32x4_m mfma_8(const float* a, const float* b, f32x4_
   return c;
 }
 
+// n of four neighbours (more than four: all); vec: they are aligned where all four are there
+template <typename T> __device__ __forceinline__ f32x4_m load4(const T* p, int n, int vec) {
+  f32x4_m v = {0.f, 0.f, 0.f, 0.f};
+  if (n >= 4 && vec) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    const v4 x = *reinterpret_cast<const v4*>(p);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = to_f(x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) v[r] = to_f(p[r]);
+  }
+  return v;
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, f32x4_m v, int n, int vec) {
+  if (n >= 4 && vec) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    v4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = from_f<T>(v[r]);
+    *reinterpret_cast<v4*>(p) = x;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) p[r] = from_f<T>(v[r]);
+  }
+}
+
 // --- activations of the linear block (all in 32 bits) ---
 // FAST: for 16-bit tensors, whose own rounding (2^-9 or 2^-12 of a value) hides the 2^-20 or so that these forms
 // lose; the library's functions for f32 tensors.  On a 256 x 256 tile they are 16 k cycles against 61 k with erff.

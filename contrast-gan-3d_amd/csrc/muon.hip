@@ -549,35 +549,6 @@ __device__ __forceinline__ int slab_t(bool tall, int u, int tid) {
   const int q = u * kSlabThreads + tid;
   return tall ? q / 16 : q % (kCols / 4) * 4;
 }
-// n of four neighbours (more than four: all); vec: they are aligned where all four are there
-template <typename T> __device__ __forceinline__ f32x4_m load4(const T* p, int n, int vec) {
-  f32x4_m v = {0.f, 0.f, 0.f, 0.f};
-  if (n >= 4 && vec) {
-    typedef T v4 __attribute__((ext_vector_type(4)));
-    const v4 x = *reinterpret_cast<const v4*>(p);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = to_f(x[r]);
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r < n) v[r] = to_f(p[r]);
-  }
-  return v;
-}
-template <typename T> __device__ __forceinline__ void store4(T* p, f32x4_m v, int n, int vec) {
-  if (n >= 4 && vec) {
-    typedef T v4 __attribute__((ext_vector_type(4)));
-    v4 x;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = from_f<T>(v[r]);
-    *reinterpret_cast<v4*>(p) = x;
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r < n) p[r] = from_f<T>(v[r]);
-  }
-}
-
 // PHASE 0: launch 0, 1: a step that is not the last, 2: the last
 template <typename T, int PHASE>
 __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, float ca, float cb, float cc, float eps,

@@ -414,22 +414,22 @@ struct PlanePick {
 // blocks where there are few
 template <int P, bool SYM = false> struct PlaneCfg;
 template <> struct PlaneCfg<1, false> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 8};
-  static constexpr bool AHEAD[3] = {true, true, true};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK[3] = {32, 32, 64}, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 4};
+  static constexpr bool AHEAD[3] = {true, true, false};
   static constexpr float RATE[3] = {1.f, 0.75f, 0.4f};
 };
 template <> struct PlaneCfg<2, false> {
-  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {3, 4, 5};
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK[3] = {32, 32, 32}, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {3, 4, 5};
   static constexpr bool AHEAD[3] = {true, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<2, true> {
-  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 4, 5};
+  static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK[3] = {32, 32, 32}, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 4, 5};
   static constexpr bool AHEAD[3] = {false, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
 template <> struct PlaneCfg<3, false> {
-  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK = 32, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 4};
+  static constexpr int BM[3] = {128, 128, 64}, BN[3] = {256, 128, 64}, BK[3] = {32, 32, 32}, WI[3] = {2, 2, 2}, WJ[3] = {4, 4, 2}, S[3] = {2, 3, 4};
   static constexpr bool AHEAD[3] = {false, true, true};
   static constexpr float RATE[3] = {1.f, 0.8f, 0.5f};
 };
@@ -453,7 +453,7 @@ template <int P, bool sym> PlanePick plane_pick(const PlaneShape* s, int n) {
   for (int c = 0; c < 3; ++c) {
     int last = 0;
     for (int sp = 1; sp <= 64; ++sp) {
-      const int kc = ((kmax + sp - 1) / sp + C::BK - 1) / C::BK * C::BK;
+      const int kc = ((kmax + sp - 1) / sp + 63) / 64 * 64;
       if (kc == last) continue;
       last = kc;
       double blocks = 0;
@@ -472,7 +472,7 @@ template <int P, bool sym> PlanePick plane_pick(const PlaneShape* s, int n) {
         best.kchunk = kc;
         best.part_floats = part;
       }
-      if (kc <= 4 * C::BK || blocks >= 2 * cus) break;
+      if (kc <= 128 || blocks >= 2 * cus) break;
     }
   }
   return best;
@@ -502,7 +502,7 @@ void plane_run(PlaneJobs<E, N>& jobs, const PlanePick& pick, float* part, hipStr
       jat += j.tiles * (BM / 32);
     }
     if (at == 0) return;
-    launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK, C::S[c], C::WI[c], C::WJ[c], C::AHEAD[c], SYM, E, N>, dim3(at),
+    launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK[c], C::S[c], C::WI[c], C::WJ[c], C::AHEAD[c], SYM, E, N>, dim3(at),
            dim3(C::WI[c] * C::WJ[c] * 64), 0, st, jobs);
     if (join) launch(plane_join_kernel<BM, BN, SYM, E, N>, dim3(jat), dim3(256), 0, st, js);
   };
