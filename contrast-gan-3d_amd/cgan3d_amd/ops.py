@@ -1510,7 +1510,7 @@ LINEAR_ACTS = (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU, L.ACT_TANH, L.ACT_GELU, L.AC
 
 def linear_preact_dtype(dtype):
     """dtype of the pre-activation kept for the backward pass (include/cgan3d.h cgan3d_linear_args)."""
-    return torch.float32 if dtype == torch.float32 else torch.float16
+    return torch.float16 if dtype == torch.bfloat16 else torch.float32
 
 
 def _linear_sizes(x, w, act, who):

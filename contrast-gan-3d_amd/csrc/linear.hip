@@ -24,6 +24,7 @@ namespace {
 constexpr int kTile = 64;
 
 int dt_bytes(int dt) { return dt == CGAN3D_DT_F32 ? 4 : 2; }
+int pre_bytes(int dt) { return dt == CGAN3D_DT_BF16 ? 2 : 4; }
 
 // Splits of the summed axis: as many as fill the card twice, each at least 256 values long.
 int mat_splits(long long I, long long J, long long K) {
@@ -290,7 +291,7 @@ void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStr
   j.e.e = m.e;
   j.e.J = m.J;
   j.e.vec = vec4(m.e.bias, 4, sizeof(T)) && vec4(m.e.residual, m.e.ldr, sizeof(T)) && vec4(m.e.out, m.e.ldo, sizeof(T)) &&
-            vec4(m.e.preact, m.J, sizeof(T));
+            vec4(m.e.preact, m.J, sizeof(typename PreT<T>::type));
   if constexpr (P == 3) {
     j.e.a = {static_cast<const bf16_t*>(a.p), a.rows * a.ld, a.strided ? 1 : a.ld, a.strided ? a.ld : 1};
     j.e.b = {static_cast<const bf16_t*>(b.p), b.rows * b.ld, b.strided ? 1 : b.ld, b.strided ? b.ld : 1};
@@ -672,7 +673,7 @@ template <typename T, int NT> void rows_fwd_nt(const MatArgs& p, int vecx, int v
 template <typename T> void rows_fwd_run(const MatArgs& p, hipStream_t st) {
   const int vecx = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % MatT<T>::VEC == 0;
   const int vece = p.J % 4 == 0 && vec4(p.e.residual, p.e.ldr, sizeof(T)) && vec4(p.e.out, p.e.ldo, sizeof(T)) &&
-                   vec4(p.e.preact, p.J, sizeof(T));
+                   vec4(p.e.preact, p.J, sizeof(typename PreT<T>::type));
   if (p.J <= 16) rows_fwd_nt<T, 1>(p, vecx, vece, st);
   else if (p.J <= 32) rows_fwd_nt<T, 2>(p, vecx, vece, st);
   else rows_fwd_nt<T, 4>(p, vecx, vece, st);
@@ -681,7 +682,7 @@ template <typename T> void rows_fwd_run(const MatArgs& p, hipStream_t st) {
 template <typename T, int NT, int KT> void rows_bwd_nk(const cgan3d_linear_args* a, float* part, hipStream_t st) {
   typedef typename PreT<T>::type preT;
   const int b = sizeof(T);
-  const int vecy = a->n % 4 == 0 && vec4(a->dy, a->lddy, b) && vec4(a->act != CGAN3D_ACT_NONE ? a->preact : nullptr, a->n, b);
+  const int vecy = a->n % 4 == 0 && vec4(a->dy, a->lddy, b) && vec4(a->act != CGAN3D_ACT_NONE ? a->preact : nullptr, a->n, sizeof(preT));
   const int vecx = a->k % 4 == 0 && vec4(a->x, a->ldx, b), vecd = a->k % 4 == 0 && vec4(a->dx, a->lddx, b);
   launch(rows_bwd_kernel<T, NT, KT>, dim3(rows_blocks(a)), dim3(256), 0, st, static_cast<const T*>(a->dy), (long long)a->lddy,
          static_cast<const preT*>(a->preact), static_cast<const T*>(a->x), (long long)a->ldx, static_cast<const T*>(a->w),
@@ -818,7 +819,7 @@ template <typename T, bool PL3>
 void act_grad_run(const cgan3d_linear_args* a, void* dz, int ldz, float* part, hipStream_t st) {
   const ActGrid g = act_grid(a);
   const int vec = reinterpret_cast<uintptr_t>(a->dy) % 16 == 0 && a->lddy % MatT<T>::VEC == 0 &&
-                  (a->act == CGAN3D_ACT_NONE || (reinterpret_cast<uintptr_t>(a->preact) % 16 == 0 && a->n % MatT<T>::VEC == 0));
+                  (a->act == CGAN3D_ACT_NONE || (reinterpret_cast<uintptr_t>(a->preact) % 32 == 0 && a->n % MatT<T>::VEC == 0));
   if (g.nb > 0 && a->n > 0)
     launch(act_grad_kernel<T, PL3>, dim3(g.bx, (unsigned)g.nb), dim3(256), 0, st, static_cast<const T*>(a->dy),
            (long long)a->lddy, static_cast<const typename PreT<T>::type*>(a->preact), dz, ldz, part, (long long)a->rows,
@@ -937,7 +938,7 @@ extern "C" int cgan3d_linear_fwd(const cgan3d_linear_args* a, void* ws, int64_t 
   const long long need = fwd_bytes(a);
   CG_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
                "cgan3d_linear_fwd: workspace of %lld bytes (16-byte aligned) needed, got %lld", need, (long long)ws_bytes);
-  const int b = dt_bytes(a->dtype), pb = a->dtype == CGAN3D_DT_F32 ? 4 : 2;
+  const int b = dt_bytes(a->dtype), pb = pre_bytes(a->dtype);
   const Span y = span(a->y, a->rows, a->n, a->ldy, b), z = span(a->preact, a->rows, a->n, a->n, pb);
   const Span x = span(a->x, a->rows, a->k, a->ldx, b), w = span(a->w, a->n, a->k, a->ldw, b);
   const Span r = span(a->residual, a->rows, a->n, a->ldr, b), bi = span(a->bias, 1, a->n, a->n, b);
@@ -989,7 +990,7 @@ extern "C" int cgan3d_linear_bwd(const cgan3d_linear_args* a, void* ws, int64_t 
   const int b = dt_bytes(a->dtype);
   const Span in[] = {span(a->x, a->rows, a->k, a->ldx, b), span(a->w, a->n, a->k, a->ldw, b),
                      span(a->dy, a->rows, a->n, a->lddy, b),
-                     a->act != CGAN3D_ACT_NONE ? span(a->preact, a->rows, a->n, a->n, b) : Span{0, 0}};
+                     a->act != CGAN3D_ACT_NONE ? span(a->preact, a->rows, a->n, a->n, pre_bytes(a->dtype)) : Span{0, 0}};
   const Span out[] = {span(a->dx, a->rows, a->k, a->lddx, b), span(a->dw, a->n, a->k, a->k, b),
                       span(a->dbias, 1, a->n, a->n, b)};
   for (int o = 0; o < 3; ++o) {

@@ -587,8 +587,8 @@ int cgan3d_adam(float* param, const float* grad, float* exp_avg, float* exp_avg_
  * epilogue.  Rows may be strided (ld*, elements; at least the row's length); preact, dz, dw and dbias are
  * contiguous.  Any size, zero included, and any alignment of whole elements.
  *   forward : x, w, y; optional bias [n], residual (may be y itself), preact.
- *             preact [rows, n], f32 for f32 tensors and f16 for 16-bit ones (saturating): z = x w^T + bias,
- *             which the backward pass of an activation reads.
+ *             preact [rows, n], f32, or f16 (saturating) for bf16 tensors: z = x w^T + bias, which the backward
+ *             pass of an activation reads.
  *   backward: dy, x (for dw), w (for dx), preact (unless act is none); outputs dx, dw, dbias, each
  *             optional.  dz = dy * act'(z), dx = dz w, dw = dz^T x, dbias = column sums of dz (f32, before
  *             dz's rounding).  The residual's gradient is dy.  All sums run in a fixed order.

@@ -6,8 +6,8 @@ the products' magnitudes and the bias's (the slack of 4: the bias's addition, th
 An activation passes an error on with at most its slope (below 1.13 for all of them) and adds a few u of
 its own; the residual's addition adds u |y|; the store adds e |y|, for f16 at least half its smallest step.
 Backward: dz = dy act'(z) is rounded to the type (e |dz|), and act'(z) is off by max |act''(z)| |z err|: for
-16-bit types z is kept as an f16 (2^-11 |z|, and |z act''(z)| < 1 for every activation here), for f32 it is
-off by the forward sum's error (|act''| < 1.2).  ReLU and LeakyReLU, whose derivative jumps, get inputs on
+bf16 z is kept as an f16 (2^-11 |z|, and |z act''(z)| < 1 for every activation here), otherwise it is off by
+the forward sum's error (|act''| < 1.2); the short forms for 16-bit tensors are good to 2^-19.  ReLU and LeakyReLU, whose derivative jumps, get inputs on
 a grid on which z is exact and never nearer to 0 than 1/64.
 """
 import math
@@ -87,10 +87,10 @@ def reference(x, w, b, r, dy, dt, act):
     dz, = torch.autograd.grad(a, q, dy)
     if act in ("none", "relu", "lrelu"):
         gerr = 4 * U * dz.abs()
-    elif dt == "f32":
-        gerr = dy.abs() * (1.2 * zerr + 16 * U)
+    elif dt == "bf16":
+        gerr = dy.abs() * (2.0 ** -11 + 1.2 * zerr + 2.0 ** -19)
     else:
-        gerr = dy.abs() * (2.0 ** -11 + 1.2 * zerr + 16 * U)
+        gerr = dy.abs() * (1.2 * zerr + (16 * U if dt == "f32" else 2.0 ** -19))
     raw = gerr
     if act != "none":
         gerr = gerr * 1.01 + e * dz.abs() * 1.01 + low
