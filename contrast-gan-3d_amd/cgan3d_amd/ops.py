@@ -1494,15 +1494,10 @@ def _workspace(ws, need, what, device):
     return ws
 
 
-def _launch_on(device, name, *args):
-    """``_launch`` on ``device``'s current stream, whichever device is current."""
-    if DRY_RUN:
-        return 0
-    i = device.index
-    if i is None or i == torch.cuda.current_device():
-        return getattr(L.lib(), name)(*args, L.stream())
-    with torch.cuda.device(device):
-        return getattr(L.lib(), name)(*args, L.stream())
+def _elsewhere(device):
+    """Whether ``device`` is a GPU other than the current one (workspace sizes go by the current device, and
+    launches go to its stream)."""
+    return not DRY_RUN and device.index is not None and device.index != torch.cuda.current_device()
 
 
 LINEAR_ACTS = (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU, L.ACT_TANH, L.ACT_GELU, L.ACT_SILU)
@@ -1530,6 +1525,9 @@ def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=
     (``linear_preact_dtype``) receives x w^T + bias for ``linear_backward``.  y may be the residual."""
     rows, k, n, dt, ldx, ldw = _linear_sizes(x, w, act, "linear")
     t, dev = x.dtype, x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return linear(x, w, y, bias, residual, act, slope, preact, ws)
     a = L.LinearArgs(
         rows, k, n, dt, act, slope, x.data_ptr(), ldx, w.data_ptr(), ldw,
         None if bias is None else _flat(bias, n, "linear", "bias", t, dev),
@@ -1540,9 +1538,9 @@ def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=
     ref = ctypes.byref(a)
     ws = _workspace(ws, L.load().cgan3d_linear_fwd_ws_bytes(ref), "linear", dev)
     if ws is None:
-        rc = _launch_on(dev, "cgan3d_linear_fwd", ref, None, 0)
+        rc = _launch("cgan3d_linear_fwd", ref, None, 0)
     else:
-        rc = _launch_on(dev, "cgan3d_linear_fwd", ref, ws.data_ptr(), ws.numel())
+        rc = _launch("cgan3d_linear_fwd", ref, ws.data_ptr(), ws.numel())
     check(rc, "linear")
 
 
@@ -1552,6 +1550,9 @@ def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slop
     activation).  The residual's gradient is dy itself."""
     rows, k, n, dt, ldx, ldw = _linear_sizes(x, w, act, "linear_backward")
     t, dev = x.dtype, x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return linear_backward(dy, x, w, dx, dw, dbias, act, slope, preact, ws)
     if act != L.ACT_NONE and preact is None:
         raise ValueError("linear_backward: the activation's gradient needs the forward call's preact")
     if dw is not None:
@@ -1567,9 +1568,9 @@ def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slop
     ref = ctypes.byref(a)
     ws = _workspace(ws, L.load().cgan3d_linear_bwd_ws_bytes(ref), "linear_backward", dev)
     if ws is None:
-        rc = _launch_on(dev, "cgan3d_linear_bwd", ref, None, 0)
+        rc = _launch("cgan3d_linear_bwd", ref, None, 0)
     else:
-        rc = _launch_on(dev, "cgan3d_linear_bwd", ref, ws.data_ptr(), ws.numel())
+        rc = _launch("cgan3d_linear_bwd", ref, ws.data_ptr(), ws.numel())
     check(rc, "linear_backward")
 
 
@@ -1590,6 +1591,9 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
     if g.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("orthogonalize has no gradient: call it under torch.no_grad() or on g.detach()")
     dt, dev = _dt(g, "orthogonalize g"), g.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return orthogonalize(g, steps, coefficients, eps, out, ws)
     rows, cols = g.shape[-2:]
     src = g.detach()
     src = (src if src.is_contiguous() else src.contiguous()).view(-1, rows, cols) if g.numel() else src
@@ -1605,7 +1609,7 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
     mats = (L.OrthoMat * max(n, 1))(*[L.OrthoMat(e[0] + i * step, e[1] + i * step, cols, cols, rows, cols)
                                       for i in range(n)])
     ws = _workspace(ws, int(L.load().cgan3d_orthogonalize_ws_bytes(mats, n, dt)), "orthogonalize", dev)
-    check(_launch_on(dev, "cgan3d_orthogonalize", mats, n, dt, steps, co, eps, ptr(ws), 0 if ws is None else ws.numel()),
+    check(_launch("cgan3d_orthogonalize", mats, n, dt, steps, co, eps, ptr(ws), 0 if ws is None else ws.numel()),
           "orthogonalize")
     return out
 
@@ -1651,6 +1655,9 @@ def muon_step(param, grad, momentum, exp_avg_sq, segs: MuonSegments, hyper, step
     include/cgan3d.h."""
     dev = param.device
     _dt(param, "muon_step param")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return muon_step(param, grad, momentum, exp_avg_sq, segs, hyper, steps, coefficients, eps, ws)
     at = [_flat(t, segs.numel, "muon_step", nm, torch.float32, dev)
           for t, nm in ((param, "param"), (grad, "grad"), (momentum, "momentum"), (exp_avg_sq, "exp_avg_sq"))]
     if len(set(at)) < 4 and segs.numel:
@@ -1658,5 +1665,5 @@ def muon_step(param, grad, momentum, exp_avg_sq, segs: MuonSegments, hyper, step
     _flat(hyper, 10, "muon_step", "hyper", torch.float32, dev)
     steps, co, eps = _ns_args(steps, coefficients, eps, "muon_step")
     ws = _workspace(ws, segs.ws_bytes(), "muon_step", dev)
-    check(_launch_on(dev, "cgan3d_muon_step", ptr(param), ptr(grad), ptr(momentum), ptr(exp_avg_sq), segs.c, segs.n,
+    check(_launch("cgan3d_muon_step", ptr(param), ptr(grad), ptr(momentum), ptr(exp_avg_sq), segs.c, segs.n,
                      ptr(hyper), steps, co, eps, ptr(ws), 0 if ws is None else ws.numel()), "muon_step")

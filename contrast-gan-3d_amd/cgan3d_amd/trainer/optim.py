@@ -179,7 +179,9 @@ class FusedMuon(torch.optim.Optimizer):
         self.hyper = torch.tensor(self._host[:4] + [0.0, weight_clip or 0.0] + self._host[4:], dtype=torch.float32,
                                   device=dev)
         # owned: a plan or graph that holds a step keeps the address; steps of one optimiser are ordered anyway
-        self.ws = torch.empty(self.segs.ws_bytes(), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev if dev.type == "cuda" else None):  # its size goes by the current device
+            need = self.segs.ws_bytes()
+        self.ws = torch.empty(need, dtype=torch.uint8, device=dev)
         self._host_step = 0
 
     def _group_hyper(self):

@@ -882,7 +882,7 @@ const char* lin_check(const cgan3d_linear_args* a, bool bwd) {
   if (!a) return "null args";
   if (a->dtype < CGAN3D_DT_F32 || a->dtype > CGAN3D_DT_F16) return "unknown dtype";
   if (a->rows < 0 || a->k < 0 || a->n < 0) return "negative size";
-  if (a->rows > (1LL << 40)) return "too many rows";
+  if (a->rows > (1LL << 40) || a->k > 1 << 30 || a->n > 1 << 30) return "size too large";
   const long long t = (a->rows + kTile - 1) / kTile, u = ((long long)std::max(a->k, a->n) + kTile - 1) / kTile;
   if (t * u > INT_MAX || u * u > INT_MAX) return "too many tiles for one launch";
   if (a->act < CGAN3D_ACT_NONE || a->act > CGAN3D_ACT_SILU || a->act == CGAN3D_ACT_NEG_DTANH)

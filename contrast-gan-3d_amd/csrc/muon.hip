@@ -1006,7 +1006,7 @@ const char* mats_check(const cgan3d_ortho_mat* m, int n, int dt) {
   if (n < 0 || (n > 0 && !m)) return "null list";
   if (dt < CGAN3D_DT_F32 || dt > CGAN3D_DT_F16) return "unknown dtype";
   for (int i = 0; i < n; ++i) {
-    if (m[i].rows < 0 || m[i].cols < 0) return "negative size";
+    if (m[i].rows < 0 || m[i].cols < 0 || m[i].rows > 1 << 30 || m[i].cols > 1 << 30) return "negative or too large size";
     if ((long long)m[i].rows * m[i].cols == 0) continue;
     if (!m[i].g || !m[i].out) return "null matrix";
     if (m[i].ldg < m[i].cols || m[i].ldo < m[i].cols) return "row stride smaller than the row";
@@ -1074,8 +1074,8 @@ void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, cha
 const char* segs_check(const cgan3d_muon_seg* s, int n) {
   if (n < 0 || (n > 0 && !s)) return "null list";
   for (int i = 0; i < n; ++i) {
-    if (s[i].offset < 0 || s[i].rows < 0 || s[i].cols < 0 || s[i].rows > INT_MAX) return "negative or too large size";
-    if (s[i].rows > 0 && s[i].cols > INT_MAX) return "negative or too large size";
+    if (s[i].offset < 0 || s[i].rows < 0 || s[i].cols < 0 || s[i].rows > 1 << 30) return "negative or too large size";
+    if (s[i].rows > 0 && s[i].cols > 1 << 30) return "negative or too large size";
     if (s[i].rows > 0) {
       const long long t = (std::max(s[i].rows, s[i].cols) + 63) / 64, u = (std::min(s[i].rows, s[i].cols) + 63) / 64;
       if (t * u > INT_MAX) return "matrix too large for one launch";

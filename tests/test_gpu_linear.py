@@ -28,6 +28,8 @@ SHAPES = [  # rows, k, n
     (1, 1, 1), (1, 64, 64), (1, 257, 130), (2, 8, 3), (3, 4096, 40), (5, 33, 1), (8, 512, 1000), (17, 64, 64),
     (64, 32, 64), (65, 31, 63), (100, 1, 7), (128, 300, 128), (129, 129, 257), (256, 1024, 256), (333, 515, 77),
     (1000, 16, 32), (4096, 64, 48), (5000, 3, 5), (2049, 40, 8), (512, 640, 384), (300, 2048, 520),
+    # a few rows with many columns; f32 products that are split into planes (both gradients, one of them)
+    (1, 4096, 4096), (2, 100, 5000), (4, 65, 4099), (1500, 1000, 1203), (2048, 512, 1024), (8000, 1000, 100),
 ]
 
 
@@ -255,7 +257,7 @@ def test_strided_rows_leave_the_rest(rows, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", list(DT))
-@pytest.mark.parametrize("rows,k,n", [(1, 64, 40), (70, 100, 65), (300, 512, 256)])
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 40), (70, 60, 33), (70, 100, 65), (300, 512, 256), (1500, 1000, 1203)])
 def test_infinities_and_nans_stay_in_their_rows(rows, k, n, dt):
     from cgan3d_amd.model.linear import fused_linear
     x, w, b, r, _ = make(rows, k, n, dt, "none", 31)
@@ -278,13 +280,14 @@ def test_large_values_keep_their_size(dt):
     """Values near the top and the bottom of the type's range go through the product as they are."""
     from cgan3d_amd.model.linear import fused_linear
     g = torch.Generator().manual_seed(4)
-    for scale in (1e-30, 1e30):
-        x = (torch.randn(260, 384, generator=g) * scale).to(DT[dt])
-        w = torch.randn(300, 384, generator=g).to(DT[dt])
-        y = fused_linear(x.cuda(), w.cuda())
-        want = x.double() @ w.double().T
-        tol = (384 + 4) * U * (x.double().abs() @ w.double().abs().T) + half_step(dt) * 1.01 * want.abs()
-        check(y, want, tol, f"scale {scale}")
+    for m, k, n in ((260, 384, 300), (1500, 1000, 1203)):
+        for scale in (1e-30, 1e30):
+            x = (torch.randn(m, k, generator=g) * scale).to(DT[dt])
+            w = torch.randn(n, k, generator=g).to(DT[dt])
+            y = fused_linear(x.cuda(), w.cuda())
+            want = x.double() @ w.double().T
+            tol = (k + 4) * U * (x.double().abs() @ w.double().abs().T) + half_step(dt) * 1.01 * want.abs()
+            check(y, want, tol, f"{m}x{k}x{n}, scale {scale}")
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
@@ -385,3 +388,38 @@ def test_repeated_runs_are_equal():
             got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
             first = first or got
             assert all(torch.equal(a, e) for a, e in zip(got, first))
+
+
+@pytest.mark.parametrize("rows,k,n", [(6, 24, 16), (700, 96, 64), (1500, 1000, 1203)])
+def test_some_gradients(rows, k, n):
+    """Only what is asked for is computed, and it is what the full call gives."""
+    from cgan3d_amd import ops
+    x, w, b, _, dy = on_gpu(*make(rows, k, n, "f32", "gelu", 71))
+    y, pre = torch.empty(rows, n, device="cuda"), torch.empty(rows, n, device="cuda")
+    ops.linear(x, w, y, bias=b, act=code("gelu"), preact=pre)
+    full = dict(dx=torch.empty_like(x), dw=torch.empty_like(w), dbias=torch.empty_like(b))
+    ops.linear_backward(dy, x, w, **full, act=code("gelu"), preact=pre)
+    for names in (("dx",), ("dw",), ("dbias",), ("dx", "dbias"), ("dw", "dbias"), ("dx", "dw"), ()):
+        part = {nm: torch.full_like(full[nm], 3.0) for nm in names}
+        ops.linear_backward(dy, x, w, **part, act=code("gelu"), preact=pre)
+        for nm in names:
+            # the same sums in the same order, unless a product takes another form without its sibling
+            scale = float(full[nm].abs().max())
+            assert float((part[nm] - full[nm]).abs().max()) <= 1e-5 * scale, (names, nm)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams with workspaces of their own do not disturb each other."""
+    from cgan3d_amd.model.linear import fused_linear
+    args = [on_gpu(*make(640, 1024, 520, "bf16", "silu", 80 + i)) for i in range(2)]
+    wants = [fused_linear(*a[:3], residual=a[3], act=code("silu")) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(fused_linear(*args[i][:3], residual=args[i][3], act=code("silu")))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, wants[i]) for y in got[i])

@@ -57,7 +57,7 @@ def grad_like(*shape, seed=0, dtype=torch.float32):
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (1, 5488), (2, 3), (16, 343), (32, 432), (64, 1728), (1728, 64), (63, 65), (64, 64),
           (65, 64), (65, 66), (70, 129), (33, 1000), (129, 128), (128, 640), (200, 200), (333, 500), (500, 333),
-          (257, 1031), (512, 1024)]
+          (257, 1031), (512, 1024), (20, 9001), (8500, 33), (60, 20000)]
 
 
 @pytest.mark.parametrize("dt", list(DT))
@@ -66,6 +66,34 @@ def test_orthogonalize(shape, dt):
     from cgan3d_amd import ops
     g = grad_like(*shape, seed=shape[0] + 3 * shape[1], dtype=DT[dt])
     check_ns(ops.orthogonalize(g.cuda()), g, dt, f"{shape} {dt}")
+
+
+@pytest.mark.parametrize("shape", [(1100, 2304), (2301, 1030)])
+def test_orthogonalize_large(shape):
+    """The largest tiles, and a transposed result through them."""
+    from cgan3d_amd import ops
+    g = grad_like(*shape, seed=9)
+    check_ns(ops.orthogonalize(g.cuda()), g, "f32", f"{shape}")
+
+
+def test_orthogonalize_strided():
+    """Rows of a wider tensor, through the C entry point's row strides: what lies between stays."""
+    import ctypes
+    from cgan3d_amd import _lib as L
+    lib = L.lib()
+    for rows, cols in ((40, 70), (90, 130), (300, 45), (200, 120)):
+        g = grad_like(rows, cols, seed=3)
+        src = torch.full((rows, cols + 5), 7.0).cuda()
+        src[:, 2:2 + cols] = g.cuda()
+        out = torch.full((rows, cols + 9), 7.0).cuda()
+        m = (L.OrthoMat * 1)(L.OrthoMat(src[:, 2:].data_ptr(), out[:, 3:].data_ptr(), cols + 5, cols + 9, rows, cols))
+        need = lib.cgan3d_orthogonalize_ws_bytes(m, 1, L.DT_F32)
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        co = (ctypes.c_float * 3)(*NS)
+        L.check(lib.cgan3d_orthogonalize(m, 1, L.DT_F32, 5, co, 1e-7, ws.data_ptr(), need, L.stream()))
+        check_ns(out[:, 3:3 + cols], g, "f32", f"{rows}x{cols}")
+        out[:, 3:3 + cols] = 7.0
+        assert (out == 7.0).all()
 
 
 @pytest.mark.parametrize("shape", [(3, 20, 30), (2, 2, 40, 16), (5, 64, 200), (2, 130, 70), (4, 96, 256), (0, 8, 8),
