@@ -1238,9 +1238,9 @@ class StepEngine:
         # The generator's Adam in two parts: every layer whose gradients are complete when the
         # backward's side stream finishes its last weight grad (all but the first WGRAD_TAIL_MAIN
         # layers) is updated and repacked on the side stream beside the main stream's tail; the
-        # tail layers' parameters (a prefix of the arena) after it, with the step tick.  Adam (another
-        # optimiser updates the arena at once, _optim_step) and single
-        # GPU only (data parallelism all-reduces the whole gradient first).
+        # tail layers' parameters (a prefix of the arena) after it, with the step tick.  Adam only (another
+        # optimiser updates the arena at once, _optim_step), and a single GPU only (data parallelism
+        # all-reduces the whole gradient first).
         self.g_split = 0
         if self.G.side is not None and not self.dp and isinstance(g_optim, FusedAdam):
             pre = tuple(self.G.layers[li].name + "." for li in range(min(self.G.wgrad_tail_main, len(self.G.layers))))

@@ -16,6 +16,7 @@ Adam for the vectors (biases, BatchNorm scales and shifts), from one host call (
 from __future__ import annotations
 
 import math
+from contextlib import nullcontext
 from functools import partial
 
 import torch
@@ -179,7 +180,7 @@ class FusedMuon(torch.optim.Optimizer):
         self.hyper = torch.tensor(self._host[:4] + [0.0, weight_clip or 0.0] + self._host[4:], dtype=torch.float32,
                                   device=dev)
         # owned: a plan or graph that holds a step keeps the address; steps of one optimiser are ordered anyway
-        with torch.cuda.device(dev if dev.type == "cuda" else None):  # its size goes by the current device
+        with torch.cuda.device(dev) if dev.type == "cuda" else nullcontext():  # its size goes by the current device
             need = self.segs.ws_bytes()
         self.ws = torch.empty(need, dtype=torch.uint8, device=dev)
         self._host_step = 0
