@@ -64,7 +64,8 @@ void mat_run(int dt, const MatArgs& p, void* ws, hipStream_t st) {
 constexpr int kGemvRows = 4;
 
 // Epilogue of a plane product.  NANFIX (f32 on three planes): an infinity times an empty lower plane
-// is NaN, so a NaN sum is computed again value by value, which leaves what f32 gives.
+// is NaN, and a first plane that was rounded up can overflow where the value's own product does not, so a sum that is
+// not finite is computed again value by value, which leaves what f32 gives.
 template <typename T, bool NANFIX> struct LinEpi {
   static constexpr bool STAGED = true;
   MatEpi e;
@@ -82,7 +83,15 @@ template <typename T, bool NANFIX> struct LinEpi {
   long long K;
   __device__ __noinline__ float again(int i, int j) const {
     float s = 0.f;
-    for (long long t = 0; t < K; ++t) s = fmaf(a.at(i, t), b.at(j, t), s);
+    long long t = 0;
+    for (; t + 8 <= K && s == s; t += 8) {  // eight loads in flight; NaN stays NaN
+      float x[8], y[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = a.at(i, t + q), y[q] = b.at(j, t + q);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s = fmaf(x[q], y[q], s);
+    }
+    for (; t < K && s == s; ++t) s = fmaf(a.at(i, t), b.at(j, t), s);
     return s;
   }
   // V: all four columns are there and every tensor takes them as one vector
@@ -148,7 +157,7 @@ template <typename T, bool NANFIX> struct LinEpi {
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (i + u * STEP < I && r < jn && v[u][r] != v[u][r]) v[u][r] = again(i + u * STEP, j + r);
+          if (i + u * STEP < I && r < jn && !(fabsf(v[u][r]) < __builtin_inff())) v[u][r] = again(i + u * STEP, j + r);
     }
     if (jn >= 4 && vec) put4_as<STEP, true>(i, j, v, I, 4);
     else put4_as<STEP, false>(i, j, v, I, jn);

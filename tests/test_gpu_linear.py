@@ -281,7 +281,7 @@ def test_large_values_keep_their_size(dt):
     from cgan3d_amd.model.linear import fused_linear
     g = torch.Generator().manual_seed(4)
     for m, k, n in ((260, 384, 300), (1500, 1000, 1203)):
-        for scale in (1e-30, 1e30):
+        for scale in (1e-36, 1e-30, 1e30):
             x = (torch.randn(m, k, generator=g) * scale).to(DT[dt])
             w = torch.randn(n, k, generator=g).to(DT[dt])
             y = fused_linear(x.cuda(), w.cuda())
@@ -423,3 +423,20 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(y, wants[i]) for y in got[i])
+
+
+def test_f32_products_close_to_overflow():
+    """Products and sums just below f32's largest value stay finite, however the operands are held inside."""
+    from cgan3d_amd.model.linear import fused_linear
+    g = torch.Generator().manual_seed(91)
+    m, k, n = 1500, 1000, 1203
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros(m, k)
+    # values whose nearest bf16 lies above them: rounding them up and multiplying would overflow
+    x[:, 17] = 1.0 + (0.55 + 0.15 * torch.rand(m, generator=g)) * 2.0 ** -7
+    w = torch.randn(n, k, generator=g)
+    w[:, 17] = top / float(x[:, 17].max()) * (1 - 1e-6)
+    y = fused_linear(x.cuda(), w.cuda())
+    want = x.double() @ w.double().T
+    assert want.abs().max() < top
+    check(y, want, (k + 4) * U * want.abs(), "largest values")

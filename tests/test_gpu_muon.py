@@ -266,6 +266,30 @@ def test_muon_steps(kw):
         assert torch.allclose(m.double().cpu(), ref.m[i], rtol=1e-5, atol=1e-9)
 
 
+def test_muon_many_segments():
+    """More matrices (of both kinds) and vectors than one launch takes, and one whose slabs outnumber a block's."""
+    from cgan3d_amd.engine import Arena
+    from cgan3d_amd.trainer.optim import FusedMuon
+    gen = torch.Generator().manual_seed(7)
+    mod = torch.nn.Module()
+    shapes = [(5, 9001), (8200, 6)]
+    for i in range(33):
+        shapes += [(1 + i, 3 + 2 * i), (4 + i,)]  # a vector between two matrices is a segment of its own
+        if i % 2:
+            shapes += [(65 + i, 70 + 3 * i)]
+    mod.ps = torch.nn.ParameterList([torch.nn.Parameter(0.1 * torch.randn(s, generator=gen)) for s in shapes])
+    arena = Arena(mod.cuda(), torch.device("cuda"))
+    opt, ref = FusedMuon(arena, weight_decay=0.1), Ref(arena.params, weight_decay=0.1)
+    for t in range(2):
+        for i, p in enumerate(arena.params):
+            p.grad.copy_(grad_like(*p.shape, seed=200 * t + i) if p.dim() == 2 else
+                         1e-3 * torch.randn(p.shape, generator=gen))
+        opt.step()
+        ref.step([p.grad for p in arena.params])
+        ref.check(arena.params, f"step {t}")
+        assert float(opt.hyper[4]) == t + 1
+
+
 def test_muon_state_dict_and_scheduler():
     """A resumed optimiser goes on with the same bits; a scheduler drives both groups' rates."""
     from torch.optim.lr_scheduler import MultiStepLR
