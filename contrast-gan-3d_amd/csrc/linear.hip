@@ -8,7 +8,8 @@
 // apart from z itself where a backward pass will want it.
 //
 // Which kernel a product takes (mat_route):
-//   rows <= 4, forward     gemv_kernel: a wave per output column pair streams the weight once
+//   rows <= 2, forward      gemv_kernel: a wave per pair of output columns streams the weight once
+//   rows <= 16, forward     skinny_kernel: a wave per 16 columns, the weight straight into matrix instructions
 //   k, n <= 64              rows_fwd_kernel, rows_bwd_kernel: every row's values are read and written once
 //   16-bit tensors         plane_kernel (planes.h) on the tensors themselves; an operand whose rows are not
 //                          whole aligned 16-byte chunks is copied once into rows that are
@@ -26,7 +27,7 @@ constexpr int kTile = 64;
 int dt_bytes(int dt) { return dt == CGAN3D_DT_F32 ? 4 : 2; }
 int pre_bytes(int dt) { return dt == CGAN3D_DT_BF16 ? 2 : 4; }
 
-// Splits of the summed axis: as many as fill the card twice, each at least 256 values long.
+// Splits of mat_kernel's summed axis: as many as fill the card twice, each at least 256 values long.
 int mat_splits(long long I, long long J, long long K) {
   const long long tiles = std::max(1LL, ((I + kTile - 1) / kTile) * ((J + kTile - 1) / kTile));
   const long long want = 2LL * cu_count() / tiles, most = K / 256;
@@ -61,7 +62,6 @@ void mat_run(int dt, const MatArgs& p, void* ws, hipStream_t st) {
 }
 
 // --- products on planes ---
-constexpr int kGemvRows = 4;
 
 // Epilogue of a plane product.  NANFIX (f32 on three planes): an infinity times an empty lower plane
 // is NaN, and a first plane that was rounded up can overflow where the value's own product does not, so a sum that is
@@ -173,7 +173,8 @@ template <typename T, bool NANFIX> struct LinEpi {
 
 bool vec4(const void* p, long long ld, int elt) { return !p || (reinterpret_cast<uintptr_t>(p) % (4 * elt) == 0 && ld % 4 == 0); }
 
-// an operand as planes: copied (16-bit) or split (f32) into rows of whole chunks, padding zeroed
+// An operand as planes, both of a product in one launch (bound by memory, or by the launch: 777 x 1001 and 515 x 1001 of
+// f16 5.9 us).  Copied (16-bit) or split (f32) into rows of whole chunks, padding zeroed
 struct Pack {
   const void* src;
   long long ld, rows;
@@ -244,13 +245,17 @@ struct Operand {
 
 enum Route { ROUTE_MAT, ROUTE_PLANES };
 
-// f32: splitting both operands (4 bytes read, 6 written a value) and six 16-bit products at ~1000 TFLOP/s
-// against f32 instructions at ~80 (measured: 2048 x 1024 -> 4096, forward and backward, see DESIGN's table)
-Route mat_route(int dt, long long I, long long J, long long K) {
+// Whether an f32 product is better off on planes: six 16-bit products at ~200 TFLOP/s behind the splitting of both operands
+// (`ready`: of b, a's planes are there), against f32 instructions at ~95.  Measured, us, f32 instructions / planes:
+// rows x k -> n 2048 x 512 -> 1024 31 / 40, 8192 x 256 -> 256 19 / 31, 1024 x 1024 -> 1024 35 / 34, 512 x 2048 -> 2048
+// 60 / 54, 2048 x 1024 -> 4096 184 / 103; both gradients of 512 x 512 -> 512 40 / 49, of 1024 x 1024 -> 1024 85 / 70.
+bool f32_planes(long long I, long long J, long long K, bool ready) {
+  const double fl = 2.0 * I * J * K, pack = 10.0 * K * (ready ? J : I + J);
+  return fl / 95e12 > fl / 200e12 + pack / 4e12 + (ready ? 5e-6 : 9e-6);
+}
+Route mat_route(int dt, long long I, long long J, long long K, bool ready) {
   if (K == 0 || K >= 1 << 30 || I >= 1 << 30 || J >= 1 << 30) return ROUTE_MAT;
-  if (dt != CGAN3D_DT_F32) return ROUTE_PLANES;
-  const double fl = 2.0 * I * J * K, pack = 10.0 * K * (I + J);
-  return fl / 80e12 > fl / 160e12 + pack / 4e12 + 4e-6 ? ROUTE_PLANES : ROUTE_MAT;
+  return dt != CGAN3D_DT_F32 || ready || f32_planes(I, J, K, false) ? ROUTE_PLANES : ROUTE_MAT;
 }
 
 long long operand_bytes(int dt, const Operand& o) {
@@ -265,7 +270,7 @@ PlanePick pick_for(int dt, long long I, long long J, long long K) {
 // workspace of one product: both operands' planes, then partial sums
 long long product_bytes(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
   if (I == 0 || J == 0) return 0;
-  if (mat_route(dt, I, J, K) == ROUTE_MAT) return mat_ws_bytes(I, J, K);
+  if (mat_route(dt, I, J, K, a.planes) == ROUTE_MAT) return mat_ws_bytes(I, J, K);
   return operand_bytes(dt, a) + operand_bytes(dt, b) + pick_for(dt, I, J, K).part_floats * 4;
 }
 
@@ -315,7 +320,7 @@ void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStr
 // C = A B^T with m's epilogue; m.a / m.b: the operands as the tensors they are
 void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void* ws, hipStream_t st) {
   if (m.I == 0 || m.J == 0) return;
-  if (mat_route(dt, m.I, m.J, m.K) == ROUTE_MAT) {
+  if (mat_route(dt, m.I, m.J, m.K, a.planes) == ROUTE_MAT) {
     if (a.strided) mat_run<true, true>(dt, m, ws, st);
     else if (b.strided) mat_run<false, true>(dt, m, ws, st);
     else mat_run<false, false>(dt, m, ws, st);
@@ -328,9 +333,14 @@ void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void*
   }
 }
 
-// --- a few rows: the weight is read once, 16 bytes a lane, and nothing else matters ---
-// A wave takes R = 2 columns of y; KW waves of the block share the summed axis (1, or 4 where there are few
-// columns).  Measured: see DESIGN's table.
+// --- one or two rows: the weight is read once, 16 bytes a lane, and nothing else matters ---
+// Bound by memory.  A wave takes R = 2 columns of y, so that a load of x serves two of the weight; KW waves of the block
+// share the summed axis: 4, unless a wave would then get less than one load a column and the columns alone fill
+// the card.  Measured, us, KW = 1 / 4, two rows: bf16 4096 -> 4096 10.8 / 8.5, 2048 -> 16384 15.7 / 13.2, 1024 -> 8192
+// 6.1 / 6.9, 512 -> 16384 6.2 / 10.9; f32 1024 -> 8192 10.1 / 8.4.  One row, weights from memory: bf16 4096 -> 4096 8.0 us
+// (4.2 TB/s), f32 13.2 (5.1 TB/s).  From three rows on the products and conversions in the vector unit take as
+// long as the loads, and skinny_kernel is faster (four rows, bf16 4096 -> 4096: 12.0 here, 9.0 there).
+constexpr int kGemvRows = 2;
 template <typename T, int M, int KW>
 __global__ __launch_bounds__(256) void gemv_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
                                                    long long ldw, int n, int k, int vec, MatEpi e) {
@@ -393,22 +403,17 @@ template <typename T, int M> void gemv_run_m(const MatArgs& p, hipStream_t st) {
   const int V = MatT<T>::VEC, n = (int)p.J, k = (int)p.K;
   const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
                   (M == 1 || p.lda % V == 0) && (n == 1 || p.ldb % V == 0);
-  // two columns a wave: below 8 waves a CU the summed axis is shared by four waves
-  if (n / 2 >= 8 * cu_count())
+  if (k < 4 * 64 * V && n / 2 >= 8 * cu_count())
     launch(gemv_kernel<T, M, 1>, dim3((n + 7) / 8), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, vec, p.e);
   else
     launch(gemv_kernel<T, M, 4>, dim3((n + 1) / 2), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, vec, p.e);
 }
 template <typename T> void gemv_run(const MatArgs& p, hipStream_t st) {
   if (p.I == 1) gemv_run_m<T, 1>(p, st);
-  else if (p.I == 2) gemv_run_m<T, 2>(p, st);
-  else if (p.I == 3) gemv_run_m<T, 3>(p, st);
-  else gemv_run_m<T, 4>(p, st);
+  else gemv_run_m<T, 2>(p, st);
 }
 
-// --- few channels (k, n <= 64): every row's values are read and written once ---
-// Forward: a wave takes 16 rows at a time, x straight from memory into fragments, the whole weight in registers; no
-// LDS, no barrier.  Bound by memory.
+// n of eight neighbours (more: all), zeros for the others; vec: they are aligned where all are there
 template <typename T> __device__ __forceinline__ void load8(const T* p, int n, int vec, T (&v)[8]) {
   if (n >= 8 && vec) {
     typedef T vt __attribute__((ext_vector_type(MatT<T>::VEC)));
@@ -421,6 +426,76 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int n, i
   }
 }
 
+// --- up to 16 rows: a wave per 16 columns, weight and rows straight from memory into fragments ---
+// Bound by memory (and, with 16 rows of many columns, by the rows' own way through L2: each block reads all of them).
+// No LDS but for the join: a value of the weight is used once.  The KW waves of a block share the summed axis, U steps
+// of 32 values each in flight; 16 waves where each has U steps to do, else 4.  Measured, us, KW = 4 / 16, 8 rows: bf16
+// 4096 -> 4096 11.1 / 9.5 (3.5 TB/s), 2048 -> 4096 6.3 / 8.4; f32 4096 -> 4096 18.9 / 16.7, 2048 -> 4096 11.4 / 9.7,
+// 1024 -> 8192 10.1 / 15.7.  As products of tiles (planes, mat_kernel) these five take 12.9, 9.8, 28, 17.5 and 18.5.
+// 16-bit weights with more columns than 32 a CU are the planes' (16 rows, 4096 -> 16384: 40 here, 33 there; 2048 ->
+// 16384: 22 and 18), f32 ones are not (68 and 96).
+constexpr int kSkinnyRows = 16;
+template <typename T> constexpr int kSkinnySteps = sizeof(T) == 2 ? 8 : 4;
+template <typename T, int KW>
+__global__ __launch_bounds__(KW * 64) void skinny_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
+                                                         long long ldw, int rows, int n, int k, int vec, MatEpi e) {
+  constexpr int U = kSkinnySteps<T>;
+  __shared__ f32x4_m red[KW][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, g = lane >> 4;
+  const int j0 = blockIdx.x * 16;
+  // rows that are not there: the last one again
+  const T* wr = w + (long long)min(j0 + row, n - 1) * ldw + g * 8;
+  const T* xr = x + (long long)min(row, rows - 1) * ldx + g * 8;
+  f32x4_m acc = {};
+  const int full = vec ? k / 32 : 0;
+  for (int s0 = wave; s0 < full; s0 += KW * U) {
+    __align__(16) T fw[U][8], fx[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // behind the last step: that one again, as zeros
+      const int s = min(s0 + u * KW, full - 1) * 32;
+      load8(wr + s, 8, 1, fw[u]);
+      load8(xr + s, 8, 1, fx[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u > 0 && s0 + u * KW >= full)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) fw[u][q] = fx[u][q] = from_f<T>(0.f);
+      acc = mfma_8(fw[u], fx[u], acc);
+    }
+  }
+  for (int s = full + wave; s * 32 < k; s += KW) {
+    __align__(16) T fw[8], fx[8];
+    load8(wr + s * 32, k - s * 32 - g * 8, vec, fw);
+    load8(xr + s * 32, k - s * 32 - g * 8, vec, fx);
+    acc = mfma_8(fw, fx, acc);
+  }
+  red[wave][lane] = acc;
+  __syncthreads();
+  const int i = threadIdx.x / 16, j = threadIdx.x % 16;
+  if (threadIdx.x < 256 && i < rows && j0 + j < n) {
+    float v = 0.f;
+#pragma unroll
+    for (int z = 0; z < KW; ++z) v += red[z][j / 4 * 16 + i][j % 4];
+    mat_store<T>(e, n, i, j0 + j, v);
+  }
+}
+template <typename T> void skinny_run(const MatArgs& p, hipStream_t st) {
+  const T* x = static_cast<const T*>(p.a);
+  const T* w = static_cast<const T*>(p.b);
+  const int V = MatT<T>::VEC, n = (int)p.J, k = (int)p.K;
+  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 && p.lda % V == 0 &&
+                  (n == 1 || p.ldb % V == 0);
+  const dim3 grid((n + 15) / 16);
+  if (k >= 16 * 32 * kSkinnySteps<T>) launch(skinny_kernel<T, 16>, grid, dim3(1024), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, vec, p.e);
+  else launch(skinny_kernel<T, 4>, grid, dim3(256), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, vec, p.e);
+}
+
+// --- few channels (k, n <= 64): every row's values are read and written once ---
+// Forward: a wave takes 16 rows at a time, x straight from memory into fragments, the whole weight in registers; no
+// LDS, no barrier.  Bound by memory where there are many rows (1048576 x 64 -> 64: f32 150 us, 3.6 TB/s, bf16 57 us,
+// 4.7 TB/s; the products' own kernels 198 and 77), by the launch and one trip for the weight and one for the rows where
+// there are few (4096 x 64 -> 64: f32 6.7 us against 7.3, bf16 4.8 against 4.0, 16 -> 16 3.6 against 3.9).
 template <typename T, int NT, int KS>
 __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
                                                        long long ldw, long long rows, int n, int k, int vecx, int vecw,
@@ -498,7 +573,9 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
 }
 
 // Backward: one pass over dy, z and x writes dx and keeps dW and db in registers; a block takes tiles of 64 rows in
-// turn and leaves one partial sum of each.  dz is used as its own type would hold it, for db before that.
+// turn and leaves one partial sum of each.  dz is used as its own type would hold it, for db before that.  dz and x go
+// through LDS in both orders, since one product sums over columns and the other over rows: that, not memory, bounds
+// the 16-bit form (1048576 x 64 -> 64 with SiLU: f32 347 us, 3.1 TB/s, bf16 273 us, 2.0 TB/s).
 constexpr int kRowsBlocks = 512;
 template <typename T, int NT, int KT>
 __global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy, long long lddy,
@@ -665,8 +742,12 @@ __global__ __launch_bounds__(1024) void rows_join_kernel(const float* __restrict
   }
 }
 
+bool skinny_takes(const cgan3d_linear_args* a) {
+  return a->rows <= kSkinnyRows && (a->dtype == CGAN3D_DT_F32 || a->n <= 32 * cu_count());
+}
 bool few_channels(long long n, long long k) { return n > 0 && k > 0 && n <= 64 && k <= 64; }
-// one pass pays where the rows fill the card; below, the products' launches are as good
+// One pass against dz, two products and their joins, us, f32 and bf16 of 64 -> 64: 16 rows 16.5 / 16.2 and 14.0 / 12.3, 64
+// rows 17.8 / 19.2 and 14.8 / 12.8, 256 rows 17.8 / 27.7 and 14.9 / 14.2, 16384 rows 22.5 / 65 and 19.1 / 61.
 bool rows_bwd_takes(const cgan3d_linear_args* a) { return few_channels(a->n, a->k) && a->rows >= 64 && (a->dx || a->dw); }
 int rows_blocks(const cgan3d_linear_args* a) { return (int)std::min<long long>((a->rows + 63) / 64, kRowsBlocks); }
 
@@ -715,7 +796,7 @@ template <typename T> void rows_bwd_run(const cgan3d_linear_args* a, void* ws, h
 // --- dz = dy * act'(z), and its column sums ---
 // CT threads of a block along the columns (V values each), the rest along the rows; column sums in 32 bits, of dz
 // before its rounding, into part [blockIdx.y][n].  dz goes to rows of ldz values whose padding is zeroed:
-// as it is, or (PL3) split into three planes.
+// as it is, or (PL3) split into three planes.  Bound by memory: 8192 x 8192 bf16 with GELU 90 us, 4.5 TB/s.
 template <typename T, bool PL3>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, long long lddy,
                                                        const typename PreT<T>::type* __restrict__ pre, void* __restrict__ dzv,
@@ -851,10 +932,10 @@ Bwd bwd_layout(const cgan3d_linear_args* a) {
     w.total = a->dw || a->dbias ? (long long)rows_blocks(a) * (a->n * a->k + a->n) * 4 : 0;
     return w;
   }
-  // both products take dz in one form: planes if either is better off with them
-  const bool rx = a->dx && mat_route(dt, a->rows, a->k, a->n) == ROUTE_PLANES && a->rows && a->k;
-  const bool rw = a->dw && mat_route(dt, a->n, a->k, a->rows) == ROUTE_PLANES && a->n && a->k;
-  w.planes3 = dt == CGAN3D_DT_F32 && rx && rw;
+  // dz goes to planes where both products are better off with them: they share the splitting
+  const long long big = 1LL << 30;
+  w.planes3 = dt == CGAN3D_DT_F32 && a->dx && a->dw && a->rows > 0 && a->rows < big && a->n > 0 && a->n < big && a->k > 0 &&
+              a->k < big && f32_planes(a->rows, a->k, a->n, true) && f32_planes(a->n, a->k, a->rows, true);
   const bool direct = a->act == CGAN3D_ACT_NONE && !w.planes3 && (dt == CGAN3D_DT_F32 || chunked(a->dy, a->lddy, a->n));
   w.has_dz = !direct && (a->dx || a->dw);
   w.ldz = (int)up8(a->n);
@@ -881,7 +962,7 @@ void fwd_operands(const cgan3d_linear_args* a, Operand* x, Operand* w) {
   *w = {a->w, a->ldw, a->n, a->k, false, false};
 }
 long long fwd_bytes(const cgan3d_linear_args* a) {
-  if (a->rows <= kGemvRows || few_channels(a->n, a->k)) return 0;
+  if (a->rows <= kGemvRows || skinny_takes(a) || few_channels(a->n, a->k)) return 0;
   Operand x, w;
   fwd_operands(a, &x, &w);
   return product_bytes(a->dtype, x, w, a->rows, a->n, a->k);
@@ -965,6 +1046,10 @@ extern "C" int cgan3d_linear_fwd(const cgan3d_linear_args* a, void* ws, int64_t 
     if (a->dtype == CGAN3D_DT_F32) gemv_run<float>(p, st);
     else if (a->dtype == CGAN3D_DT_BF16) gemv_run<bf16_t>(p, st);
     else gemv_run<f16_t>(p, st);
+  } else if (skinny_takes(a)) {
+    if (a->dtype == CGAN3D_DT_F32) skinny_run<float>(p, st);
+    else if (a->dtype == CGAN3D_DT_BF16) skinny_run<bf16_t>(p, st);
+    else skinny_run<f16_t>(p, st);
   } else if (few_channels(a->n, a->k)) {
     if (a->dtype == CGAN3D_DT_F32) rows_fwd_run<float>(p, st);
     else if (a->dtype == CGAN3D_DT_BF16) rows_fwd_run<bf16_t>(p, st);

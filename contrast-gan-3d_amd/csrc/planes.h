@@ -6,6 +6,10 @@
 //   P = 3  three bf16 planes, hi + mid + lo = all 24 bits of an f32: the six products of the first two
 //          orders (f32 operands of any size; what is left out is below 2^-24 of a product)
 //
+// Bound by the matrix instructions and, there, by the card's power: a Gram product has them busy 68 % of the time at
+// 1.63 GHz, a step 42 % at 1.93.  Reached, whole products with their epilogues: P = 1 275 GFLOP (8192 x 8192 -> 2048) in 250
+// us, 1100 TFLOP/s; P = 2 the step of two 2048 x 8192 in 381 us, 361 TFLOP/s of f32 accuracy (1082 of 16-bit products);
+// P = 3 4096 x 4096 -> 4096 in 677 us with the splitting, 203 TFLOP/s (1218).
 // f32 matrix instructions run at 154 TFLOP/s on a large product, 16-bit ones at 1365: a third of that is 455, a
 // sixth 227, so f32 accuracy from planes is 3.0 and 1.5 times what the f32 instructions can reach.
 //
@@ -379,10 +383,10 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
   }
 }
 
-// Partial sums added in the order of their splits, then the epilogue: blocks of 32 rows of a tile.
+// Partial sums added in the order of their splits, then the epilogue: blocks of 16 rows of a tile.
 template <int BM, int BN, bool SYM, class E, int N>
 __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
-  constexpr int SUB = BM / 32;
+  constexpr int SUB = BM / 16;
   int b = blockIdx.x;
   const int jn = plane_job(jobs, b);
   const PlaneJob<E>& p = jobs.j[jn];
@@ -391,12 +395,13 @@ __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
   const int t = b / SUB, sub = b - t * SUB;
   int ti, tj;
   plane_tile<BM, SYM>(t, p.I, p.tj, ti, tj);
-  for (int q = threadIdx.x; q < 32 * BN / 4; q += 256) {
+  for (int q = threadIdx.x; q < 16 * BN / 4; q += 256) {
     // 16 lanes on 16 rows, as the products leave them: a mirrored value's neighbours are written together
-    const int li = sub * 32 + q / (BN * 4) * 16 + q % 16, lj = q / 16 % (BN / 4) * 4, i = ti * BM + li, j = tj * BN + lj;
+    const int li = sub * 16 + q % 16, lj = q / 16 * 4, i = ti * BM + li, j = tj * BN + lj;
     if (i >= p.I || j >= p.J) continue;
     const float* s = p.part + (long long)t * (BM * BN) + li * BN + lj;
     f32x4_m v = *reinterpret_cast<const f32x4_m*>(s);
+#pragma unroll 8
     for (int z = 1; z < p.splits; ++z) v += *reinterpret_cast<const f32x4_m*>(s + (long long)z * p.tiles * (BM * BN));
     p.e.put(i, j, v, p.J - j, SYM && ti != tj);
   }
@@ -410,8 +415,12 @@ struct PlanePick {
   int cfg = 0, kchunk = 0;
   long long part_floats = 0;
 };
-// tile configurations by planes: 0 the largest (8 waves, one block a CU), 1 and 2 smaller ones that give more
-// blocks where there are few
+// Tile configurations by planes: 0 the largest (8 waves, one block a CU), 1 and 2 smaller ones that give more
+// blocks where there are few.  RATE: a CU's share of the largest tile's.  Measured, us, tiles 0 / 1 / 2 without splits and
+// what plane_pick took: bf16 8192 x 4096 -> 4096 217 / 310 / 436, took 0; 2048 x 2048 -> 2048 50 / 27 / 36, took 1;
+// 512 x 4096 -> 4096 87 / 43 / 34, took 2; f32 the same three 1398 / 1681 / 2465, 154 / 116 / 172 (took 113 with a
+// split), 277 / 180 / 162 (140).  Five steps of 4096 x 4096 4412 / 4600 / 6320, took 0 (4305); of 1024 x 4096 1974 / 691 /
+// 461, took 406 with splits.
 template <int P, bool SYM = false> struct PlaneCfg;
 template <> struct PlaneCfg<1, false> {
   static constexpr int BM[3] = {256, 128, 64}, BN[3] = {256, 128, 64}, BK[3] = {32, 32, 64}, WI[3] = {2, 2, 2}, WJ[3] = {4, 2, 2}, S[3] = {5, 5, 4};
@@ -442,7 +451,8 @@ inline long long plane_tiles(const PlaneShape& s, int bm, int bn, bool sym) {
 // The tile size and the length of a split that the launch of these products is expected to be fastest
 // with: the blocks that the fullest CU gets, at the rate a CU reaches with that tile (PlaneCfg::RATE), 64
 // t-values' worth of start and end per block, and the joining of partial sums (written and read once, a
-// launch of its own).
+// launch of its own).  Measured, us, bf16 128 x 8192 -> 128, tile 2 in 1 / 4 / 16 / 64 splits: 44 / 17 / 12 / 17;
+// 128 x 65536 -> 128: 321 / 87 / 30 / 21; 1024 x 16384 -> 1024, tile 1 in 1 / 4 / 16: 140 / 51 / 63, took 53.
 template <int P, bool sym> PlanePick plane_pick(const PlaneShape* s, int n) {
   using C = PlaneCfg<P, sym>;
   const double cus = cu_count(), rate = 1.1e15 / (P * (P + 1) / 2) / 2 / cus;  // products of a CU per second
@@ -465,7 +475,7 @@ template <int P, bool sym> PlanePick plane_pick(const PlaneShape* s, int n) {
       }
       const double rounds = blocks <= cus ? 1. : std::max(std::ceil(blocks / cus), 1.);
       double t = rounds * C::BM[c] * C::BN[c] * (double)(kc + 64) / (rate * C::RATE[c]);
-      if (part) t += part * 8. / 3.5e12 + 4e-6;
+      if (part) t += part * 8. / 3.5e12 + 4e-6 + sp * 5e-8;
       if (t < tb) {
         tb = t;
         best.cfg = c;
@@ -499,7 +509,7 @@ void plane_run(PlaneJobs<E, N>& jobs, const PlanePick& pick, float* part, hipStr
       jobs.start[i] = at;
       js.start[i] = jat;
       at += j.tiles * j.splits;
-      jat += j.tiles * (BM / 32);
+      jat += j.tiles * (BM / 16);
     }
     if (at == 0) return;
     launch(plane_kernel<T, P, AT, BT, BM, BN, C::BK[c], C::S[c], C::WI[c], C::WJ[c], C::AHEAD[c], SYM, E, N>, dim3(at),

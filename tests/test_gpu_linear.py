@@ -29,7 +29,8 @@ SHAPES = [  # rows, k, n
     (64, 32, 64), (65, 31, 63), (100, 1, 7), (128, 300, 128), (129, 129, 257), (256, 1024, 256), (333, 515, 77),
     (1000, 16, 32), (4096, 64, 48), (5000, 3, 5), (2049, 40, 8), (512, 640, 384), (300, 2048, 520),
     # a few rows with many columns; f32 products that are split into planes (both gradients, one of them)
-    (1, 4096, 4096), (2, 100, 5000), (4, 65, 4099), (1500, 1000, 1203), (2048, 512, 1024), (8000, 1000, 100),
+    (1, 4096, 4096), (2, 100, 5000), (4, 65, 4099), (3, 4096, 520), (9, 5000, 70), (16, 2048, 1000),
+    (5, 31, 8200), (2, 1024, 8192), (12, 72, 9000), (1500, 1000, 1203), (2048, 512, 1024), (8000, 1000, 100),
 ]
 
 
