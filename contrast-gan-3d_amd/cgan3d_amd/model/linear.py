@@ -58,45 +58,48 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _LinearFn.apply(x, weight, bias, residual, act, slope)
-    return _forward(x, weight, bias, residual, act, slope, None)
+    k = weight.shape[1]
+    return _forward(x, _rows(x, k), _rows(weight, k), bias, residual, act, slope, None)[0]
 
 
-def _forward(x, weight, bias, residual, act, slope, preact):
-    n, k = weight.shape
-    x2 = _rows(x, k)
+def _forward(x, x2, w2, bias, residual, act, slope, preact):
+    n = w2.shape[0]
     y = x.new_empty((*x.shape[:-1], n))
-    ops.linear(x2, _rows(weight, k), y if y.dim() == 2 else y.view(x2.shape[0], n),
-               bias if bias is None or bias.is_contiguous() else bias.contiguous(),
-               residual if residual is None else _rows(residual, n), act, slope, preact)
-    return y
+    args = ops._linear_forward(x2, w2, y if y.dim() == 2 else y.view(x2.shape[0], n),
+                               bias if bias is None or bias.is_contiguous() else bias.contiguous(),
+                               residual if residual is None else _rows(residual, n), act, slope, preact)
+    return y, args
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, slope):
-        preact = None
-        if act != L.ACT_NONE and any(ctx.needs_input_grad[:3]):
-            preact = torch.empty((math.prod(x.shape[:-1]), weight.shape[0]), dtype=ops.linear_preact_dtype(x.dtype),
-                                 device=x.device)
-        y = _forward(x, weight, bias, residual, act, slope, preact)
-        ctx.act, ctx.slope = act, slope
-        ctx.save_for_backward(x, weight, preact)
+        n, k = weight.shape
+        x2, w2, preact = _rows(x, k), _rows(weight, k), None
+        if act != L.ACT_NONE and True in ctx.needs_input_grad[:3]:
+            preact = torch.empty((x2.shape[0], n), dtype=ops.linear_preact_dtype(x.dtype), device=x.device)
+        y, ctx.args = _forward(x, x2, w2, bias, residual, act, slope, preact)
+        ctx.shape, ctx.act, ctx.slope = x.shape, act, slope
+        ctx.save_for_backward(x2, w2, preact)
         return y
 
     @staticmethod
     def backward(ctx, grad_out):
         if torch.is_grad_enabled():
             raise NotImplementedError("double backward through the HIP linear block is not implemented")
-        x, weight, preact = ctx.saved_tensors
-        n, k = weight.shape
+        x2, w2, preact = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx = x.new_empty(x.shape) if nx else None
-        dw = x.new_empty((n, k)) if nw else None
-        db = x.new_empty(n) if nb else None
+        dx = x2.new_empty(ctx.shape) if nx else None
+        dw = x2.new_empty(w2.shape) if nw else None
+        db = x2.new_empty(w2.shape[0]) if nb else None
         if nx or nw or nb:
-            x2 = _rows(x, k)
-            ops.linear_backward(_rows(grad_out, n), x2, _rows(weight, k),
-                                dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db, ctx.act, ctx.slope, preact)
+            a, dy = ctx.args, _rows(grad_out, w2.shape[0])
+            here = (x2.data_ptr() or None, w2.data_ptr() or None, None if preact is None else preact.data_ptr() or None)
+            if here == (a.x, a.w, a.preact):
+                ops._linear_backward_of(a, dy, x2, dx, dw, db)
+            else:  # hooks on saved tensors gave others back
+                ops.linear_backward(dy, x2, w2, dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db,
+                                    ctx.act, ctx.slope, preact)
         return dx, dw, db, grad_out if nr else None, None, None
 
 

@@ -1519,15 +1519,30 @@ def _linear_sizes(x, w, act, who):
     return rows, k, n, dt, _matrix(x, rows, k, who, "x", x.dtype, dev), _matrix(w, n, k, who, "w", x.dtype, dev)
 
 
+def _linear_call(entry, a, device, ws, who):
+    """The launches of a ``LinearArgs`` on ``device`` (not the current one: in its context), with a workspace."""
+    st = None if DRY_RUN else torch.cuda.current_stream()
+    if st is not None and st.device_index != device.index:
+        with torch.cuda.device(device):
+            return _linear_call(entry, a, device, ws, who)
+    lib, ref = L.load(), ctypes.byref(a)
+    ws = _workspace(ws, getattr(lib, entry + "_ws_bytes")(ref), who, device)
+    if st is not None:
+        check(getattr(lib, entry)(ref, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                                  st.cuda_stream), who)
+
+
 def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
     """``y = act(x w^T + bias) + residual`` (cgan3d_linear_fwd): x [rows, k], w [n, k], bias [n], residual
     and y [rows, n], all of one dtype (f32, bf16 or f16), rows strided as they like.  ``preact`` [rows, n]
     (``linear_preact_dtype``) receives x w^T + bias for ``linear_backward``.  y may be the residual."""
+    _linear_forward(x, w, y, bias, residual, act, slope, preact, ws)
+
+
+def _linear_forward(x, w, y, bias, residual, act, slope, preact, ws=None):
+    """``linear``; returns its arguments, which ``_linear_backward_of`` starts from."""
     rows, k, n, dt, ldx, ldw = _linear_sizes(x, w, act, "linear")
     t, dev = x.dtype, x.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return linear(x, w, y, bias, residual, act, slope, preact, ws)
     a = L.LinearArgs(
         rows, k, n, dt, act, slope, x.data_ptr(), ldx, w.data_ptr(), ldw,
         None if bias is None else _flat(bias, n, "linear", "bias", t, dev),
@@ -1535,13 +1550,8 @@ def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=
         0 if residual is None else _matrix(residual, rows, n, "linear", "residual", t, dev),
         y.data_ptr(), _matrix(y, rows, n, "linear", "y", t, dev),
         None if preact is None else _flat(preact, rows * n, "linear", "preact", linear_preact_dtype(t), dev))
-    ref = ctypes.byref(a)
-    ws = _workspace(ws, L.load().cgan3d_linear_fwd_ws_bytes(ref), "linear", dev)
-    if ws is None:
-        rc = _launch("cgan3d_linear_fwd", ref, None, 0)
-    else:
-        rc = _launch("cgan3d_linear_fwd", ref, ws.data_ptr(), ws.numel())
-    check(rc, "linear")
+    _linear_call("cgan3d_linear_fwd", a, dev, ws, "linear")
+    return a
 
 
 def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
@@ -1550,9 +1560,6 @@ def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slop
     activation).  The residual's gradient is dy itself."""
     rows, k, n, dt, ldx, ldw = _linear_sizes(x, w, act, "linear_backward")
     t, dev = x.dtype, x.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return linear_backward(dy, x, w, dx, dw, dbias, act, slope, preact, ws)
     if act != L.ACT_NONE and preact is None:
         raise ValueError("linear_backward: the activation's gradient needs the forward call's preact")
     if dw is not None:
@@ -1565,13 +1572,24 @@ def linear_backward(dy, x, w, dx=None, dw=None, dbias=None, act=L.ACT_NONE, slop
         0 if dx is None else _matrix(dx, rows, k, "linear_backward", "dx", t, dev),
         None if dw is None else _flat(dw, n * k, "linear_backward", "dw", t, dev),
         None if dbias is None else _flat(dbias, n, "linear_backward", "dbias", t, dev))
-    ref = ctypes.byref(a)
-    ws = _workspace(ws, L.load().cgan3d_linear_bwd_ws_bytes(ref), "linear_backward", dev)
-    if ws is None:
-        rc = _launch("cgan3d_linear_bwd", ref, None, 0)
-    else:
-        rc = _launch("cgan3d_linear_bwd", ref, ws.data_ptr(), ws.numel())
-    check(rc, "linear_backward")
+    _linear_call("cgan3d_linear_bwd", a, dev, ws, "linear_backward")
+
+
+def _linear_backward_of(fwd, dy, x, dx, dw, dbias):
+    """``linear_backward`` after a ``_linear_forward`` whose operands are still where they were: the caller vouches
+    for them and for dx, dw and dbias (contiguous, or None), so that only dy is looked at."""
+    dev = x.device
+    a = L.LinearArgs.from_buffer_copy(fwd)  # two backward passes of one graph may run at once
+    a.bias = a.residual = a.y = None
+    a.ldr = a.ldy = 0
+    a.dy, a.lddy = dy.data_ptr(), _matrix(dy, a.rows, a.n, "linear_backward", "dy", x.dtype, dev)
+    if dx is not None:
+        a.dx, a.lddx = dx.data_ptr(), a.k
+    if dw is not None:
+        a.dw = dw.data_ptr()
+    if dbias is not None:
+        a.dbias = dbias.data_ptr()
+    _linear_call("cgan3d_linear_bwd", a, dev, None, "linear_backward")
 
 
 def _ns_args(steps, coefficients, eps, what):

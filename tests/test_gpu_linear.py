@@ -441,3 +441,21 @@ def test_f32_products_close_to_overflow():
     want = x.double() @ w.double().T
     assert want.abs().max() < top
     check(y, want, (k + 4) * U * want.abs(), "largest values")
+
+
+@pytest.mark.parametrize("rows,k,n", [(70, 24, 40), (300, 136, 200)])
+def test_saved_tensor_hooks_and_repeated_backward(rows, k, n):
+    """Operands that come back from the host at other addresses, a kept graph run twice, and a transposed weight."""
+    from cgan3d_amd.model.linear import fused_linear
+    x, w, b, r, dy = on_gpu(*make(rows, k, n, "f32", "silu", 95))
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+    wants = torch.autograd.grad(fused_linear(*leaves, act=code("silu")), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = fused_linear(*leaves, act=code("silu"))
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(y, leaves, dy), wants))
+    y = fused_linear(*leaves, act=code("silu"))
+    for keep in (True, True, False):
+        assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(y, leaves, dy, retain_graph=keep), wants))
+    wt = w.detach().t().contiguous().requires_grad_(True)
+    got = torch.autograd.grad(fused_linear(x, wt.t(), b, r, act=code("silu")), (x, wt), dy)
+    assert torch.equal(got[0], wants[0]) and torch.equal(got[1], wants[1].t())
