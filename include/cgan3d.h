@@ -585,7 +585,7 @@ int cgan3d_adam(float* param, const float* grad, float* exp_avg, float* exp_avg_
  * A pointwise convolution over channels-last voxels, or any layer of rows times a weight in torch's
  * [out, in] layout.  Every tensor is of `dtype`; products are summed in f32 and rounded once, in the
  * epilogue.  Rows may be strided (ld*, elements; at least the row's length); preact, dz, dw and dbias are
- * contiguous.  Any size, zero included, and any alignment of whole elements.
+ * contiguous.  Any size up to 2^30 columns (k, n) and 2^40 rows, zero included, and any alignment of whole elements.
  *   forward : x, w, y; optional bias [n], residual (may be y itself), preact.
  *             preact [rows, n], f32, or f16 (saturating) for bf16 tensors: z = x w^T + bias, which the backward
  *             pass of an activation reads.
@@ -628,7 +628,7 @@ int cgan3d_linear_bwd(const cgan3d_linear_args* args, void* ws, int64_t ws_bytes
  * Newton-Schulz iteration on each of n matrices (host list): X = g / (|g|_F + eps), then `steps` times
  * X = a X + (b A + c A A) X with A = X X^T (a tall g by its transpose); out = X, of g's dtype.
  * coefficients (host): a, b, c.  out may be g itself.  The norm is summed in f64, the iteration keeps f32
- * accuracy whatever the dtype. */
+ * accuracy whatever the dtype.  Sides of up to 2^30, zero included. */
 typedef struct cgan3d_ortho_mat {
   const void* g;
   void* out;

@@ -155,6 +155,34 @@ def test_orthogonalize_settings(shape):
     check_ns(ops.orthogonalize(view[:, :shape[0]].T), g, "f32", "transposed view")
 
 
+@pytest.mark.parametrize("shape", [(24, 40), (130, 80), (3, 90)])
+def test_orthogonalize_coefficients_out_of_range(shape):
+    """Coefficients whose iterates leave the range that the planes hold run on f32 products.  Bound, in Frobenius norms:
+    a product of K terms is off by K u |A| |B|, a sum by u of its terms, and a step passes an error on by
+    |a| + 3 |b| n^2 + 5 |c| n^4 at most, n = |X|."""
+    from cgan3d_amd import ops
+    g = grad_like(*shape, seed=6)
+    s, l = min(shape), max(shape)
+    for co in ((2.0, -65.0, 60.0), (70.0, 0.0, -61.0)):
+        a, b, c = (abs(v) for v in co)
+        for steps in (1, 2):
+            x = (g.double() if shape[0] <= shape[1] else g.double().T)
+            x = x / (x.square().sum().sqrt() + 1e-7)
+            tol = 4 * U * float(x.norm())
+            for _ in range(steps):
+                n = float(x.norm())
+                dm = (l + 2) * U * n ** 2
+                db = b * dm + c * (2 * n ** 2 * dm + (s + 2) * U * n ** 4) + 2 * U * (b * n ** 2 + c * n ** 4)
+                step = db * n + (s + 2) * U * (b * n ** 2 + c * n ** 4) * n + 3 * U * (a * n + b * n ** 3 + c * n ** 5)
+                tol = (a + 3 * b * n ** 2 + 5 * c * n ** 4) * tol + 1.01 * step
+                m = x @ x.T
+                x = co[0] * x + (co[1] * m + co[2] * m @ m) @ x
+            want = x if shape[0] <= shape[1] else x.T
+            err = float((ops.orthogonalize(g.cuda(), steps=steps, coefficients=co).double().cpu() - want).norm())
+            assert err <= tol, f"{co}, {steps} steps: off by {err:.3e}, bound {tol:.3e}, norm {float(want.norm()):.3e}"
+            assert tol < 0.02 * float(want.norm()), "the bound says something"
+
+
 @pytest.mark.parametrize("shape", [(20, 30), (80, 130)])
 def test_orthogonalize_nonfinite(shape):
     """A NaN or an infinity makes its own matrix NaN, and no other."""

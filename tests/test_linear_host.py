@@ -223,3 +223,17 @@ def test_engine_step_with_muon_dry_run(dry, clip):
                      weight_clip=0.01 if clip else None)
     eng.step()
     assert eng.g_split == 0 and go._host_step == 1 and do._host_step == 1
+
+
+def test_sizes_beyond_the_limits_are_refused():
+    from cgan3d_amd import _lib as L
+    lib, big = L.load(), (1 << 30) + 8
+    for kw in (dict(k=big, n=4, ldx=big, ldw=big), dict(k=4, n=big, ldx=4, ldw=4, ldy=big, lddy=big),
+               dict(k=4, n=4, rows=(1 << 40) + 1, ldx=4, ldw=4, ldy=4, lddy=4)):
+        a = L.LinearArgs(**(dict(rows=2, ldy=4, lddy=4, x=64, w=64, y=64, dy=64, dx=64, lddx=big) | kw))
+        assert lib.cgan3d_linear_fwd_ws_bytes(C.byref(a)) == -1 and lib.cgan3d_linear_bwd_ws_bytes(C.byref(a)) == -1
+        assert b"too large" in lib.cgan3d_get_last_error()
+    m = (L.OrthoMat * 1)(L.OrthoMat(64, 64, big, big, 2, big))
+    assert lib.cgan3d_orthogonalize_ws_bytes(m, 1, L.DT_F32) == -1
+    s = (L.MuonSeg * 1)(L.MuonSeg(0, 2, big, 1.0))
+    assert lib.cgan3d_muon_ws_bytes(s, 1) == -1
