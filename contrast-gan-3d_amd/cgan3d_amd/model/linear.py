@@ -36,6 +36,8 @@ def _rows(t: Tensor, cols: int) -> Tensor:
     """``t`` [..., cols] as a matrix with contiguous rows (a view wherever its strides allow one)."""
     if t.dim() != 2:
         t = t.reshape(math.prod(t.shape[:-1]), cols)
+    elif t.is_contiguous():
+        return t
     if not t.is_contiguous():
         s = t.stride()
         if (cols > 1 and s[1] != 1) or (t.shape[0] > 1 and s[0] < cols):
@@ -50,21 +52,26 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     (``_lib.ACT_NONE``, ``ACT_RELU``, ``ACT_LRELU`` with ``slope``, ``ACT_TANH``, ``ACT_GELU``, ``ACT_SILU``).
     Differentiable once.  A HIP graph that captures the backward pass must be the only autograd graph alive
     on its leaves (torch's own rule: their gradient accumulators belong to the stream they were made on)."""
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"fused_linear: x {tuple(x.shape)} does not multiply weight {tuple(weight.shape)}")
-    if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
+    xs, ws = x.shape, weight.shape
+    if len(ws) != 2 or not xs or xs[-1] != ws[1]:
+        raise ValueError(f"fused_linear: x {tuple(xs)} does not multiply weight {tuple(ws)}")
+    if residual is not None and (len(residual.shape) != len(xs) or residual.shape[-1] != ws[0]
+                                 or residual.shape[:-1] != xs[:-1]):
         raise ValueError(f"fused_linear: residual {tuple(residual.shape)} is not of the result's shape "
-                         f"{(*x.shape[:-1], weight.shape[0])}")
+                         f"{(*xs[:-1], ws[0])}")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _LinearFn.apply(x, weight, bias, residual, act, slope)
-    k = weight.shape[1]
+    k = ws[1]
     return _forward(x, _rows(x, k), _rows(weight, k), bias, residual, act, slope, None)[0]
 
 
 def _forward(x, x2, w2, bias, residual, act, slope, preact):
     n = w2.shape[0]
-    y = x.new_empty((*x.shape[:-1], n))
+    if residual is not None and residual.is_contiguous() and residual.dtype is x.dtype:
+        y = torch.empty_like(residual)  # the same shape, and cheaper to ask for
+    else:
+        y = x.new_empty((*x.shape[:-1], n))
     args = ops._linear_forward(x2, w2, y if y.dim() == 2 else y.view(x2.shape[0], n),
                                bias if bias is None or bias.is_contiguous() else bias.contiguous(),
                                residual if residual is None else _rows(residual, n), act, slope, preact)

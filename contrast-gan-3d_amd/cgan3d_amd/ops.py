@@ -1447,8 +1447,11 @@ def _matrix(t, rows, cols, who, name, dtype, device):
     """Row stride of a [rows, cols] operand whose rows are contiguous (a padded or sliced row stride is
     fine); anything else is refused.  (These run on every call of a small layer: plain comparisons, and
     texts only where something is wrong.)"""
-    shape, stride = t.shape, t.stride()
-    if t.dtype is dtype and len(shape) == 2 and shape[0] == rows and shape[1] == cols and t.device == device:
+    shape = t.shape
+    if t.dtype is dtype and shape == (rows, cols) and t.device == device:
+        if t.is_contiguous():
+            return cols or 1
+        stride = t.stride()
         ld = stride[0] if rows > 1 else cols or 1
         if (cols <= 1 or stride[1] == 1) and ld >= cols:
             return ld
@@ -1462,21 +1465,22 @@ def _matrix(t, rows, cols, who, name, dtype, device):
 
 def _flat(t, n, who, name, dtype, device):
     """Address of a contiguous operand of n values."""
+    if t.dtype is dtype and t.device == device and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{who} {name}: dtype {t.dtype} != {dtype}")
     if t.device != device:
         raise ValueError(f"{who} {name}: on {t.device}, the other operands are on {device}")
-    if t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{who} {name}: {n} contiguous values needed, got shape {tuple(t.shape)}, strides {t.stride()}")
-    return t.data_ptr()
+    raise ValueError(f"{who} {name}: {n} contiguous values needed, got shape {tuple(t.shape)}, strides {t.stride()}")
 
 
 def _dt(t, what):
-    if t.dtype not in L.DTYPES:
+    dt = L.DTYPES.get(t.dtype)
+    if dt is None:
         raise TypeError(f"{what}: dtype {t.dtype} (float32, bfloat16 or float16)")
     if not t.is_cuda and not DRY_RUN:
         raise ValueError(f"{what}: operands must be on the GPU, got {t.device}")
-    return L.DTYPES[t.dtype]
+    return dt
 
 
 def _workspace(ws, need, what, device):
@@ -1512,11 +1516,12 @@ def _linear_sizes(x, w, act, who):
     """(rows, k, n, dtype code, row strides of x and w)."""
     if act not in LINEAR_ACTS:
         raise ValueError(f"{who}: activation code {act} (none, relu, lrelu, tanh, gelu or silu)")
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError(f"{who}: x and w must be matrices, got {tuple(x.shape)} and {tuple(w.shape)}")
-    dt, dev = _dt(x, who), x.device
-    (rows, k), n = x.shape, w.shape[0]
-    return rows, k, n, dt, _matrix(x, rows, k, who, "x", x.dtype, dev), _matrix(w, n, k, who, "w", x.dtype, dev)
+    xs, ws = x.shape, w.shape
+    if len(xs) != 2 or len(ws) != 2:
+        raise ValueError(f"{who}: x and w must be matrices, got {tuple(xs)} and {tuple(ws)}")
+    dt, t, dev = _dt(x, who), x.dtype, x.device
+    (rows, k), n = xs, ws[0]
+    return rows, k, n, dt, k or 1 if x.is_contiguous() else _matrix(x, rows, k, who, "x", t, dev), _matrix(w, n, k, who, "w", t, dev)
 
 
 def _linear_call(entry, a, device, ws, who):
@@ -1526,10 +1531,14 @@ def _linear_call(entry, a, device, ws, who):
         with torch.cuda.device(device):
             return _linear_call(entry, a, device, ws, who)
     lib, ref = L.load(), ctypes.byref(a)
-    ws = _workspace(ws, getattr(lib, entry + "_ws_bytes")(ref), who, device)
+    need = getattr(lib, entry + "_ws_bytes")(ref)
+    if need or ws is not None:
+        ws = _workspace(ws, need, who, device)
     if st is not None:
-        check(getattr(lib, entry)(ref, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-                                  st.cuda_stream), who)
+        rc = getattr(lib, entry)(ref, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                                 st.cuda_stream)
+        if rc:
+            check(rc, who)
 
 
 def linear(x, w, y, bias=None, residual=None, act=L.ACT_NONE, slope=0.0, preact=None, ws=None):
