@@ -96,8 +96,11 @@ class _LinearFn(torch.autograd.Function):
             raise NotImplementedError("double backward through the HIP linear block is not implemented")
         x2, w2, preact = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx = x2.new_empty(ctx.shape) if nx else None
-        dw = x2.new_empty(w2.shape) if nw else None
+        dx = dw = None
+        if nx:
+            dx = torch.empty_like(x2) if x2.shape == ctx.shape and x2.is_contiguous() else x2.new_empty(ctx.shape)
+        if nw:
+            dw = torch.empty_like(w2) if w2.is_contiguous() else w2.new_empty(w2.shape)
         db = x2.new_empty(w2.shape[0]) if nb else None
         if nx or nw or nb:
             a, dy = ctx.args, _rows(grad_out, w2.shape[0])
