@@ -70,7 +70,6 @@ template <typename T, bool NANFIX> struct LinEpi {
   static constexpr bool STAGED = true;
   MatEpi e;
   long long J;
-  int vec;  // every tensor of the epilogue takes vectors of four
   struct Values {  // NANFIX: an operand's planes; element (i, t) at i si + t st
     const bf16_t* p;
     long long plane, si, st;
@@ -94,7 +93,7 @@ template <typename T, bool NANFIX> struct LinEpi {
     for (; t < K && s == s; ++t) s = fmaf(a.at(i, t), b.at(j, t), s);
     return s;
   }
-  // V: all four columns are there and every tensor takes them as one vector
+  // V: all four columns are there
   template <int STEP, bool V> __device__ __forceinline__ void put4_as(int i, int j, f32x4_m* v, int I, int jn) const {
     typedef typename PreT<T>::type preT;
     typedef T v4 __attribute__((ext_vector_type(4)));
@@ -102,7 +101,7 @@ template <typename T, bool NANFIX> struct LinEpi {
     // load under a branch is waited for by itself)
     const auto fetch = [&](const T* row) {
       v4 x;
-      if (V) return *reinterpret_cast<const v4*>(row + j);
+      if (V) return load_v<v4>(row + j);
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = row[j + min(r, jn - 1)];
       return x;
@@ -130,7 +129,7 @@ template <typename T, bool NANFIX> struct LinEpi {
           mat_preact(&q, v[u][r]);
           p[r] = q;
         }
-        if (V) *reinterpret_cast<p4*>(o) = p;
+        if (V) store_v(o, p);
         else
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -145,7 +144,7 @@ template <typename T, bool NANFIX> struct LinEpi {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[u][r] += e.beta * to_f(res[u][r]);
       }
-      store4(static_cast<T*>(e.out) + (i + u * STEP) * e.ldo + j, v[u], jn, V);
+      store4(static_cast<T*>(e.out) + (i + u * STEP) * e.ldo + j, v[u], jn);
     }
   }
   // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store, so that they are in
@@ -159,7 +158,7 @@ template <typename T, bool NANFIX> struct LinEpi {
         for (int r = 0; r < 4; ++r)
           if (i + u * STEP < I && r < jn && !(fabsf(v[u][r]) < __builtin_inff())) v[u][r] = again(i + u * STEP, j + r);
     }
-    if (jn >= 4 && vec) put4_as<STEP, true>(i, j, v, I, 4);
+    if (jn >= 4) put4_as<STEP, true>(i, j, v, I, 4);
     else put4_as<STEP, false>(i, j, v, I, jn);
   }
   __device__ __forceinline__ bool turned() const { return false; }
@@ -170,8 +169,6 @@ template <typename T, bool NANFIX> struct LinEpi {
     put4<1>(i, j, w, i + 1, jn);
   }
 };
-
-bool vec4(const void* p, long long ld, int elt) { return !p || (reinterpret_cast<uintptr_t>(p) % (4 * elt) == 0 && ld % 4 == 0); }
 
 // An operand as planes, both of a product in one launch (bound by memory, or by the launch: 777 x 1001 and 515 x 1001 of
 // f16 5.9 us).  Copied (16-bit) or split (f32) into rows of whole chunks, padding zeroed
@@ -198,12 +195,9 @@ __global__ __launch_bounds__(256) void pack_kernel(Packs ps) {
     const long long row = u / nc;
     const int c = (int)(u - row * nc) * 8;
     const T* s = static_cast<const T*>(p.src) + row * p.ld + c;
-    T v[8];
-    if (c + 8 <= p.cols && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
-      typedef T vt __attribute__((ext_vector_type(MatT<T>::VEC)));
-#pragma unroll
-      for (int h = 0; h < 8 / MatT<T>::VEC; ++h)
-        *reinterpret_cast<vt*>(v + h * MatT<T>::VEC) = *reinterpret_cast<const vt*>(s + h * MatT<T>::VEC);
+    __align__(16) T v[8];
+    if (c + 8 <= p.cols) {
+      __builtin_memcpy(v, s, sizeof(v));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? s[e] : from_f<T>(0.f);
@@ -304,8 +298,6 @@ void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStr
   j.K = (int)m.K;
   j.e.e = m.e;
   j.e.J = m.J;
-  j.e.vec = vec4(m.e.bias, 4, sizeof(T)) && vec4(m.e.residual, m.e.ldr, sizeof(T)) && vec4(m.e.out, m.e.ldo, sizeof(T)) &&
-            vec4(m.e.preact, m.J, sizeof(typename PreT<T>::type));
   if constexpr (P == 3) {
     j.e.a = {static_cast<const bf16_t*>(a.p), a.rows * a.ld, a.strided ? 1 : a.ld, a.strided ? a.ld : 1};
     j.e.b = {static_cast<const bf16_t*>(b.p), b.rows * b.ld, b.strided ? 1 : b.ld, b.strided ? b.ld : 1};
@@ -343,7 +335,7 @@ void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void*
 constexpr int kGemvRows = 2;
 template <typename T, int M, int KW>
 __global__ __launch_bounds__(256) void gemv_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
-                                                   long long ldw, int n, int k, int vec, MatEpi e) {
+                                                   long long ldw, int n, int k, MatEpi e) {
   constexpr int V = MatT<T>::VEC, R = 2;
   typedef T vecT __attribute__((ext_vector_type(V)));
   __shared__ float red[4][M * R];
@@ -355,23 +347,21 @@ __global__ __launch_bounds__(256) void gemv_kernel(const T* __restrict__ x, long
 #pragma unroll
     for (int r = 0; r < R; ++r) wr[r] = w + std::min(j0 + r, n - 1) * ldw;
     int t = (part * 64 + lane) * V;
-    if (vec) {
 #pragma unroll 4
-      for (; t + V <= k; t += KW * 64 * V) {
-        vecT xv[M], wv[R];
+    for (; t + V <= k; t += KW * 64 * V) {
+      vecT xv[M], wv[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) wv[r] = *reinterpret_cast<const vecT*>(wr[r] + t);
+      for (int r = 0; r < R; ++r) wv[r] = load_v<vecT>(wr[r] + t);
 #pragma unroll
-        for (int m = 0; m < M; ++m) xv[m] = *reinterpret_cast<const vecT*>(x + m * ldx + t);
+      for (int m = 0; m < M; ++m) xv[m] = load_v<vecT>(x + m * ldx + t);
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int q = 0; q < V; ++q) acc[m][r] = fmaf(to_f(xv[m][q]), to_f(wv[r][q]), acc[m][r]);
-      }
+          for (int q = 0; q < V; ++q) acc[m][r] = fmaf(to_f(xv[m][q]), to_f(wv[r][q]), acc[m][r]);
     }
-    // unaligned rows, and the last values of aligned ones
+    // the last values
     for (; t < k; t += KW * 64 * V)
       for (int q = 0; q < V && t + q < k; ++q)
 #pragma unroll
@@ -401,25 +391,20 @@ template <typename T, int M> void gemv_run_m(const MatArgs& p, hipStream_t st) {
   const T* x = static_cast<const T*>(p.a);
   const T* w = static_cast<const T*>(p.b);
   const int V = MatT<T>::VEC, n = (int)p.J, k = (int)p.K;
-  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
-                  (M == 1 || p.lda % V == 0) && (n == 1 || p.ldb % V == 0);
   if (k < 4 * 64 * V && n / 2 >= 8 * cu_count())
-    launch(gemv_kernel<T, M, 1>, dim3((n + 7) / 8), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, vec, p.e);
+    launch(gemv_kernel<T, M, 1>, dim3((n + 7) / 8), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, p.e);
   else
-    launch(gemv_kernel<T, M, 4>, dim3((n + 1) / 2), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, vec, p.e);
+    launch(gemv_kernel<T, M, 4>, dim3((n + 1) / 2), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, p.e);
 }
 template <typename T> void gemv_run(const MatArgs& p, hipStream_t st) {
   if (p.I == 1) gemv_run_m<T, 1>(p, st);
   else gemv_run_m<T, 2>(p, st);
 }
 
-// n of eight neighbours (more: all), zeros for the others; vec: they are aligned where all are there
-template <typename T> __device__ __forceinline__ void load8(const T* p, int n, int vec, T (&v)[8]) {
-  if (n >= 8 && vec) {
-    typedef T vt __attribute__((ext_vector_type(MatT<T>::VEC)));
-#pragma unroll
-    for (int h = 0; h < 8 / MatT<T>::VEC; ++h)
-      *reinterpret_cast<vt*>(v + h * MatT<T>::VEC) = *reinterpret_cast<const vt*>(p + h * MatT<T>::VEC);
+// n of eight neighbours (more: all), zeros for the others
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, T (&v)[8]) {
+  if (n >= 8) {
+    __builtin_memcpy(v, p, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : from_f<T>(0.f);
@@ -438,7 +423,7 @@ constexpr int kSkinnyRows = 16;
 template <typename T> constexpr int kSkinnySteps = sizeof(T) == 2 ? 8 : 4;
 template <typename T, int KW>
 __global__ __launch_bounds__(KW * 64) void skinny_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
-                                                         long long ldw, int rows, int n, int k, int vec, MatEpi e) {
+                                                         long long ldw, int rows, int n, int k, MatEpi e) {
   constexpr int U = kSkinnySteps<T>;
   __shared__ f32x4_m red[KW][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, g = lane >> 4;
@@ -447,14 +432,14 @@ __global__ __launch_bounds__(KW * 64) void skinny_kernel(const T* __restrict__ x
   const T* wr = w + (long long)min(j0 + row, n - 1) * ldw + g * 8;
   const T* xr = x + (long long)min(row, rows - 1) * ldx + g * 8;
   f32x4_m acc = {};
-  const int full = vec ? k / 32 : 0;
+  const int full = k / 32;
   for (int s0 = wave; s0 < full; s0 += KW * U) {
     __align__(16) T fw[U][8], fx[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {  // behind the last step: that one again, as zeros
       const int s = min(s0 + u * KW, full - 1) * 32;
-      load8(wr + s, 8, 1, fw[u]);
-      load8(xr + s, 8, 1, fx[u]);
+      load8(wr + s, 8, fw[u]);
+      load8(xr + s, 8, fx[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -464,10 +449,10 @@ __global__ __launch_bounds__(KW * 64) void skinny_kernel(const T* __restrict__ x
       acc = mfma_8(fw[u], fx[u], acc);
     }
   }
-  for (int s = full + wave; s * 32 < k; s += KW) {
+  if (wave == 0 && full * 32 < k) {
     __align__(16) T fw[8], fx[8];
-    load8(wr + s * 32, k - s * 32 - g * 8, vec, fw);
-    load8(xr + s * 32, k - s * 32 - g * 8, vec, fx);
+    load8(wr + full * 32, k - full * 32 - g * 8, fw);
+    load8(xr + full * 32, k - full * 32 - g * 8, fx);
     acc = mfma_8(fw, fx, acc);
   }
   red[wave][lane] = acc;
@@ -483,12 +468,10 @@ __global__ __launch_bounds__(KW * 64) void skinny_kernel(const T* __restrict__ x
 template <typename T> void skinny_run(const MatArgs& p, hipStream_t st) {
   const T* x = static_cast<const T*>(p.a);
   const T* w = static_cast<const T*>(p.b);
-  const int V = MatT<T>::VEC, n = (int)p.J, k = (int)p.K;
-  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 && p.lda % V == 0 &&
-                  (n == 1 || p.ldb % V == 0);
+  const int n = (int)p.J, k = (int)p.K;
   const dim3 grid((n + 15) / 16);
-  if (k >= 16 * 32 * kSkinnySteps<T>) launch(skinny_kernel<T, 16>, grid, dim3(1024), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, vec, p.e);
-  else launch(skinny_kernel<T, 4>, grid, dim3(256), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, vec, p.e);
+  if (k >= 16 * 32 * kSkinnySteps<T>) launch(skinny_kernel<T, 16>, grid, dim3(1024), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
+  else launch(skinny_kernel<T, 4>, grid, dim3(256), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
 }
 
 // --- few channels (k, n <= 64): every row's values are read and written once ---
@@ -498,8 +481,7 @@ template <typename T> void skinny_run(const MatArgs& p, hipStream_t st) {
 // there are few (4096 x 64 -> 64: f32 6.7 us against 7.3, bf16 4.8 against 4.0, 16 -> 16 3.6 against 3.9).
 template <typename T, int NT, int KS>
 __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w,
-                                                       long long ldw, long long rows, int n, int k, int vecx, int vecw,
-                                                       int vece, MatEpi e) {
+                                                       long long ldw, long long rows, int n, int k, MatEpi e) {
   typedef T v4 __attribute__((ext_vector_type(4)));
   typedef typename PreT<T>::type preT;
   typedef preT p4 __attribute__((ext_vector_type(4)));
@@ -510,7 +492,7 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int j = t * 16 + row, c = s * 32 + g * 8;
-      load8(w + (long long)min(j, n - 1) * ldw + c, j < n ? k - c : 0, vecw, fw[t][s]);
+      load8(w + (long long)min(j, n - 1) * ldw + c, j < n ? k - c : 0, fw[t][s]);
     }
   v4 bias[NT] = {};
   if (e.bias)
@@ -526,11 +508,11 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
     __align__(16) T fx[KS][8];
     v4 res[NT];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) load8(x + i * ldx + s * 32 + g * 8, in ? k - (s * 32 + g * 8) : 0, vecx, fx[s]);
-    if (e.residual && vece && in)
+    for (int s = 0; s < KS; ++s) load8(x + i * ldx + s * 32 + g * 8, in ? k - (s * 32 + g * 8) : 0, fx[s]);
+    if (e.residual && in)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
-        if (t * 16 + g * 4 < n) res[t] = *reinterpret_cast<const v4*>(static_cast<const T*>(e.residual) + i * e.ldr + t * 16 + g * 4);
+        if (t * 16 + g * 4 + 4 <= n) res[t] = load_v<v4>(static_cast<const T*>(e.residual) + i * e.ldr + t * 16 + g * 4);
     f32x4_m acc[NT] = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -542,7 +524,7 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
       const int j = t * 16 + g * 4;
       if (j >= n) continue;
       f32x4_m v = acc[t];
-      if (!vece) {
+      if (j + 4 > n) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (j + r < n) mat_store<T>(e, n, i, j + r, v[r]);
@@ -559,7 +541,7 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
           mat_preact(&z, v[r]);
           p[r] = z;
         }
-        *reinterpret_cast<p4*>(static_cast<preT*>(e.preact) + i * n + j) = p;
+        store_v(static_cast<preT*>(e.preact) + i * n + j, p);
       }
       v4 o;
 #pragma unroll
@@ -567,7 +549,7 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
         v[r] = mat_act<sizeof(T) == 2>(v[r], e.act, e.slope);
         o[r] = from_f<T>(e.residual ? v[r] + to_f(res[t][r]) : v[r]);
       }
-      *reinterpret_cast<v4*>(static_cast<T*>(e.out) + i * e.ldo + j) = o;
+      store_v(static_cast<T*>(e.out) + i * e.ldo + j, o);
     }
   }
 }
@@ -583,7 +565,7 @@ __global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy,
                                                        const T* __restrict__ x, long long ldx, const T* __restrict__ w,
                                                        long long ldw, T* __restrict__ dx, long long lddx,
                                                        float* __restrict__ part, long long rows, int n, int k, int act,
-                                                       float slope, int vecy, int vecx, int vecd, int want_w) {
+                                                       float slope, int want_w) {
   constexpr int NP = NT * 16, KP = KT * 16, PAD = MatT<T>::PAD, NS = (NP + 31) / 32 * 32;
   typedef T v4 __attribute__((ext_vector_type(4)));
   typedef typename PreT<T>::type preT;
@@ -613,9 +595,9 @@ __global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy,
       vy[u] = v4{};
       vz[u] = p4{};
       if (i < rows && j < n) {
-        if (vecy) {
-          vy[u] = *reinterpret_cast<const v4*>(dy + i * lddy + j);
-          if (act != CGAN3D_ACT_NONE) vz[u] = *reinterpret_cast<const p4*>(pre + i * n + j);
+        if (j + 4 <= n) {
+          vy[u] = load_v<v4>(dy + i * lddy + j);
+          if (act != CGAN3D_ACT_NONE) vz[u] = load_v<p4>(pre + i * n + j);
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -633,7 +615,7 @@ __global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy,
         const long long i = r0 + q / KC;
         vx[u] = v4{};
         if (i < rows && c < k) {
-          if (vecx) vx[u] = *reinterpret_cast<const v4*>(x + i * ldx + c);
+          if (c + 4 <= k) vx[u] = load_v<v4>(x + i * ldx + c);
           else
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -681,7 +663,7 @@ __global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy,
           v4 o;
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[r] = from_f<T>(ax[t][r]);
-          if (vecd) *reinterpret_cast<v4*>(dx + i * lddx + c) = o;
+          if (c + 4 <= k) store_v(dx + i * lddx + c, o);
           else
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -751,33 +733,26 @@ bool few_channels(long long n, long long k) { return n > 0 && k > 0 && n <= 64 &
 bool rows_bwd_takes(const cgan3d_linear_args* a) { return few_channels(a->n, a->k) && a->rows >= 64 && (a->dx || a->dw); }
 int rows_blocks(const cgan3d_linear_args* a) { return (int)std::min<long long>((a->rows + 63) / 64, kRowsBlocks); }
 
-template <typename T, int NT> void rows_fwd_nt(const MatArgs& p, int vecx, int vece, hipStream_t st) {
+template <typename T, int NT> void rows_fwd_nt(const MatArgs& p, hipStream_t st) {
   const T* x = static_cast<const T*>(p.a);
   const T* w = static_cast<const T*>(p.b);
-  const int vecw = reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.ldb % MatT<T>::VEC == 0;
   // four waves a block; enough blocks to fill the card, each wave going on from there
   const unsigned blocks = (unsigned)std::min((p.I + 63) / 64, 8LL * cu_count());
-  if (p.K <= 32) launch(rows_fwd_kernel<T, NT, 1>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vecw, vece, p.e);
-  else launch(rows_fwd_kernel<T, NT, 2>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, vecx, vecw, vece, p.e);
+  if (p.K <= 32) launch(rows_fwd_kernel<T, NT, 1>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, p.e);
+  else launch(rows_fwd_kernel<T, NT, 2>, dim3(blocks), dim3(256), 0, st, x, p.lda, w, p.ldb, p.I, (int)p.J, (int)p.K, p.e);
 }
 template <typename T> void rows_fwd_run(const MatArgs& p, hipStream_t st) {
-  const int vecx = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.lda % MatT<T>::VEC == 0;
-  const int vece = p.J % 4 == 0 && vec4(p.e.residual, p.e.ldr, sizeof(T)) && vec4(p.e.out, p.e.ldo, sizeof(T)) &&
-                   vec4(p.e.preact, p.J, sizeof(typename PreT<T>::type));
-  if (p.J <= 16) rows_fwd_nt<T, 1>(p, vecx, vece, st);
-  else if (p.J <= 32) rows_fwd_nt<T, 2>(p, vecx, vece, st);
-  else rows_fwd_nt<T, 4>(p, vecx, vece, st);
+  if (p.J <= 16) rows_fwd_nt<T, 1>(p, st);
+  else if (p.J <= 32) rows_fwd_nt<T, 2>(p, st);
+  else rows_fwd_nt<T, 4>(p, st);
 }
 
 template <typename T, int NT, int KT> void rows_bwd_nk(const cgan3d_linear_args* a, float* part, hipStream_t st) {
   typedef typename PreT<T>::type preT;
-  const int b = sizeof(T);
-  const int vecy = a->n % 4 == 0 && vec4(a->dy, a->lddy, b) && vec4(a->act != CGAN3D_ACT_NONE ? a->preact : nullptr, a->n, sizeof(preT));
-  const int vecx = a->k % 4 == 0 && vec4(a->x, a->ldx, b), vecd = a->k % 4 == 0 && vec4(a->dx, a->lddx, b);
   launch(rows_bwd_kernel<T, NT, KT>, dim3(rows_blocks(a)), dim3(256), 0, st, static_cast<const T*>(a->dy), (long long)a->lddy,
          static_cast<const preT*>(a->preact), static_cast<const T*>(a->x), (long long)a->ldx, static_cast<const T*>(a->w),
          (long long)a->ldw, static_cast<T*>(a->dx), (long long)a->lddx, part, (long long)a->rows, a->n, a->k, a->act,
-         a->slope, vecy, vecx, vecd, a->dw != nullptr ? 1 : 0);
+         a->slope, a->dw != nullptr ? 1 : 0);
 }
 template <typename T> void rows_bwd_run(const cgan3d_linear_args* a, void* ws, hipStream_t st) {
   float* part = a->dw || a->dbias ? static_cast<float*>(ws) : nullptr;
@@ -801,7 +776,7 @@ template <typename T, bool PL3>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, long long lddy,
                                                        const typename PreT<T>::type* __restrict__ pre, void* __restrict__ dzv,
                                                        int ldz, float* __restrict__ part, long long rows, int n,
-                                                       long long chunk, int act, float slope, int ct, int vec) {
+                                                       long long chunk, int act, float slope, int ct) {
   constexpr int V = MatT<T>::VEC;
   typedef typename PreT<T>::type preT;
   typedef T vecT __attribute__((ext_vector_type(V)));
@@ -814,12 +789,12 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
   if (j < n || (dzv && j < ldz)) {
     for (long long i = (long long)blockIdx.y * chunk + r; i < i1; i += rt) {
       float v[V];
-      if (vec && j + V <= n) {
-        const vecT y = *reinterpret_cast<const vecT*>(dy + i * lddy + j);
+      if (j + V <= n) {
+        const vecT y = load_v<vecT>(dy + i * lddy + j);
 #pragma unroll
         for (int q = 0; q < V; ++q) v[q] = to_f(y[q]);
         if (act != CGAN3D_ACT_NONE) {
-          const vecP z = *reinterpret_cast<const vecP*>(pre + i * n + j);
+          const vecP z = load_v<vecP>(pre + i * n + j);
 #pragma unroll
           for (int q = 0; q < V; ++q) v[q] *= mat_act_grad<sizeof(T) == 2>(to_f(z[q]), act, slope);
         }
@@ -908,12 +883,10 @@ ActGrid act_grid(const cgan3d_linear_args* a) {
 template <typename T, bool PL3>
 void act_grad_run(const cgan3d_linear_args* a, void* dz, int ldz, float* part, hipStream_t st) {
   const ActGrid g = act_grid(a);
-  const int vec = reinterpret_cast<uintptr_t>(a->dy) % 16 == 0 && a->lddy % MatT<T>::VEC == 0 &&
-                  (a->act == CGAN3D_ACT_NONE || (reinterpret_cast<uintptr_t>(a->preact) % 32 == 0 && a->n % MatT<T>::VEC == 0));
   if (g.nb > 0 && a->n > 0)
     launch(act_grad_kernel<T, PL3>, dim3(g.bx, (unsigned)g.nb), dim3(256), 0, st, static_cast<const T*>(a->dy),
            (long long)a->lddy, static_cast<const typename PreT<T>::type*>(a->preact), dz, ldz, part, (long long)a->rows,
-           a->n, g.chunk, a->act, a->slope, g.ct, vec);
+           a->n, g.chunk, a->act, a->slope, g.ct);
   if (a->dbias && a->n > 0)
     launch(bias_join_kernel<T>, dim3((a->n + 15) / 16), dim3(256), 0, st, (const float*)part, (int)g.nb, a->n,
            static_cast<T*>(a->dbias));

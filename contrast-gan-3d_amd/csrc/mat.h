@@ -50,12 +50,21 @@ __device__ __forceinline__ f32x4_m mfma_8(const float* a, const float* b, f32x4_
   return c;
 }
 
-// n of four neighbours (more than four: all); vec: they are aligned where all four are there
-template <typename T> __device__ __forceinline__ f32x4_m load4(const T* p, int n, int vec) {
+// A vector at any address of whole elements: global memory takes accesses of up to 16 bytes unaligned, which then cost a
+// second line now and then and not an access per value (rows of 7195 f32 values, measured at skinny_kernel).
+template <typename V, typename T> __device__ __forceinline__ V load_v(const T* p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+template <typename V, typename T> __device__ __forceinline__ void store_v(T* p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
+
+// n of four neighbours (more than four: all)
+template <typename T> __device__ __forceinline__ f32x4_m load4(const T* p, int n) {
   f32x4_m v = {0.f, 0.f, 0.f, 0.f};
-  if (n >= 4 && vec) {
+  if (n >= 4) {
     typedef T v4 __attribute__((ext_vector_type(4)));
-    const v4 x = *reinterpret_cast<const v4*>(p);
+    const v4 x = load_v<v4>(p);
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = to_f(x[r]);
   } else {
@@ -65,13 +74,13 @@ template <typename T> __device__ __forceinline__ f32x4_m load4(const T* p, int n
   }
   return v;
 }
-template <typename T> __device__ __forceinline__ void store4(T* p, f32x4_m v, int n, int vec) {
-  if (n >= 4 && vec) {
+template <typename T> __device__ __forceinline__ void store4(T* p, f32x4_m v, int n) {
+  if (n >= 4) {
     typedef T v4 __attribute__((ext_vector_type(4)));
     v4 x;
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = from_f<T>(v[r]);
-    *reinterpret_cast<v4*>(p) = x;
+    store_v(p, x);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -241,8 +250,8 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
     vecT v = {};
     if (outer < no && inner < ni) {
       const T* s = base + outer * ld + inner;
-      if (inner + V <= ni && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
-        v = *reinterpret_cast<const vecT*>(s);
+      if (inner + V <= ni) {
+        v = load_v<vecT>(s);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)

@@ -71,9 +71,9 @@ __global__ __launch_bounds__(256) void norm_kernel(MatList l) {
   const T* g = static_cast<const T*>(m.g);
   const long long total = (long long)m.rows * m.cols, tid = (long long)blockIdx.x * 256 + threadIdx.x;
   double s = 0.;
-  if ((m.ldg == m.cols || m.rows == 1) && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+  if (m.ldg == m.cols || m.rows == 1) {
     for (long long q = tid; q < total / V; q += kNormBlocks * 256LL) {
-      const vecT x = reinterpret_cast<const vecT*>(g)[q];
+      const vecT x = load_v<vecT>(g + q * V);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const double v = to_f(x[e]);
@@ -266,29 +266,15 @@ struct StepEpi {
 
   __device__ __forceinline__ bool turned() const { return tall && mode; }
 
-  // four values at p, neighbours in memory, n of them
-  template <typename T> static __device__ __forceinline__ void store(T* p, f32x4_m x, int n) {
-    typedef T v4 __attribute__((ext_vector_type(4)));
-    if (n >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0) {
-      v4 o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = (T)x[r];
-      *reinterpret_cast<v4*>(p) = o;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < n) p[r] = (T)x[r];
-    }
-  }
   // the last step's values x at offset d of the result or the parameter, n of them
   __device__ __forceinline__ void finish(long long d, f32x4_m x, int n) const {
     x *= 1.f / kXs;
     if (mode == 1 + CGAN3D_DT_F32) {
-      store(static_cast<float*>(res) + d, x, n);
+      store4(static_cast<float*>(res) + d, x, n);
     } else if (mode == 1 + CGAN3D_DT_BF16) {
-      store(static_cast<bf16_t*>(res) + d, x, n);
+      store4(static_cast<bf16_t*>(res) + d, x, n);
     } else if (mode == 1 + CGAN3D_DT_F16) {
-      store(static_cast<f16_t*>(res) + d, x, n);
+      store4(static_cast<f16_t*>(res) + d, x, n);
     } else {
       float* p = static_cast<float*>(res) + d;
       const float lr = hyper[H_LR], clip = hyper[H_CLIP], keep = 1.f - lr * hyper[H_WD], rate = lr * scale;
@@ -298,7 +284,7 @@ struct StepEpi {
         w[r] = r < n ? p[r] * keep - rate * x[r] : 0.f;
         if (clip > 0.f) w[r] = fminf(fmaxf(w[r], -clip), clip);
       }
-      store(p, w, n);
+      store4(p, w, n);
     }
   }
   // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store
@@ -380,12 +366,15 @@ __global__ __launch_bounds__(256) void planes_kernel(MatList l, PlaneMats pm, fl
       const int i = i0 + q / 16, t = t0 + q % 16 * 4;
       if (i >= p.s || t >= p.ldx) continue;
       f16x4_m h, lo;
+      f32x4_m x;
+      if (tall)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = tile[t - t0 + r][i - i0];
+      else x = load4<T>(g + i * m.ldg + t, p.l - t);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = 0.f;
-        if (t + r < p.l) x = (tall ? tile[t - t0 + r][i - i0] : to_f(g[i * m.ldg + t + r])) / norm * kXs;
         f16_t v[2];
-        split2(x, v);
+        split2(x[r] / norm * kXs, v);
         h[r] = v[0];
         lo[r] = v[1];
       }
@@ -511,7 +500,6 @@ struct SlabMat {
   int rows, cols;   // rows 0: a vector of `count` values
   float scale;
   int nslab, sub;   // blocks, and slabs a block takes
-  int vec_g, vec_o; // rows of G (and the momentum) / of the result start at multiples of four aligned values
   long long count;
   f16_t* x;         // planes, [slab][2][64][kCols], LDS order
   float* part;      // [2][nslab][64 * 64]
@@ -598,8 +586,8 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
         const int i = slab_i(tall, u, tid), t = t0 + slab_t(tall, u, tid);
         const int n = i < s && t < len ? (tall ? s - i : len - t) : 0;
         const long long o = tall ? t * m.ldg + i : i * m.ldg + t;
-        v[u] = load4<T>(g + o, n, m.vec_g);
-        w[u] = hyper ? load4<float>(m.mom + o, n, m.vec_g) : f32x4_m{0.f, 0.f, 0.f, 0.f};
+        v[u] = load4<T>(g + o, n);
+        w[u] = hyper ? load4<float>(m.mom + o, n) : f32x4_m{0.f, 0.f, 0.f, 0.f};
       }
       if (!hyper) return;
 #pragma unroll
@@ -608,7 +596,7 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
         const int n = i < s && t < len ? (tall ? s - i : len - t) : 0;
         w[u] += (1.f - mu) * (v[u] - w[u]);
         v[u] = nest ? v[u] + mu * (w[u] - v[u]) : w[u];
-        if (keep) store4<float>(m.mom + (tall ? t * m.ldg + i : i * m.ldg + t), w[u], n, m.vec_g);
+        if (keep) store4<float>(m.mom + (tall ? t * m.ldg + i : i * m.ldg + t), w[u], n);
       }
     };
     float big = 0.f;
@@ -820,7 +808,7 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
         for (int u = 0; u < 4; ++u) {
           const int i = slab_i(tall, u, tid), t = t0 + slab_t(tall, u, tid);
           const int n = hyper && i < s && t < len ? (tall ? s - i : len - t) : 0;
-          w[u] = load4<float>(static_cast<const float*>(m.out) + (tall ? t * m.ldo + i : i * m.ldo + t), n, m.vec_o);
+          w[u] = load4<float>(static_cast<const float*>(m.out) + (tall ? t * m.ldo + i : i * m.ldo + t), n);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -839,9 +827,9 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
             if (clip > 0.f)
 #pragma unroll
               for (int r = 0; r < 4; ++r) x[r] = fminf(fmaxf(x[r], -clip), clip);
-            store4<float>(static_cast<float*>(m.out) + o, x, n, m.vec_o);
+            store4<float>(static_cast<float*>(m.out) + o, x, n);
           } else {
-            store4<T>(static_cast<T*>(m.out) + o, x, n, m.vec_o);
+            store4<T>(static_cast<T*>(m.out) + o, x, n);
           }
         }
         lds_barrier();
@@ -862,13 +850,11 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
 bool slab_takes(long long rows, long long cols) { return std::min(rows, cols) <= 64; }
 
 // blocks of a matrix, and its part of the workspace from `ws` on
-long long slab_place(SlabMat& m, char* ws, int elt) {
+long long slab_place(SlabMat& m, char* ws) {
   const int len = std::max(m.rows, m.cols), all = (len + kCols - 1) / kCols;
   m.sub = (all + kMaxSlabs - 1) / kMaxSlabs;
   m.nslab = (all + m.sub - 1) / m.sub;
   const long long xb = (long long)m.nslab * m.sub * kSlab * 4, pb = 2LL * m.nslab * 4096 * 4;
-  m.vec_g = m.ldg % 4 == 0 && reinterpret_cast<uintptr_t>(m.g) % (4 * elt) == 0 && reinterpret_cast<uintptr_t>(m.mom) % 16 == 0;
-  m.vec_o = m.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(m.out) % (4 * elt) == 0;
   m.x = reinterpret_cast<f16_t*>(ws);
   m.part = reinterpret_cast<float*>(ws + xb);
   m.expo = reinterpret_cast<float*>(ws + xb + pb);
@@ -964,7 +950,7 @@ template <class F> long long slab_bytes(int n, F rc) {
     SlabMat m = {};
     m.rows = (int)r;
     m.cols = (int)c;
-    sum += slab_place(m, nullptr, 4);
+    sum += slab_place(m, nullptr);
     most = std::max(most, sum);
     if (++at == kSlabMats) at = 0, sum = 0;
   }
@@ -1041,7 +1027,7 @@ void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, cha
         SlabMat& m = sl.m[sl.n++];
         m = {};
         m.g = q.g; m.out = q.out; m.ldg = q.ldg; m.ldo = q.ldo; m.rows = q.rows; m.cols = q.cols;
-        used += slab_place(m, ws + w.x + used, sizeof(T));
+        used += slab_place(m, ws + w.x + used);
       }
       if (sl.n == kSlabMats || (i == n - 1 && sl.n > 0)) {
         slab_run<T>(sl, steps, co, eps, nullptr, st);
@@ -1234,7 +1220,7 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
     m.rows = (int)segs[i].rows; m.cols = (int)segs[i].cols;
     m.ldg = m.ldo = m.cols;
     m.scale = segs[i].lr_scale;
-    used += slab_place(m, base + w.x + used, 4);
+    used += slab_place(m, base + w.x + used);
     if (--left > 0 && sl.n < kSlabMats) continue;
     for (int v = 0; v < n && ride > 0; ++v) {
       if (segs[v].rows > 0 || segs[v].cols == 0) continue;
