@@ -395,9 +395,11 @@ __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
   const int t = b / SUB, sub = b - t * SUB;
   int ti, tj;
   plane_tile<BM, SYM>(t, p.I, p.tj, ti, tj);
+  bool across = SYM;
+  if constexpr (!SYM) across = p.e.turned();
   for (int q = threadIdx.x; q < 16 * BN / 4; q += 256) {
-    // 16 lanes on 16 rows, as the products leave them: a mirrored value's neighbours are written together
-    const int li = sub * 16 + q % 16, lj = q / 16 * 4, i = ti * BM + li, j = tj * BN + lj;
+    // lanes along a row; a value that is (also) written to a column: 16 lanes on 16 rows, as the products leave them
+    const int li = sub * 16 + (across ? q % 16 : q / (BN / 4)), lj = (across ? q / 16 : q % (BN / 4)) * 4, i = ti * BM + li, j = tj * BN + lj;
     if (i >= p.I || j >= p.J) continue;
     const float* s = p.part + (long long)t * (BM * BN) + li * BN + lj;
     f32x4_m v = *reinterpret_cast<const f32x4_m*>(s);
