@@ -183,7 +183,10 @@ struct Packs {
   Pack p[2];
   long long chunks;
 };
-long long up8(long long v) { return (v + 7) / 8 * 8; }
+// Row length of planes: whole 16-byte chunks, and whole 128-byte lines where that adds little: the products fetch 64 bytes
+// of each row at a time, which else lie in two lines (bf16 97852 x 520 -> 1024, us by row length: 520 196, 544 186, 576
+// 165; 8192 x 1000 -> 1024: 1000 33.6, 1008 31.4, 1024 28.1).
+long long row_pad(long long cols) { return cols >= 256 ? (cols + 63) / 64 * 64 : (cols + 7) / 8 * 8; }
 long long up256(long long v) { return (v + 255) / 256 * 256; }
 
 template <typename T>
@@ -254,8 +257,8 @@ Route mat_route(int dt, long long I, long long J, long long K, bool ready) {
 
 long long operand_bytes(int dt, const Operand& o) {
   if (o.planes) return 0;
-  if (dt == CGAN3D_DT_F32) return up256(o.rows * up8(o.cols) * 6);
-  return chunked(o.p, o.ld, o.cols) ? 0 : up256(o.rows * up8(o.cols) * 2);
+  if (dt == CGAN3D_DT_F32) return up256(o.rows * row_pad(o.cols) * 6);
+  return chunked(o.p, o.ld, o.cols) ? 0 : up256(o.rows * row_pad(o.cols) * 2);
 }
 PlanePick pick_for(int dt, long long I, long long J, long long K) {
   const PlaneShape s = {(int)I, (int)J, (int)K};
@@ -278,7 +281,7 @@ void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStr
   for (Operand* o : os) {
     const long long bytes = operand_bytes(dt, *o);
     if (!bytes) continue;
-    const int ldp = (int)up8(o->cols);
+    const int ldp = (int)row_pad(o->cols);
     ps.p[np++] = {o->p, o->ld, o->rows, o->cols, ldp, at, ps.chunks};
     ps.chunks += o->rows * (ldp / 8);
     o->p = at;
@@ -869,7 +872,7 @@ struct ActGrid {
 ActGrid act_grid(const cgan3d_linear_args* a) {
   const int v = a->dtype == CGAN3D_DT_F32 ? 4 : 8;
   ActGrid g;
-  const long long width = up8(a->n);
+  const long long width = row_pad(a->n);
   g.ct = 1;
   while (g.ct < 32 && g.ct * v < width) g.ct *= 2;
   g.bx = (int)((width + g.ct * v - 1) / (g.ct * v));
@@ -911,7 +914,7 @@ Bwd bwd_layout(const cgan3d_linear_args* a) {
               a->k < big && f32_planes(a->rows, a->k, a->n, true) && f32_planes(a->n, a->k, a->rows, true);
   const bool direct = a->act == CGAN3D_ACT_NONE && !w.planes3 && (dt == CGAN3D_DT_F32 || chunked(a->dy, a->lddy, a->n));
   w.has_dz = !direct && (a->dx || a->dw);
-  w.ldz = (int)up8(a->n);
+  w.ldz = (int)row_pad(a->n);
   long long at = w.has_dz ? up256(a->rows * w.ldz * (w.planes3 ? 6 : dt_bytes(dt))) : 0;
   w.part = at;
   if (a->dbias) at += up256(act_grid(a).nb * a->n * 4);
