@@ -484,9 +484,10 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
 // seventeen and joins.  Bound by latency: a launch of 64 x 1728 is ~7.5 us, of which a fourth is the trip to the
 // arguments, and about as much each the Gram partials, the step and the Gram product.  Measured, us, here / on planes:
 // 16 x 343 50 / 69, 64 x 1728 55 / 98, 64 x 16384 103 / 139, 64 x 65536 182 / 213, four of these 250 / 417; a
-// very long single one loses (16 x 200000 381 / 332).  kMaxSlabs 32 / 64 / 128: 64 x 16384
-// 99 / 103 / 103, 64 x 65536 244 / 182 / 186, four of these 288 / 250 / 399.  G's planes are scaled by the power of two of the slab's largest value, and the norm is the trace of
-// the partial Gram matrices, in 64 bits: no pass of its own.  Vectors' Adam rides on launch 0.
+// very long single one loses (16 x 200000 381 / 332).  kMaxSlabs 32 / 64 / 128: 64 x 16384 99 / 103 / 103, 64 x 65536
+// 244 / 182 / 186, four of these 288 / 250 / 399.  G's planes are scaled by the power of two of the slab's largest value,
+// and the norm is the trace of the partial Gram matrices, in 64 bits: no pass of its own.  Vectors' Adam rides on
+// launch 0.
 constexpr int kSlabMats = 28, kMaxSlabs = 64, kBatch = 16, kCols = 256, kSlab = 64 * kCols;
 constexpr int kSlabThreads = 4 * kCols, kSlabWaves = kSlabThreads / 64;  // a wave: 16 columns, and one tile of a 64 x 64 matrix
 static_assert(kSlabWaves == 16, "a wave for each tile of the Gram matrix");
