@@ -78,6 +78,10 @@ def _forward(x, x2, w2, bias, residual, act, slope, preact):
     return y, args
 
 
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, slope):
@@ -87,6 +91,7 @@ class _LinearFn(torch.autograd.Function):
             preact = torch.empty((x2.shape[0], n), dtype=ops.linear_preact_dtype(x.dtype), device=x.device)
         y, ctx.args = _forward(x, x2, w2, bias, residual, act, slope, preact)
         ctx.shape, ctx.act, ctx.slope = x.shape, act, slope
+        ctx.layout = _layout(x2), _layout(w2), _layout(preact)
         ctx.save_for_backward(x2, w2, preact)
         return y
 
@@ -105,9 +110,9 @@ class _LinearFn(torch.autograd.Function):
         if nx or nw or nb:
             a, dy = ctx.args, _rows(grad_out, w2.shape[0])
             here = (x2.data_ptr() or None, w2.data_ptr() or None, None if preact is None else preact.data_ptr() or None)
-            if here == (a.x, a.w, a.preact):
+            if here == (a.x, a.w, a.preact) and (_layout(x2), _layout(w2), _layout(preact)) == ctx.layout:
                 ops._linear_backward_of(a, dy, x2, dx, dw, db)
-            else:  # hooks on saved tensors gave others back
+            else:  # hooks on saved tensors gave others back: elsewhere, or where the freed ones were, but dense
                 ops.linear_backward(dy, x2, w2, dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db,
                                     ctx.act, ctx.slope, preact)
         return dx, dw, db, grad_out if nr else None, None, None
