@@ -50,7 +50,7 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     """``act(x weight^T + bias) + residual``: x [..., k], weight [n, k], bias [n], residual of the result's
     shape [..., n]; all of one dtype (float32, bfloat16 or float16).  ``act``: an activation code
     (``_lib.ACT_NONE``, ``ACT_RELU``, ``ACT_LRELU`` with ``slope``, ``ACT_TANH``, ``ACT_GELU``, ``ACT_SILU``).
-    Differentiable once.  A HIP graph that captures the backward pass must be the only autograd graph alive
+    Differentiable once, in reverse mode.  A HIP graph that captures the backward pass must be the only autograd graph alive
     on its leaves (torch's own rule: their gradient accumulators belong to the stream they were made on)."""
     xs, ws = x.shape, weight.shape
     if len(ws) != 2 or not xs or xs[-1] != ws[1]:
@@ -59,6 +59,7 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
                                  or residual.shape[:-1] != xs[:-1]):
         raise ValueError(f"fused_linear: residual {tuple(residual.shape)} is not of the result's shape "
                          f"{(*xs[:-1], ws[0])}")
+    ops._no_tangents("fused_linear", x, weight, bias, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _LinearFn.apply(x, weight, bias, residual, act, slope)
@@ -99,6 +100,7 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, grad_out):
         if torch.is_grad_enabled():
             raise NotImplementedError("double backward through the HIP linear block is not implemented")
+        ops._no_tangents("fused_linear's backward pass", grad_out)
         x2, w2, preact = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = None

@@ -16,6 +16,7 @@ import os
 from typing import Dict, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from ._lib import ConvGeom, Epilogue, PackDesc, check, ptr
@@ -1504,6 +1505,13 @@ def _elsewhere(device):
     return not DRY_RUN and device.index is not None and device.index != torch.cuda.current_device()
 
 
+def _no_tangents(who, *tensors):
+    """Refuses forward-mode derivatives, which would be dropped (a result without a tangent is a derivative of zero)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f"{who}: no forward-mode derivative")
+
+
 LINEAR_ACTS = (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU, L.ACT_TANH, L.ACT_GELU, L.ACT_SILU)
 
 
@@ -1617,6 +1625,7 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
         raise ValueError(f"orthogonalize: matrices needed, got shape {tuple(g.shape)}")
     if g.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("orthogonalize has no gradient: call it under torch.no_grad() or on g.detach()")
+    _no_tangents("orthogonalize", g)
     dt, dev = _dt(g, "orthogonalize g"), g.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):

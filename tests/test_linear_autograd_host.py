@@ -61,3 +61,40 @@ def test_saved_tensors_that_stay_take_the_forward_arguments(calls):
     torch.autograd.grad(fused_linear(x, w), (x, w), torch.ones(6, 5))
     bwd = calls[1][1]
     assert (bwd.ldx, bwd.ldw, bwd.x, bwd.w) == (16, 8, x.data_ptr(), w.data_ptr())
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_derivatives_are_refused(dry, which, leaf):
+    """A dual tensor's tangent is not dropped without a word, whether or not something requires grad."""
+    import torch.autograd.forward_ad as fw
+    from cgan3d_amd.model.linear import fused_linear
+    ts = [torch.randn(6, 8), torch.randn(5, 8), torch.randn(5), torch.randn(6, 5)]
+    if leaf:
+        ts[which].requires_grad_(True)
+    with fw.dual_level():
+        fused_linear(*ts)  # no tangents: as ever
+        ts[which] = fw.make_dual(ts[which], torch.ones_like(ts[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            fused_linear(*ts)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            fused_linear(*ts)
+
+
+def test_orthogonalize_refuses_forward_mode(dry):
+    import torch.autograd.forward_ad as fw
+    g = torch.randn(4, 4)
+    with fw.dual_level():
+        dry.orthogonalize(g)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            dry.orthogonalize(fw.make_dual(g, torch.ones(4, 4)))
+
+
+def test_backward_refuses_a_tangent(dry):
+    import torch.autograd.forward_ad as fw
+    from cgan3d_amd.model.linear import fused_linear
+    x = torch.randn(6, 8).requires_grad_(True)
+    with fw.dual_level():
+        y = fused_linear(x, torch.randn(5, 8))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, fw.make_dual(torch.ones(6, 5), torch.ones(6, 5)))
