@@ -98,3 +98,38 @@ def test_backward_refuses_a_tangent(dry):
         y = fused_linear(x, torch.randn(5, 8))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, fw.make_dual(torch.ones(6, 5), torch.ones(6, 5)))
+
+
+def _uses(ops):
+    from cgan3d_amd.model.linear import fused_linear
+    w = torch.randn(5, 8)
+    return [lambda x: fused_linear(x, w), lambda x: fused_linear(x.requires_grad_(True), w),
+            lambda x: ops.orthogonalize(x)]
+
+
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+@pytest.mark.parametrize("use", range(3))
+def test_tracing_is_refused(dry, use, mode):
+    """The program would be an empty buffer."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with pytest.raises(NotImplementedError, match="traced"):
+        make_fx(_uses(dry)[use], tracing_mode=mode)(torch.randn(6, 8))
+
+
+@pytest.mark.parametrize("use", [0, 2])
+def test_jit_trace_and_fake_tensors_are_refused(dry, use):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    f = _uses(dry)[use]
+    with pytest.raises(NotImplementedError, match="jit.trace"):
+        torch.jit.trace(f, (torch.randn(6, 8),))
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(NotImplementedError, match="fake"):
+        f(torch.randn(6, 8))
+
+
+def test_counting_modes_and_compiled_callers_run(dry):
+    """A mode that only watches is no tracer, and a compiled caller breaks its graph at the call."""
+    from torch.utils.flop_counter import FlopCounterMode
+    f = _uses(dry)[0]
+    with FlopCounterMode(display=False):
+        assert f(torch.randn(6, 8)).shape == (6, 5)
+    assert torch.compile(lambda x: f(x * 2) + 1, backend="eager")(torch.randn(6, 8)).shape == (6, 5)
