@@ -45,13 +45,23 @@ def _rows(t: Tensor, cols: int) -> Tensor:
     return t
 
 
+def _autocast(*tensors):
+    """The operands in autocast's dtype (float64 ones are left as they are, as torch leaves them)."""
+    dt = torch.get_autocast_dtype("cuda")
+    return [t.to(dt) if t is not None and t.dtype in L.DTYPES else t for t in tensors]
+
+
 def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: Tensor | None = None,
                  act: int = L.ACT_NONE, slope: float = 0.0) -> Tensor:
     """``act(x weight^T + bias) + residual``: x [..., k], weight [n, k], bias [n], residual of the result's
     shape [..., n]; all of one dtype (float32, bfloat16 or float16).  ``act``: an activation code
     (``_lib.ACT_NONE``, ``ACT_RELU``, ``ACT_LRELU`` with ``slope``, ``ACT_TANH``, ``ACT_GELU``, ``ACT_SILU``).
+    Under ``torch.autocast("cuda")`` all four are cast to its dtype first, as ``torch.nn.functional.linear``'s operands
+    are (the residual too: bias, activation and sum stay in 32 bits, the result is rounded to that dtype once).
     Differentiable once, in reverse mode.  A HIP graph that captures the backward pass must be the only autograd graph alive
     on its leaves (torch's own rule: their gradient accumulators belong to the stream they were made on)."""
+    if torch.is_autocast_enabled("cuda"):
+        x, weight, bias, residual = _autocast(x, weight, bias, residual)
     xs, ws = x.shape, weight.shape
     if len(ws) != 2 or not xs or xs[-1] != ws[1]:
         raise ValueError(f"fused_linear: x {tuple(xs)} does not multiply weight {tuple(ws)}")

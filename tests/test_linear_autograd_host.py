@@ -133,3 +133,29 @@ def test_counting_modes_and_compiled_callers_run(dry):
     with FlopCounterMode(display=False):
         assert f(torch.randn(6, 8)).shape == (6, 5)
     assert torch.compile(lambda x: f(x * 2) + 1, backend="eager")(torch.randn(6, 8)).shape == (6, 5)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_autocast_casts_the_operands(calls, dt):
+    """As torch's linear: half-precision activations beside f32 parameters run in autocast's type, and the parameters'
+    gradients come back in their own."""
+    from cgan3d_amd.model.linear import LinearBlock
+    torch.set_autocast_enabled("cuda", True)
+    torch.set_autocast_dtype("cuda", dt)
+    try:
+        blk = LinearBlock(8, 5, torch.nn.GELU)
+        for x in (torch.randn(6, 8).to(dt), torch.randn(6, 8)):
+            x.requires_grad_(True)
+            y = blk(x, residual=torch.randn(6, 5))
+            assert y.dtype == dt
+            gx, gw = torch.autograd.grad(y, (x, blk.linear.weight), torch.ones_like(y))
+            assert gx.dtype == x.dtype and gw.dtype == torch.float32
+        with torch.no_grad():
+            assert blk(x).dtype == dt
+        with pytest.raises(TypeError):
+            blk(torch.randn(6, 8).double())
+    finally:
+        torch.set_autocast_enabled("cuda", False)
+        torch.set_autocast_dtype("cuda", torch.float16)
+    from cgan3d_amd import _lib as L
+    assert [a.dtype for _, a in calls] == [L.DTYPES[dt]] * 5
