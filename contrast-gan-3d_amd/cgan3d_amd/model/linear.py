@@ -102,6 +102,7 @@ class _LinearFn(torch.autograd.Function):
             preact = torch.empty((x2.shape[0], n), dtype=ops.linear_preact_dtype(x.dtype), device=x.device)
         y, ctx.args = _forward(x, x2, w2, bias, residual, act, slope, preact)
         ctx.shape, ctx.act, ctx.slope = x.shape, act, slope
+        ctx.bias_shape = None if bias is None else bias.shape
         ctx.layout = _layout(x2), _layout(w2), _layout(preact)
         ctx.save_for_backward(x2, w2, preact)
         return y
@@ -127,6 +128,8 @@ class _LinearFn(torch.autograd.Function):
             else:  # hooks on saved tensors gave others back: elsewhere, or where the freed ones were, but dense
                 ops.linear_backward(dy, x2, w2, dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db,
                                     ctx.act, ctx.slope, preact)
+        if nb and db.shape != ctx.bias_shape:  # n values in any shape
+            db = db.view(ctx.bias_shape)
         return dx, dw, db, grad_out if nr else None, None, None
 
 

@@ -159,3 +159,12 @@ def test_autocast_casts_the_operands(calls, dt):
         torch.set_autocast_dtype("cuda", torch.float16)
     from cgan3d_amd import _lib as L
     assert [a.dtype for _, a in calls] == [L.DTYPES[dt]] * 5
+
+
+@pytest.mark.parametrize("shape", [(1, 5), (5, 1), (1, 1, 5), (5,)])
+def test_bias_of_any_shape_gets_its_gradient(dry, shape):
+    """n contiguous values in any shape are a bias; the gradient has that shape."""
+    from cgan3d_amd.model.linear import fused_linear
+    b = torch.randn(shape).requires_grad_(True)
+    y = fused_linear(torch.randn(6, 8), torch.randn(5, 8), b)
+    assert torch.autograd.grad(y, b, torch.ones(6, 5))[0].shape == b.shape
