@@ -277,6 +277,23 @@ PlanePick pick_for(int dt, long long I, long long J, long long K) {
   const PlaneShape s = {(int)I, (int)J, (int)K};
   return dt == CGAN3D_DT_F32 ? plane_pick<3, false>(&s, 1) : plane_pick<1, false>(&s, 1);
 }
+// Whether the product's launches are ones that HIP takes: fewer than 2^32 threads along x, sides that the kernels count in
+// 32 bits
+template <int P> long long plane_threads(const PlanePick& p, const PlaneShape& s) {
+  using C = PlaneCfg<P, false>;
+  return plane_tiles(s, C::BM[p.cfg], C::BN[p.cfg], false) * std::max(1, (s.K + p.kchunk - 1) / p.kchunk) * C::WI[p.cfg] *
+         C::WJ[p.cfg] * 64;
+}
+bool launchable(int dt, long long I, long long J, long long K, bool ready) {
+  const long long side = 1LL << 30, tiles = (I + kTile - 1) / kTile * ((J + kTile - 1) / kTile);
+  if (I == 0 || J == 0) return true;
+  if (I > side || J > side || K > side) return false;
+  if (tiles < 1 << 22) return true;  // of the smallest tile; no block has more than 512 threads, splits come with few tiles
+  if (mat_route(dt, I, J, K, ready) == ROUTE_MAT) return tiles * 256 < 1LL << 32;
+  const PlaneShape s = {(int)I, (int)J, (int)K};
+  const PlanePick p = pick_for(dt, I, J, K);
+  return (dt == CGAN3D_DT_F32 ? plane_threads<3>(p, s) : plane_threads<1>(p, s)) < 1LL << 32;
+}
 // workspace of one product: both operands' planes, then partial sums
 long long product_bytes(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
   if (I == 0 || J == 0) return 0;
@@ -341,6 +358,14 @@ void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void*
   }
 }
 
+// A grid along x and, where that would be 2^32 threads or more (HIP refuses it), y too.  Blocks past the last find nothing
+// to do.
+dim3 long_grid(long long blocks, int threads) {
+  const long long x = std::min(blocks, (1LL << 31) / threads);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ int long_block() { return blockIdx.x + gridDim.x * blockIdx.y; }
+
 // --- one or two rows: the weight is read once, 16 bytes a lane, and nothing else matters ---
 // Bound by memory.  A wave takes R = 2 columns of y, so that a load of x serves two of the weight; KW waves of the block
 // share the summed axis: 4, unless a wave would then get less than one load a column and the columns alone fill
@@ -356,7 +381,7 @@ __global__ __launch_bounds__(256) void gemv_kernel(const T* __restrict__ x, long
   typedef T vecT __attribute__((ext_vector_type(V)));
   __shared__ float red[4][M * R];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % KW;
-  const int j0 = (blockIdx.x * (4 / KW) + wave / KW) * R;
+  const int j0 = (long_block() * (4 / KW) + wave / KW) * R;
   float acc[M][R] = {};
   if (j0 < n) {
     const T* wr[R];
@@ -408,9 +433,9 @@ template <typename T, int M> void gemv_run_m(const MatArgs& p, hipStream_t st) {
   const T* w = static_cast<const T*>(p.b);
   const int V = MatT<T>::VEC, n = (int)p.J, k = (int)p.K;
   if (k < 4 * 64 * V && n / 2 >= 8 * cu_count())
-    launch(gemv_kernel<T, M, 1>, dim3((n + 7) / 8), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, p.e);
+    launch(gemv_kernel<T, M, 1>, long_grid((n + 7) / 8, 256), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, p.e);
   else
-    launch(gemv_kernel<T, M, 4>, dim3((n + 1) / 2), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, p.e);
+    launch(gemv_kernel<T, M, 4>, long_grid((n + 1) / 2, 256), dim3(256), 0, st, x, p.lda, w, p.ldb, n, k, p.e);
 }
 template <typename T> void gemv_run(const MatArgs& p, hipStream_t st) {
   if (p.I == 1) gemv_run_m<T, 1>(p, st);
@@ -443,7 +468,7 @@ __global__ __launch_bounds__(KW * 64) void skinny_kernel(const T* __restrict__ x
   constexpr int U = kSkinnySteps<T>;
   __shared__ f32x4_m red[KW][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, g = lane >> 4;
-  const int j0 = blockIdx.x * 16;
+  const int j0 = long_block() * 16;
   // rows that are not there: the last one again
   const T* wr = w + (long long)min(j0 + row, n - 1) * ldw + g * 8;
   const T* xr = x + (long long)min(row, rows - 1) * ldx + g * 8;
@@ -485,9 +510,10 @@ template <typename T> void skinny_run(const MatArgs& p, hipStream_t st) {
   const T* x = static_cast<const T*>(p.a);
   const T* w = static_cast<const T*>(p.b);
   const int n = (int)p.J, k = (int)p.K;
-  const dim3 grid((n + 15) / 16);
-  if (k >= 16 * 32 * kSkinnySteps<T>) launch(skinny_kernel<T, 16>, grid, dim3(1024), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
-  else launch(skinny_kernel<T, 4>, grid, dim3(256), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
+  const int blocks = (n + 15) / 16;
+  if (k >= 16 * 32 * kSkinnySteps<T>)
+    launch(skinny_kernel<T, 16>, long_grid(blocks, 1024), dim3(1024), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
+  else launch(skinny_kernel<T, 4>, long_grid(blocks, 256), dim3(256), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
 }
 
 // --- few channels (k, n <= 64): every row's values are read and written once ---
@@ -866,7 +892,7 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict_
   // 16 columns a block, 16 threads on each, added in a fixed order
   __shared__ double red[16][16];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-  const long long j = (long long)blockIdx.x * 16 + c;
+  const long long j = long_block() * 16LL + c;
   double s = 0.;
   if (j < n)
     for (int b = r; b < nb; b += 16) s += part[(long long)b * n + j];
@@ -904,7 +930,7 @@ void act_grad_run(const cgan3d_linear_args* a, void* dz, int ldz, float* part, h
            (long long)a->lddy, static_cast<const typename PreT<T>::type*>(a->preact), dz, ldz, part, (long long)a->rows,
            a->n, g.chunk, a->act, a->slope, g.ct);
   if (a->dbias && a->n > 0)
-    launch(bias_join_kernel<T>, dim3((a->n + 15) / 16), dim3(256), 0, st, (const float*)part, (int)g.nb, a->n,
+    launch(bias_join_kernel<T>, long_grid((a->n + 15) / 16, 256), dim3(256), 0, st, (const float*)part, (int)g.nb, a->n,
            static_cast<T*>(a->dbias));
 }
 
@@ -962,8 +988,11 @@ const char* lin_check(const cgan3d_linear_args* a, bool bwd) {
   if (a->dtype < CGAN3D_DT_F32 || a->dtype > CGAN3D_DT_F16) return "unknown dtype";
   if (a->rows < 0 || a->k < 0 || a->n < 0) return "negative size";
   if (a->rows > (1LL << 40) || a->k > 1 << 30 || a->n > 1 << 30) return "size too large";
-  const long long t = (a->rows + kTile - 1) / kTile, u = ((long long)std::max(a->k, a->n) + kTile - 1) / kTile;
-  if (t * u > INT_MAX || u * u > INT_MAX) return "too many tiles for one launch";
+  const bool fits = bwd ? rows_bwd_takes(a) || ((!a->dx || launchable(a->dtype, a->rows, a->k, a->n, false)) &&
+                                                (!a->dw || launchable(a->dtype, a->n, a->k, a->rows, false)))
+                        : a->rows <= kGemvRows || skinny_takes(a) || few_channels(a->n, a->k) ||
+                              launchable(a->dtype, a->rows, a->n, a->k, false);
+  if (!fits) return "too many tiles for one launch";
   if (a->act < CGAN3D_ACT_NONE || a->act > CGAN3D_ACT_SILU || a->act == CGAN3D_ACT_NEG_DTANH)
     return "activation must be none, relu, lrelu, tanh, gelu or silu";
   if ((a->k > 0 && a->rows > 0 && !a->x) || (a->k > 0 && a->n > 0 && !a->w)) return "null operand";

@@ -585,7 +585,9 @@ int cgan3d_adam(float* param, const float* grad, float* exp_avg, float* exp_avg_
  * A pointwise convolution over channels-last voxels, or any layer of rows times a weight in torch's
  * [out, in] layout.  Every tensor is of `dtype`; products are summed in f32 and rounded once, in the
  * epilogue.  Rows may be strided (ld*, elements; at least the row's length); preact, dz, dw and dbias are
- * contiguous.  Any size up to 2^30 columns (k, n) and 2^40 rows, zero included, and any alignment of whole elements.
+ * contiguous.  k and n up to 2^30, rows up to 2^30 (2^40 where k and n are at most 64, or where dbias alone is asked
+ * for), zero included, and any alignment of whole elements; a product of 2^24 tiles of 64 x 64 or more, which may need a
+ * grid that HIP does not take, is refused.
  *   forward : x, w, y; optional bias [n], residual (may be y itself), preact.
  *             preact [rows, n], f32, or f16 (saturating) for bf16 tensors: z = x w^T + bias, which the backward
  *             pass of an activation reads.

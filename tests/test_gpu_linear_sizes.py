@@ -1,0 +1,58 @@
+"""The linear block at sizes with one very long side, and the large tiles of its products.  Tolerances as in
+test_gpu_linear.py; where every product and sum is a whole number that f32 and the type hold, results are equal."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def whole(gen, *shape, top=2):
+    return torch.randint(-top, top + 1, shape, generator=gen, device="cuda", dtype=torch.int8)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,k,n", [(1, 4_096_000, 8), (7, 4_096_001, 8), (40, 4_096_003, 5), (8, 8, 4_096_000),
+                                      (40, 7, 4_096_001), (1, 3, 4_096_003)])
+def test_a_long_side_and_its_gradients(rows, k, n, dt):
+    """A flattened 160^3 volume as inputs or outputs.  Every 4099th value of a long sum is not zero: whole numbers below
+    2^8 at each step, so that every order of summation gives them exactly."""
+    from cgan3d_amd.model.linear import fused_linear
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    x, w, dy = whole(g, rows, k), whole(g, n, k), whole(g, rows, n, top=1)
+    if k > 100:
+        x *= (torch.arange(k, device="cuda") % 131071 == 5).to(torch.int8)  # 31 products of at most 4
+    if n > 100:
+        dy *= (torch.arange(n, device="cuda") % 131071 == 7).to(torch.int8)
+    t = DT[dt]
+    xs, ws = x.to(t).requires_grad_(True), w.to(t).requires_grad_(True)
+    b = torch.zeros(n, dtype=t, device="cuda", requires_grad=True)
+    y = fused_linear(xs, ws, b)
+    y.backward(dy.to(t))
+    x, w, dy = x.float(), w.float(), dy.float()
+    assert torch.equal(y.detach().float(), x @ w.T), "y"
+    assert torch.equal(xs.grad.float(), dy @ w), "dx"
+    assert torch.equal(ws.grad.float(), dy.T @ x), "dw"
+    assert torch.equal(b.grad.float(), dy.sum(0)), "db"
+
+
+def test_grids_beyond_one_axis():
+    """More blocks than a grid of one axis holds: one row, three rows, and the column sums alone."""
+    from cgan3d_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for rows, k, n, t in ((1, 4, (1 << 26) + 5, torch.bfloat16), (3, 1, (1 << 27) + 19, torch.float32)):
+        x, w = whole(g, rows, k).to(t), whole(g, n, k).to(t)
+        y = torch.full((rows, n), 7.0, dtype=t, device="cuda")
+        ops.linear(x, w, y)
+        for i in range(rows):
+            want = torch.zeros(n, dtype=torch.float32, device="cuda")
+            for q in range(k):
+                want += x[i, q].float() * w[:, q].float()
+            assert torch.equal(y[i].float(), want), (rows, n)
+        del y, w, want
+    n = (1 << 27) + 19
+    dy, db = whole(g, 2, n).float(), torch.full((n,), 7.0, device="cuda")
+    ops.linear_backward(dy, torch.empty(2, 0, device="cuda"), torch.empty(n, 0, device="cuda"), dbias=db)
+    assert torch.equal(db, dy[0] + dy[1])
