@@ -1007,6 +1007,10 @@ const char* mats_check(const cgan3d_ortho_mat* m, int n, int dt) {
   return nullptr;
 }
 
+// The f32 products run on tiles of 64 x 64, 256 threads each: HIP takes fewer than 2^32 threads.  (On planes the largest
+// matrices that fit the memory stay below it.)
+bool mat_grid_holds(long long rows, long long cols) { return ((rows + 63) / 64) * ((cols + 63) / 64) < 1 << 24; }
+
 Layout ortho_layout(const cgan3d_ortho_mat* m, int n) {
   Layout w = {};
   for (int i = 0; i < n; ++i) size_mat(w, m[i].rows, m[i].cols);
@@ -1109,6 +1113,9 @@ extern "C" int cgan3d_orthogonalize(const cgan3d_ortho_mat* mats, int32_t n, int
   CG_CHECK_ARG(!e, "cgan3d_orthogonalize: %s", e);
   e = ns_check(steps, coefficients, eps);
   CG_CHECK_ARG(!e, "cgan3d_orthogonalize: %s", e);
+  if (!planes_hold(steps, coefficients))
+    for (int i = 0; i < n; ++i)
+      CG_CHECK_ARG(mat_grid_holds(mats[i].rows, mats[i].cols), "cgan3d_orthogonalize: matrix too large for one launch");
   const Layout w = ortho_layout(mats, n);
   CG_CHECK_ARG(ws_bytes >= w.total && (w.total == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
                "cgan3d_orthogonalize: workspace of %lld bytes (16-byte aligned) needed, got %lld", w.total,
@@ -1141,6 +1148,10 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   e = ns_check(steps, coefficients, eps);
   CG_CHECK_ARG(!e, "cgan3d_muon_step: %s", e);
   CG_CHECK_ARG(param && grad && momentum && exp_avg_sq && hyper, "cgan3d_muon_step: null operand");
+  const bool planes = planes_hold(steps, coefficients);
+  for (int i = 0; i < n && !planes; ++i)
+    CG_CHECK_ARG(segs[i].rows == 0 || mat_grid_holds(segs[i].rows, segs[i].cols),
+                 "cgan3d_muon_step: matrix too large for one launch");
   const Layout w = muon_layout(segs, n);
   CG_CHECK_ARG(ws_bytes >= w.total && (w.total == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
                "cgan3d_muon_step: workspace of %lld bytes (16-byte aligned) needed, got %lld", w.total,
@@ -1149,7 +1160,6 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   char* base = static_cast<char*>(ws);
   float* u = reinterpret_cast<float*>(base + w.u);
   double* part = reinterpret_cast<double*>(base + w.part);
-  const bool planes = planes_hold(steps, coefficients);
   // segment i: a matrix of slab_kernel, another one, or a vector; vectors ride along with the first list of the
   // former as long as there is room
   const auto is_slab = [&](int i) { return planes && segs[i].rows > 0 && segs[i].cols > 0 && slab_takes(segs[i].rows, segs[i].cols); };

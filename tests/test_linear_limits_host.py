@@ -40,3 +40,16 @@ def test_what_no_grid_holds_is_refused(dt):
     assert bwd(8, LONG, 1 << 10, dt, dw=None) >= 0
     assert bwd((1 << 30) + 1, 8, 65, dt) == -1
     assert bwd((1 << 30) + 1, 8, 65, dt, dx=None, dw=None) >= 0  # column sums alone
+
+
+def test_coefficients_beside_very_long_matrices():
+    """Coefficients that take the f32 products: a matrix that their grid does not hold is refused, not left to HIP."""
+    from cgan3d_amd import _lib as L
+    lib, big = L.load(), 1 << 30
+    wild = (C.c_float * 3)(70.0, 0.0, -61.0)
+    m = (L.OrthoMat * 1)(L.OrthoMat(64, 64, big, big, 1, big))
+    assert lib.cgan3d_orthogonalize(m, 1, L.DT_F32, 5, wild, 1e-7, 256, 1 << 62, None) == 22
+    assert b"too large" in lib.cgan3d_get_last_error()
+    s = (L.MuonSeg * 1)(L.MuonSeg(0, big, 1, 1.0))
+    assert lib.cgan3d_muon_step(64, 64, 64, 64, s, 1, 64, 5, wild, 1e-7, 256, 1 << 62, None) == 22
+    assert b"too large" in lib.cgan3d_get_last_error()
