@@ -692,8 +692,9 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
       const double norm = sqrt(tr) + (double)eps, inv = 1. / (norm * norm);
 #pragma unroll
       for (int r = 0; r < 4; ++r) sum[r] = (float)(d[r] * inv);
-      // from G's planes to X's; a slab of zeros may have any factor but an infinite one
-      const float r0 = (float)fmin(ldexp(1.0, (int)m.expo[slab]) / norm * kXs, 1e38);
+      // from G's planes to X's; a slab of zeros may have any factor that stays finite times a coefficient (|a| < 68, or
+      // planes_hold refuses it)
+      const float r0 = (float)fmin(ldexp(1.0, (int)m.expo[slab]) / norm * kXs, 1e30);
       alpha *= r0;
       beta *= r0;
     } else {

@@ -1,0 +1,50 @@
+"""Newton-Schulz and Muon at the ends of the range: matrices far below eps, far above one, and the largest tiles.
+Tolerances of test_gpu_muon.py."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+NS = (3.4445, -4.7750, 2.0315)
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def ns64(g, steps=5, co=NS, eps=1e-7):
+    """(result, tolerance in the Frobenius norm) of one matrix in float64: see test_gpu_muon.py."""
+    x = g.double()
+    tall = x.shape[0] > x.shape[1]
+    if tall:
+        x = x.mT.contiguous()
+    x = x / (torch.linalg.vector_norm(x) + eps)
+    a, b, c = co
+    tol = 0.0
+    for _ in range(steps):
+        tol = abs(a) * (tol + 4 * U * float(x.norm()))
+        m = x @ x.mT
+        x = a * x + (b * m + c * m @ m) @ x
+    tol += 4 * U * float(x.norm())
+    return (x.mT if tall else x), tol
+
+
+def check_ns(got, g, dt, what, **kw):
+    want, tol = ns64(g, **kw)
+    got = got.double().to(want.device)
+    assert got.shape == want.shape and torch.isfinite(got).all(), what
+    tol += torch.finfo(DT[dt]).eps / 2 * float(want.norm()) + (2.0 ** -25 * math.sqrt(want.numel()) if dt == "f16" else 0)
+    err = float((got - want).norm())
+    assert err <= tol, f"{what}: off by {err:.3e}, bound {tol:.3e}, norm {float(want.norm()):.3e}"
+
+
+@pytest.mark.parametrize("shape", [(40, 600), (600, 40), (100, 600)])
+def test_zeros_beside_the_smallest_values(shape):
+    """A stretch of zeros along the long side of a matrix of f32's smallest values, without an eps: zeros stay zeros."""
+    from cgan3d_amd import ops
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(5)) * 1e-37
+    long = g if shape[1] > shape[0] else g.T
+    long[:, 256:512] = 0
+    got = ops.orthogonalize(g.cuda(), eps=0.0)
+    check_ns(got, g, "f32", f"{shape}", eps=0.0)
+    assert not (got if shape[1] > shape[0] else got.T)[:, 256:512].any()
