@@ -129,14 +129,14 @@ template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(MatList l, float eps) {
   const Mat& m = l.m[blockIdx.y];
   const double s = block_sum_d(m.part[threadIdx.x]);  // one partial sum a thread
-  const float norm = (float)(sqrt(s) + (double)eps);
+  const double inv = 1. / (sqrt(s) + (double)eps);  // the norm of finite values may be beyond f32
   const T* g = static_cast<const T*>(m.g);
   const bool tall = m.rows > m.cols;
   const int lng = tall ? m.rows : m.cols;
   const long long total = (long long)m.rows * m.cols;
   for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256LL) {
     const long long i = q / lng, t = q - i * lng;
-    m.x[q] = to_f(tall ? g[t * m.ldg + i] : g[i * m.ldg + t]) / norm;
+    m.x[q] = (float)(to_f(tall ? g[t * m.ldg + i] : g[i * m.ldg + t]) * inv);
   }
 }
 
@@ -346,7 +346,9 @@ __global__ __launch_bounds__(256) void planes_kernel(MatList l, PlaneMats pm, fl
   const Mat& m = l.m[blockIdx.y];
   const PlaneMat& p = pm.p[blockIdx.y];
   const double s = block_sum_d(m.part[threadIdx.x]);  // one partial sum a thread
-  const float norm = (float)(sqrt(s) + (double)eps);
+  // from G to the planes, the rest of a power of two apart: either may be beyond f32 where G is
+  int to;
+  const float rest = (float)frexp(kXs / (sqrt(s) + (double)eps), &to);
   const T* g = static_cast<const T*>(m.g);
   const bool tall = m.rows > m.cols;
   const long long xp = (long long)p.s * p.ldx, ap = (long long)p.s * p.lda;
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(256) void planes_kernel(MatList l, PlaneMats pm, fl
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         f16_t v[2];
-        split2(x[r] / norm * kXs, v);
+        split2(ldexpf(x[r], to) * rest, v);
         h[r] = v[0];
         lo[r] = v[1];
       }

@@ -536,7 +536,11 @@ __device__ __forceinline__ void split3(float x, bf16_t* o) {
   o[1] = m;
   o[2] = (bf16_t)(r - (float)m);
 }
+// Two f16.  x is one value from here on: where it is a product or a sum, the compiler else rounds it to f16 once straight
+// from its operands (v_fma_mix) and once by way of f32, and the two planes belong to unlike first planes wherever
+// the roundings differ (one in 2^13, by 2^-11: ten times the error of a whole iteration).
 __device__ __forceinline__ void split2(float x, f16_t* o) {
+  asm("" : "+v"(x));
   o[0] = (f16_t)x;
   o[1] = (f16_t)(x - (float)o[0]);
 }

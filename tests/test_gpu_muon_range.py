@@ -48,3 +48,19 @@ def test_zeros_beside_the_smallest_values(shape):
     got = ops.orthogonalize(g.cuda(), eps=0.0)
     check_ns(got, g, "f32", f"{shape}", eps=0.0)
     assert not (got if shape[1] > shape[0] else got.T)[:, 256:512].any()
+
+
+SLABS_AND_PLANES = [(40, 600), (50, 30), (64, 20000), (100, 300), (333, 97)]
+
+
+SLABS_AND_PLANES = [(40, 600), (50, 30), (64, 20000), (100, 300), (333, 97)]
+
+
+@pytest.mark.parametrize("steps", [0, 5])
+@pytest.mark.parametrize("shape", SLABS_AND_PLANES)
+def test_finite_matrices_whose_norm_is_beyond_f32(shape, steps):
+    from cgan3d_amd import ops
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(9))
+    g = g * (3e38 / float(g.abs().max()))
+    assert torch.isfinite(g).all() and float(g.double().norm()) > torch.finfo(torch.float32).max
+    check_ns(ops.orthogonalize(g.cuda(), steps=steps), g, "f32", f"{shape}", steps=steps)
