@@ -163,7 +163,7 @@ template <typename T, bool NANFIX> struct LinEpi {
   // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store, so that they are in
   // flight together
   template <int STEP>
-  __device__ __forceinline__ void put4(int i, int j, f32x4_m* v, int I, int jn) const {
+  __device__ __forceinline__ void put4(int i, int j, f32x4_m* v, int I, int jn, int) const {
     if constexpr (NANFIX) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -174,12 +174,13 @@ template <typename T, bool NANFIX> struct LinEpi {
     if (jn >= 4) put4_as<STEP, true>(i, j, v, I, 4);
     else put4_as<STEP, false>(i, j, v, I, jn);
   }
+  __device__ __forceinline__ int begin() const { return 0; }
   __device__ __forceinline__ bool turned() const { return false; }
   __device__ __forceinline__ void put_turned(int, int, f32x4_m, int) const {}
   // the joined sums, a row at a time
-  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool, int) const {
     f32x4_m w[4] = {v};
-    put4<1>(i, j, w, i + 1, jn);
+    put4<1>(i, j, w, i + 1, jn, 0);
   }
 };
 

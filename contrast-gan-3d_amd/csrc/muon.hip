@@ -14,6 +14,9 @@
 // accuracy on two f16 planes per matrix (planes.h): the iterates are bounded (|X| <= 1.2, |A| <= 1.5 with the
 // coefficients above), so a fixed power of two keeps hi + lo within f16's range: X at 2^12 (an entry of a
 // large orthogonal matrix, ~2^-6, and one of a fresh gradient's, ~2^-12, both keep 22 bits), A and B at 2^10.
+// A matrix far below eps starts at |X| = |G| / eps << 1 and grows by at most a factor per step that planes_hold finds
+// (a = 3.4445 here): its planes are held at a further 2^e, e from the norm and smaller by that factor's exponent with
+// every step, which the epilogues take back (A and B are needed to 2^-34 beside a alone, so theirs need none).
 // The first term a X is added in the epilogue from X's own planes: as part of B it would lose the
 // products of the low planes, which directions that start near zero then carry a^5 = 485 times larger.
 // Coefficients that let the iterates leave that range, and no steps at all, take the f32 products of mat.h.
@@ -125,6 +128,12 @@ __global__ __launch_bounds__(256) void muon_moment_kernel(SegList l, float* __re
   if (threadIdx.x == 0) part[(long long)l.mat[blockIdx.y] * kNormBlocks + blockIdx.x] = s;
 }
 
+// The exponent e of the planes' further factor: x = |G| / (|G| + eps) in [1/2, 1) as they hold it, 0 where it is larger
+// or no number
+__device__ __forceinline__ int start_exponent(double x) {
+  return x > 0. && x < 0.5 ? -ilogb(x) - 1 : 0;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(MatList l, float eps) {
   const Mat& m = l.m[blockIdx.y];
@@ -178,9 +187,13 @@ struct GramEpi {
   int ld, n;        // row stride, side
   long long plane;  // elements between planes
   float alpha, beta;
+  const int* expo;  // A: X's start exponent (B: null)
+  int drop;         // by how much it has fallen
+  __device__ __forceinline__ int begin() const { return expo ? *expo : 0; }
   // called by whole waves: lane l has row l % 16 and columns 4 (l / 16) .. + 3 of a 16 x 16 block
-  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool mirror) const {
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool mirror, int start) const {
     const long long o = (long long)i * ld + j;
+    const float alpha = ldexpf(this->alpha, -2 * max(start - drop, 0));
     const int lane = threadIdx.x & 63, t = lane & 3;
     if (jn >= 4) {
       f16x4_m h, l;
@@ -263,7 +276,10 @@ struct StepEpi {
   int tall;
   float scale;
   const float* hyper;
+  const int* expo;  // X's start exponent
+  int drop, next;   // by how much it has fallen, and will have in the result
 
+  __device__ __forceinline__ int begin() const { return *expo; }
   __device__ __forceinline__ bool turned() const { return tall && mode; }
 
   // the last step's values x at offset d of the result or the parameter, n of them
@@ -288,7 +304,8 @@ struct StepEpi {
     }
   }
   // four columns from j of rows i, i + STEP, .. + 3 STEP: every load before the first store
-  template <int STEP> __device__ __forceinline__ void put4(int i, int j, f32x4_m* v, int I, int jn) const {
+  template <int STEP> __device__ __forceinline__ void put4(int i, int j, f32x4_m* v, int I, int jn, int start) const {
+    const int ex = max(start - next, 0) - max(start - drop, 0);
     f16x4_m a[4], c[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -299,7 +316,7 @@ struct StepEpi {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[u][r] = alpha * v[u][r] + beta * ((float)a[u][r] + (float)c[u][r]);
+      for (int r = 0; r < 4; ++r) v[u][r] = ldexpf(alpha * v[u][r] + beta * ((float)a[u][r] + (float)c[u][r]), ex);
       if (i + u * STEP >= I || turned()) continue;
       if (mode == 0) {
         f16x4_m h, l;
@@ -320,9 +337,9 @@ struct StepEpi {
   }
   // column j of the result, rows i .. i + 3 of the iterate
   __device__ __forceinline__ void put_turned(int i, int j, f32x4_m v, int in_) const { finish(j * ldr + i, v, in_); }
-  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool) const {
+  __device__ __forceinline__ void put(int i, int j, f32x4_m v, int jn, bool, int start) const {
     f32x4_m w[4] = {v};
-    put4<1>(i, j, w, i + 1, jn);
+    put4<1>(i, j, w, i + 1, jn, start);
     if (turned())
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -332,6 +349,7 @@ struct StepEpi {
 
 struct PlaneMat {  // one matrix's planes in the workspace
   f16_t *x, *y, *a, *b;
+  int* expo;  // start exponent
   int s, l, lda, ldx;  // short and long side, row strides of A / B and X / Y (multiples of 32)
 };
 struct PlaneMats {
@@ -346,9 +364,13 @@ __global__ __launch_bounds__(256) void planes_kernel(MatList l, PlaneMats pm, fl
   const Mat& m = l.m[blockIdx.y];
   const PlaneMat& p = pm.p[blockIdx.y];
   const double s = block_sum_d(m.part[threadIdx.x]);  // one partial sum a thread
+  const double size = sqrt(s), inv = 1. / (size + (double)eps);
+  const int e = start_exponent(size * inv);
   // from G to the planes, the rest of a power of two apart: either may be beyond f32 where G is
   int to;
-  const float rest = (float)frexp(kXs / (sqrt(s) + (double)eps), &to);
+  const float rest = (float)frexp(kXs * inv, &to);
+  to += e;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.expo = e;
   const T* g = static_cast<const T*>(m.g);
   const bool tall = m.rows > m.cols;
   const long long xp = (long long)p.s * p.ldx, ap = (long long)p.s * p.lda;
@@ -406,12 +428,13 @@ struct PlaneLayout {
 PlaneLayout plane_layout(const int (*sl)[2], int n, char* ws, PlaneMat* out) {
   PlaneLayout w;
   PlaneShape gram[kJobs], poly[kJobs], step[kJobs];
+  w.bytes = up256(kJobs * 4);
   for (int i = 0; i < n; ++i) {
     const int s = sl[i][0], l = sl[i][1], ldx = up32(l), lda = up32(s);
     const long long xb = up256((long long)s * ldx * 4), ab = up256((long long)s * lda * 4);
     if (out) {
       f16_t* at = reinterpret_cast<f16_t*>(ws + w.bytes);
-      out[i] = {at, at + xb / 2, at + xb, at + xb + ab / 2, s, l, lda, ldx};
+      out[i] = {at, at + xb / 2, at + xb, at + xb + ab / 2, reinterpret_cast<int*>(ws) + i, s, l, lda, ldx};
     }
     w.bytes += 2 * xb + 2 * ab;
     gram[i] = {s, s, ldx};
@@ -427,8 +450,8 @@ PlaneLayout plane_layout(const int (*sl)[2], int n, char* ws, PlaneMat* out) {
 
 // `steps` >= 1 iterations on the matrices of l; the last one writes the results (dt) or the parameters (hyper)
 template <typename T>
-void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co, float eps, int dt, const float* hyper,
-                   hipStream_t st) {
+void plane_iterate(const MatList& l, int n, char* ws, int steps, int shift, const float* co, float eps, int dt,
+                   const float* hyper, hipStream_t st) {
   PlaneMats pm;
   int sl[kJobs][2];
   long long most = 1;
@@ -451,19 +474,23 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, const float* co
     step[i] = {p.s, p.l, p.lda};
     const long long xp = (long long)p.s * p.ldx, ap = (long long)p.s * p.lda;
     jg.j[i] = {{p.x, p.ldx, xp}, {p.x, p.ldx, xp}, p.s, p.s, p.ldx, 0, 0, 0, 0, nullptr,
-               {p.a, nullptr, p.lda, p.s, ap, kAs / (kXs * kXs), 0.f}};
+               {p.a, nullptr, p.lda, p.s, ap, kAs / (kXs * kXs), 0.f, p.expo, 0}};
     jp.j[i] = {{p.a, p.lda, ap}, {p.a, p.lda, ap}, p.s, p.s, p.lda, 0, 0, 0, 0, nullptr,
-               {p.b, p.a, p.lda, p.s, ap, co[2] / kAs, co[1]}};
+               {p.b, p.a, p.lda, p.s, ap, co[2] / kAs, co[1], nullptr, 0}};
     js.j[i] = {{p.b, p.lda, ap}, {p.x, p.ldx, xp}, p.s, p.l, p.s, 0, 0, 0, 0, nullptr,
                {p.y, p.x, xp, p.ldx, 0, 1.f / kAs, co[0], l.m[i].out, l.m[i].ldo, l.m[i].rows > l.m[i].cols,
-                l.m[i].scale, hyper}};
+                l.m[i].scale, hyper, p.expo, 0, 0}};
   }
   const PlanePick pg = plane_pick<2, true>(gram, n), pp = plane_pick<2, true>(poly, n), ps = plane_pick<2, false>(step, n);
   for (int k = 0; k < steps; ++k) {
+    const bool last = k == steps - 1;
+    for (int i = 0; i < n; ++i) {
+      jg.j[i].e.drop = js.j[i].e.drop = k * shift;
+      js.j[i].e.next = last ? INT_MAX : (k + 1) * shift;  // the result itself: no factor
+      if (last) js.j[i].e.mode = hyper ? 4 : 1 + dt;
+    }
     plane_run<f16_t, 2, false, false, true>(jg, pg, part, st);
     plane_run<f16_t, 2, false, false, true>(jp, pp, part, st);
-    if (k == steps - 1)
-      for (int i = 0; i < n; ++i) js.j[i].e.mode = hyper ? 4 : 1 + dt;
     plane_run<f16_t, 2, false, true, false>(js, ps, part, st);
     for (int i = 0; i < n; ++i) {  // X and Y change places
       const f16_t* x = js.j[i].e.out;
@@ -506,7 +533,7 @@ struct SlabMat {
   long long count;
   f16_t* x;         // planes, [slab][2][64][kCols], LDS order
   float* part;      // [2][nslab][64 * 64]
-  float* expo;      // [nslab]: G = planes * 2^expo
+  float* expo;      // [nslab]: G = planes * 2^expo; [nslab] X's start exponent, a copy for each block
 };
 struct SlabList {
   int n, tick;  // tick: the last launch advances the step counter
@@ -546,8 +573,8 @@ __device__ __forceinline__ int slab_t(bool tall, int u, int tid) {
 }
 // PHASE 0: launch 0, 1: a step that is not the last, 2: the last
 template <typename T, int PHASE>
-__global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, float ca, float cb, float cc, float eps,
-                                                   float* __restrict__ hyper) {
+__global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, int shift, float ca, float cb, float cc,
+                                                            float eps, float* __restrict__ hyper) {
   __shared__ __align__(16) f16_t X[2 * kSlab];  // a wave's columns are its own: the step's result replaces them
   __shared__ __align__(16) f16_t A[2 * 64 * 64];
   __shared__ __align__(16) f16_t B[2 * 64 * 64];
@@ -662,6 +689,8 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
     const bool some = ri < s && rj < s;
     f32x4_m sum = {};
     float alpha = 1.f / kAs, beta = ca;
+    int ex;  // of the result beside alpha and beta
+    const int start = k > 1 ? (int)m.expo[m.nslab + slab] : 0;
     const auto slabs = [&](auto f) {
       for (int z0 = 0; z0 < m.nslab; z0 += kBatch) {
         f32x4_m p[kBatch];
@@ -691,17 +720,22 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
       tr = 0.;
 #pragma unroll
       for (int w = 0; w < kSlabWaves; ++w) tr += redd[w];
-      const double norm = sqrt(tr) + (double)eps, inv = 1. / (norm * norm);
+      const double size = sqrt(tr), inv = 1. / (size + (double)eps);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum[r] = (float)(d[r] * inv);
-      // from G's planes to X's; a slab of zeros may have any factor that stays finite times a coefficient (|a| < 68, or
-      // planes_hold refuses it)
-      const float r0 = (float)fmin(ldexp(1.0, (int)m.expo[slab]) / norm * kXs, 1e30);
+      for (int r = 0; r < 4; ++r) sum[r] = (float)(d[r] * inv * inv);
+      const int e = start_exponent(size * inv);
+      if (tid == 0) m.expo[m.nslab + slab] = (float)e;
+      // from G's planes to X's, exponent and the rest apart (a slab of zeros may have any)
+      const float r0 = (float)frexp(kXs * inv, &ex);
+      ex += (int)m.expo[slab] + (PHASE == 2 ? 0 : max(e - shift, 0));
       alpha *= r0;
       beta *= r0;
     } else {
       slabs([&](int, const f32x4_m& p) { sum += p; });
-      sum *= 1.f / (kXs * kXs);
+      const int in = max(start - (k - 1) * shift, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[r] = ldexpf(sum[r] * (1.f / (kXs * kXs)), -2 * in);
+      ex = (PHASE == 2 ? 0 : max(start - k * shift, 0)) - in;
     }
     {
       f16x4_m hi, lo;
@@ -772,7 +806,7 @@ __global__ __launch_bounds__(kSlabThreads) void slab_kernel(SlabList l, int k, f
         const f16x4_m h = *reinterpret_cast<const f16x4_m*>(X + o), lw = *reinterpret_cast<const f16x4_m*>(X + kSlab + o);
         f32x4_m x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = alpha * acc[q][r] + beta * ((float)h[r] + (float)lw[r]);
+        for (int r = 0; r < 4; ++r) x[r] = ldexpf(alpha * acc[q][r] + beta * ((float)h[r] + (float)lw[r]), ex);
         if constexpr (PHASE == 1) {
           f16x4_m oh, ol;
 #pragma unroll
@@ -862,37 +896,40 @@ long long slab_place(SlabMat& m, char* ws) {
   m.x = reinterpret_cast<f16_t*>(ws);
   m.part = reinterpret_cast<float*>(ws + xb);
   m.expo = reinterpret_cast<float*>(ws + xb + pb);
-  return xb + pb + up256(m.nslab * 4);
+  return xb + pb + up256(2 * m.nslab * 4);
 }
 
-// five launches and one per step; `hyper`: the Muon step of the list (f32)
+// one launch and one per step; `hyper`: the Muon step of the list (f32)
 template <typename T>
-void slab_run(SlabList& l, int steps, const float* co, float eps, float* hyper, hipStream_t st) {
+void slab_run(SlabList& l, int steps, int shift, const float* co, float eps, float* hyper, hipStream_t st) {
   int at = 0;
   for (int i = 0; i < l.n; ++i) {
     l.start[i] = at;
     at += l.m[i].nslab;
   }
-  launch(slab_kernel<T, 0>, dim3(at), dim3(kSlabThreads), 0, st, l, 0, co[0], co[1], co[2], eps, hyper);
+  launch(slab_kernel<T, 0>, dim3(at), dim3(kSlabThreads), 0, st, l, 0, shift, co[0], co[1], co[2], eps, hyper);
   for (int k = 1; k < steps; ++k)
-    launch(slab_kernel<T, 1>, dim3(at), dim3(kSlabThreads), 0, st, l, k, co[0], co[1], co[2], eps, hyper);
-  launch(slab_kernel<T, 2>, dim3(at), dim3(kSlabThreads), 0, st, l, steps, co[0], co[1], co[2], eps, hyper);
+    launch(slab_kernel<T, 1>, dim3(at), dim3(kSlabThreads), 0, st, l, k, shift, co[0], co[1], co[2], eps, hyper);
+  launch(slab_kernel<T, 2>, dim3(at), dim3(kSlabThreads), 0, st, l, steps, shift, co[0], co[1], co[2], eps, hyper);
 }
 
 // Whether iterates that start within |X| <= 1 stay where the planes hold them: |X| < 2^16 / kXs, |A| and |B|
-// (largest entry <= largest singular value) < 2^16 / kAs
-bool planes_hold(int steps, const float* co) {
+// (largest entry <= largest singular value) < 2^16 / kAs.  *shift: a step makes no singular value larger by more than
+// 2^shift
+bool planes_hold(int steps, const float* co, int* shift) {
   if (steps < 1) return false;
-  double r = 1.0;
+  double r = 1.0, gain = std::fabs(co[0]);
   for (int k = 0; k < steps; ++k) {
     if (r > 7.5 || std::fabs(co[1]) * r * r + std::fabs(co[2]) * r * r * r * r > 60.) return false;
     double next = 0;
     for (int q = 1; q <= 4096; ++q) {
-      const double x = r * q / 4096, x2 = x * x;
-      next = std::max(next, std::fabs(x * (co[0] + x2 * (co[1] + x2 * co[2]))));
+      const double x = r * q / 4096, x2 = x * x, g = std::fabs(co[0] + x2 * (co[1] + x2 * co[2]));
+      gain = std::max(gain, g);
+      next = std::max(next, x * g);
     }
     r = next * 1.01;
   }
+  *shift = std::max(0, std::ilogb(gain * 1.01) + 1);
   return r <= 7.5;
 }
 
@@ -1025,7 +1062,8 @@ Layout ortho_layout(const cgan3d_ortho_mat* m, int n) {
 template <typename T>
 void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, char* ws, int steps, const float* co,
                float eps, hipStream_t st) {
-  const bool planes = planes_hold(steps, co);
+  int shift = 0;
+  const bool planes = planes_hold(steps, co, &shift);
   if (planes) {
     SlabList sl = {};
     long long used = 0;
@@ -1038,7 +1076,7 @@ void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, cha
         used += slab_place(m, ws + w.x + used);
       }
       if (sl.n == kSlabMats || (i == n - 1 && sl.n > 0)) {
-        slab_run<T>(sl, steps, co, eps, nullptr, st);
+        slab_run<T>(sl, steps, shift, co, eps, nullptr, st);
         sl.n = 0;
         used = 0;
       }
@@ -1050,7 +1088,7 @@ void ortho_run(const cgan3d_ortho_mat* mats, int n, int dt, const Layout& w, cha
     if (!at) return;
     launch(norm_kernel<T>, dim3(kNormBlocks, at), dim3(256), 0, st, l);
     if (planes) {
-      plane_iterate<T>(l, at, ws + w.x, steps, co, eps, dt, nullptr, st);
+      plane_iterate<T>(l, at, ws + w.x, steps, shift, co, eps, dt, nullptr, st);
     } else {
       const unsigned blocks = (unsigned)std::min(((long long)l.m[0].rows * l.m[0].cols + 1023) / 1024, 4096LL);
       launch(scale_kernel<T>, dim3(blocks, 1), dim3(256), 0, st, l, eps);
@@ -1116,7 +1154,8 @@ extern "C" int cgan3d_orthogonalize(const cgan3d_ortho_mat* mats, int32_t n, int
   CG_CHECK_ARG(!e, "cgan3d_orthogonalize: %s", e);
   e = ns_check(steps, coefficients, eps);
   CG_CHECK_ARG(!e, "cgan3d_orthogonalize: %s", e);
-  if (!planes_hold(steps, coefficients))
+  int shift = 0;
+  if (!planes_hold(steps, coefficients, &shift))
     for (int i = 0; i < n; ++i)
       CG_CHECK_ARG(mat_grid_holds(mats[i].rows, mats[i].cols), "cgan3d_orthogonalize: matrix too large for one launch");
   const Layout w = ortho_layout(mats, n);
@@ -1151,7 +1190,8 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   e = ns_check(steps, coefficients, eps);
   CG_CHECK_ARG(!e, "cgan3d_muon_step: %s", e);
   CG_CHECK_ARG(param && grad && momentum && exp_avg_sq && hyper, "cgan3d_muon_step: null operand");
-  const bool planes = planes_hold(steps, coefficients);
+  int shift = 0;
+  const bool planes = planes_hold(steps, coefficients, &shift);
   for (int i = 0; i < n && !planes; ++i)
     CG_CHECK_ARG(segs[i].rows == 0 || mat_grid_holds(segs[i].rows, segs[i].cols),
                  "cgan3d_muon_step: matrix too large for one launch");
@@ -1204,7 +1244,7 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
   const auto run = [&]() {
     if (!qn) return;
     if (planes) {
-      plane_iterate<float>(q, qn, base + w.x, steps, coefficients, eps, 0, hyper, st);
+      plane_iterate<float>(q, qn, base + w.x, steps, shift, coefficients, eps, 0, hyper, st);
     } else {
       const unsigned blocks = (unsigned)std::min(((long long)q.m[0].rows * q.m[0].cols + 1023) / 1024, 4096LL);
       launch(scale_kernel<float>, dim3(blocks, 1), dim3(256), 0, st, q, eps);
@@ -1248,7 +1288,7 @@ extern "C" int cgan3d_muon_step(float* param, const float* grad, float* momentum
     }
     ride = 0;
     sl.tick = left == 0;
-    slab_run<float>(sl, steps, coefficients, eps, hyper, st);
+    slab_run<float>(sl, steps, shift, coefficients, eps, hyper, st);
     sl.n = 0;
     used = 0;
   }

@@ -184,6 +184,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
   const int i0 = ti * BM, j0 = tj * BN;
   const int k0 = split * p.kchunk, k1 = min(p.K, k0 + p.kchunk), steps = (k1 - k0 + BK - 1) / BK;
   const int wi = (wave / WJ) * WM, wj = (wave % WJ) * WN;
+  const int own = p.e.begin();  // the epilogue's scalar, on its way under the products
 
   TA ta;
   TB tb;
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
           f32x4_m v[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f32x4_m*>(my + (r + u * (64 / LPR)) * LD + lane % LPR * 4);
-          p.e.template put4<64 / LPR>(i0 + wi + mb * 16 + r, j, v, p.I, p.J - j);
+          p.e.template put4<64 / LPR>(i0 + wi + mb * 16 + r, j, v, p.I, p.J - j, own);
           if (p.e.turned()) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) *reinterpret_cast<f32x4_m*>(my + (r + u * (64 / LPR)) * LD + lane % LPR * 4) = v[u];
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void plane_kernel(PlaneJobs<E, N> job
 #pragma unroll
         for (int n = 0; n < FN; ++n) {
           const int j = j0 + wj + n * 16 + (lane >> 4) * 4;
-          if (j < p.J) p.e.put(i, j, acc[m][n], p.J - j, SYM && ti != tj);
+          if (j < p.J) p.e.put(i, j, acc[m][n], p.J - j, SYM && ti != tj, own);
         }
       }
     }
@@ -392,6 +393,7 @@ __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
   const PlaneJob<E>& p = jobs.j[jn];
   b -= jobs.start[jn];
   if (!p.part) return;
+  const int own = p.e.begin();
   const int t = b / SUB, sub = b - t * SUB;
   int ti, tj;
   plane_tile<BM, SYM>(t, p.I, p.tj, ti, tj);
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(256) void plane_join_kernel(PlaneJobs<E, N> jobs) {
     f32x4_m v = *reinterpret_cast<const f32x4_m*>(s);
 #pragma unroll 8
     for (int z = 1; z < p.splits; ++z) v += *reinterpret_cast<const f32x4_m*>(s + (long long)z * p.tiles * (BM * BN));
-    p.e.put(i, j, v, p.J - j, SYM && ti != tj);
+    p.e.put(i, j, v, p.J - j, SYM && ti != tj, own);
   }
 }
 

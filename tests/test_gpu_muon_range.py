@@ -53,7 +53,33 @@ def test_zeros_beside_the_smallest_values(shape):
 SLABS_AND_PLANES = [(40, 600), (50, 30), (64, 20000), (100, 300), (333, 97)]
 
 
-SLABS_AND_PLANES = [(40, 600), (50, 30), (64, 20000), (100, 300), (333, 97)]
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e-5, 1e-8, 1e-11, 1e-13, 1e-16, 1e-24, 1e-36])
+@pytest.mark.parametrize("shape", SLABS_AND_PLANES)
+def test_matrices_far_below_eps(shape, size, dt):
+    """|G| << eps: the iterates start near |G| / eps and grow by 3.4445 a step; every one of them keeps f32's accuracy
+    relative to itself."""
+    from cgan3d_amd import ops
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(7))
+    g = (g * (size / float(g.norm()))).to(DT[dt])
+    check_ns(ops.orthogonalize(g.cuda()), g, dt, f"{shape} of {size}")
+
+
+@pytest.mark.parametrize("shape", SLABS_AND_PLANES)
+def test_far_below_eps_with_other_steps(shape):
+    """One step, few, many; coefficients of another growth; and a list whose matrices differ by their sizes alone."""
+    from cgan3d_amd import ops
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(8)) * 1e-14
+    for steps in (1, 2, 3, 9):
+        check_ns(ops.orthogonalize(g.cuda(), steps=steps), g, "f32", f"{steps} steps", steps=steps)
+    co = (1.5, -0.5, 0.0)
+    for steps in (2, 20):
+        check_ns(ops.orthogonalize(g.cuda(), steps=steps, coefficients=co), g, "f32", f"cubic, {steps}", steps=steps, co=co)
+    many = torch.stack([g * s for s in (1.0, 1e14, 1e5, 0.0, 1e-9, 1e9)])
+    got = ops.orthogonalize(many.cuda())
+    for i in range(len(many)):
+        check_ns(got[i], many[i], "f32", f"matrix {i}")
+    assert torch.equal(got[1], ops.orthogonalize(many[1].cuda()))
 
 
 @pytest.mark.parametrize("steps", [0, 5])
@@ -64,3 +90,17 @@ def test_finite_matrices_whose_norm_is_beyond_f32(shape, steps):
     g = g * (3e38 / float(g.abs().max()))
     assert torch.isfinite(g).all() and float(g.double().norm()) > torch.finfo(torch.float32).max
     check_ns(ops.orthogonalize(g.cuda(), steps=steps), g, "f32", f"{shape}", steps=steps)
+
+
+@pytest.mark.parametrize("shape", SLABS_AND_PLANES)
+def test_muon_step_far_below_eps(shape):
+    """The parameter's change under a gradient of 1e-13 from a parameter of zeros."""
+    from cgan3d_amd import ops
+    n = shape[0] * shape[1]
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(10)) * (1e-13 / math.sqrt(n))
+    segs = ops.MuonSegments(n, [(0, *shape, 1.0)], [])
+    p, m, v = (torch.zeros(n, device="cuda") for _ in range(3))
+    hyper = torch.tensor([0.5, 0.75, 0.0, 0.0, 0.0, 0.0, 0.0, 0.9, 0.999, 1e-8], device="cuda")
+    ops.muon_step(p, g.reshape(-1).cuda(), m, v, segs, hyper)
+    assert torch.equal(m.cpu(), 0.25 * g.reshape(-1))  # exact: powers of two
+    check_ns(p.view(shape) * -2.0, 0.25 * g, "f32", f"{shape}")
