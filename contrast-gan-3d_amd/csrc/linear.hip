@@ -10,7 +10,8 @@
 // Which kernel a product takes (mat_route):
 //   rows <= 2, forward      gemv_kernel: a wave per pair of output columns streams the weight once
 //   rows <= 16, forward     skinny_kernel: a wave per 16 columns, the weight straight into matrix instructions
-//   k, n <= 64              rows_fwd_kernel, rows_bwd_kernel: every row's values are read and written once
+//   k, n <= 64              rows_fwd_kernel, rows_bwd_kernel: every row's values are read and written once (16-bit ones
+//                           with few rows: rows_fwd_takes, rows_bwd_takes)
 //   16-bit tensors         plane_kernel (planes.h) on the tensors themselves; an operand whose rows are not
 //                          whole aligned 16-byte chunks is copied once into rows that are
 //   f32 tensors            plane_kernel on three bf16 planes where the product is large enough to pay for
@@ -256,17 +257,34 @@ struct Operand {
 
 enum Route { ROUTE_MAT, ROUTE_PLANES };
 
-// Whether an f32 product is better off on planes: six 16-bit products at ~200 TFLOP/s behind the splitting of both operands
-// (`ready`: of b, a's planes are there), against f32 instructions at ~95.  Measured, us, f32 instructions / planes:
-// rows x k -> n 2048 x 512 -> 1024 31 / 40, 8192 x 256 -> 256 19 / 31, 1024 x 1024 -> 1024 35 / 34, 512 x 2048 -> 2048
-// 60 / 54, 2048 x 1024 -> 4096 184 / 103; both gradients of 512 x 512 -> 512 40 / 49, of 1024 x 1024 -> 1024 85 / 70.
-bool f32_planes(long long I, long long J, long long K, bool ready) {
-  const double fl = 2.0 * I * J * K, pack = 10.0 * K * (ready ? J : I + J);
-  return fl / 95e12 > fl / 200e12 + pack / 4e12 + (ready ? 5e-6 : 9e-6);
+// What an f32 product is expected to take.  On f32 instructions: the rounds of tiles that the fullest CU gets, at 100
+// TFLOP/s of the card, a tenth more where an operand is turned on its way to LDS, and each round's start; the output;
+// the launch, and the join of split sums.  On planes: plane_pick's own estimate, the splitting, the output and three launches.
+// Measured, us, f32 instructions / planes, what is taken in brackets.  Forward: rows x k -> n 2048 x 512 -> 1024 29.6 / 40.5
+// (f), 1500 x 1000 -> 1203 51 / 56 (f), 8191 x 65 -> 4099 109 / 133 (f), 2048 x 1024 -> 2048 96 / 68 (p), 2500 x 777 -> 1111
+// 58 / 56 (f); dx and dw: 1300 x 700 -> 900 37 / 33 (p) and 38 / 46 (f), 6001 x 203 -> 2999 205 / 105 (p) and 273 / 104 (p),
+// 4096 x 256 -> 1024 41 / 35 (f) and 40 / 39 (f).  Over 30 sizes the slower form costs 0.6 % on average, 16 % once.
+double mat_seconds(const Operand& a, const Operand& b, long long I, long long J, long long K) {
+  const int splits = mat_splits(I, J, K), cus = cu_count();
+  const double tiles = (double)((I + kTile - 1) / kTile) * ((J + kTile - 1) / kTile) * splits;
+  const double len = std::ceil(std::ceil(K / 32.) / splits) * 32;
+  const double tile = 2. * kTile * kTile * len / (100e12 / cus) * (b.strided ? 1.1 : 1.) + (a.strided ? 1.5e-6 : b.strided ? 8e-7 : 0);
+  return std::ceil(tiles / cus) * tile + 4. * I * J / 2.7e12 + 4e-6 + (splits > 1 ? 9e-6 : 0);
 }
-Route mat_route(int dt, long long I, long long J, long long K, bool ready) {
-  if (K == 0 || K >= 1 << 30 || I >= 1 << 30 || J >= 1 << 30) return ROUTE_MAT;
-  return dt != CGAN3D_DT_F32 || ready || f32_planes(I, J, K, false) ? ROUTE_PLANES : ROUTE_MAT;
+double planes_seconds(const Operand& a, const Operand& b, long long I, long long J, long long K) {
+  const PlaneShape s = {(int)I, (int)J, (int)K};
+  double values = 0;
+  for (const Operand* o : {&a, &b})
+    if (!o->planes) values += (double)o->rows * row_pad(o->cols);
+  return 0.7 * plane_pick<3, false>(&s, 1).seconds + values * 10 / 8e12 + 4. * I * J / 1.95e12 + 15e-6;
+}
+bool f32_planes(const Operand& a, const Operand& b, long long I, long long J, long long K) {
+  const double m = mat_seconds(a, b, I, J, K);
+  return m > 15e-6 && m > planes_seconds(a, b, I, J, K);
+}
+Route mat_route(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
+  if (K == 0 || K > 1 << 30 || I > 1 << 30 || J > 1 << 30) return ROUTE_MAT;
+  return dt != CGAN3D_DT_F32 || a.planes || f32_planes(a, b, I, J, K) ? ROUTE_PLANES : ROUTE_MAT;
 }
 
 long long operand_bytes(int dt, const Operand& o) {
@@ -285,20 +303,20 @@ template <int P> long long plane_threads(const PlanePick& p, const PlaneShape& s
   return plane_tiles(s, C::BM[p.cfg], C::BN[p.cfg], false) * std::max(1, (s.K + p.kchunk - 1) / p.kchunk) * C::WI[p.cfg] *
          C::WJ[p.cfg] * 64;
 }
-bool launchable(int dt, long long I, long long J, long long K, bool ready) {
+bool launchable(int dt, long long I, long long J, long long K) {
   const long long side = 1LL << 30, tiles = (I + kTile - 1) / kTile * ((J + kTile - 1) / kTile);
   if (I == 0 || J == 0) return true;
   if (I > side || J > side || K > side) return false;
   if (tiles < 1 << 22) return true;  // of the smallest tile; no block has more than 512 threads, splits come with few tiles
-  if (mat_route(dt, I, J, K, ready) == ROUTE_MAT) return tiles * 256 < 1LL << 32;
   const PlaneShape s = {(int)I, (int)J, (int)K};
   const PlanePick p = pick_for(dt, I, J, K);
-  return (dt == CGAN3D_DT_F32 ? plane_threads<3>(p, s) : plane_threads<1>(p, s)) < 1LL << 32;
+  if (dt != CGAN3D_DT_F32) return plane_threads<1>(p, s) < 1LL << 32;
+  return plane_threads<3>(p, s) < 1LL << 32 && tiles * 256 < 1LL << 32;
 }
 // workspace of one product: both operands' planes, then partial sums
 long long product_bytes(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
   if (I == 0 || J == 0) return 0;
-  if (mat_route(dt, I, J, K, a.planes) == ROUTE_MAT) return mat_ws_bytes(I, J, K);
+  if (mat_route(dt, a, b, I, J, K) == ROUTE_MAT) return mat_ws_bytes(I, J, K);
   return operand_bytes(dt, a) + operand_bytes(dt, b) + pick_for(dt, I, J, K).part_floats * 4;
 }
 
@@ -346,7 +364,7 @@ void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStr
 // C = A B^T with m's epilogue; m.a / m.b: the operands as the tensors they are
 void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void* ws, hipStream_t st) {
   if (m.I == 0 || m.J == 0) return;
-  if (mat_route(dt, m.I, m.J, m.K, a.planes) == ROUTE_MAT) {
+  if (mat_route(dt, a, b, m.I, m.J, m.K) == ROUTE_MAT) {
     if (a.strided) mat_run<true, true>(dt, m, ws, st);
     else if (b.strided) mat_run<false, true>(dt, m, ws, st);
     else mat_run<false, false>(dt, m, ws, st);
@@ -458,7 +476,8 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int n, T
 // No LDS but for the join: a value of the weight is used once.  The KW waves of a block share the summed axis, U steps
 // of 32 values each in flight; 16 waves where each has U steps to do, else 4.  Measured, us, KW = 4 / 16, 8 rows: bf16
 // 4096 -> 4096 11.1 / 9.5 (3.5 TB/s), 2048 -> 4096 6.3 / 8.4; f32 4096 -> 4096 18.9 / 16.7, 2048 -> 4096 11.4 / 9.7,
-// 1024 -> 8192 10.1 / 15.7.  As products of tiles (planes, mat_kernel) these five take 12.9, 9.8, 28, 17.5 and 18.5.
+// 1024 -> 8192 10.1 / 15.7.  With more than 32 columns a CU, four waves from ten rows on (f32 16 x 8192 -> 16384 126 / 133,
+// 10 x 110 / 118, 8 x 8192 -> 32768 231 / 219, 3 x 230 / 204).  As products of tiles (planes, mat_kernel) these five take 12.9, 9.8, 28, 17.5 and 18.5.
 // 16-bit weights with more columns than 32 a CU are the planes' (16 rows, 4096 -> 16384: 40 here, 33 there; 2048 ->
 // 16384: 22 and 18), f32 ones are not (68 and 96).
 constexpr int kSkinnyRows = 16;
@@ -512,7 +531,7 @@ template <typename T> void skinny_run(const MatArgs& p, hipStream_t st) {
   const T* w = static_cast<const T*>(p.b);
   const int n = (int)p.J, k = (int)p.K;
   const int blocks = (n + 15) / 16;
-  if (k >= 16 * 32 * kSkinnySteps<T>)
+  if (k >= 16 * 32 * kSkinnySteps<T> && (p.I < 10 || n <= 32 * cu_count()))
     launch(skinny_kernel<T, 16>, long_grid(blocks, 1024), dim3(1024), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
   else launch(skinny_kernel<T, 4>, long_grid(blocks, 256), dim3(256), 0, st, x, p.lda, w, p.ldb, (int)p.I, n, k, p.e);
 }
@@ -771,9 +790,26 @@ bool skinny_takes(const cgan3d_linear_args* a) {
   return a->rows <= kSkinnyRows && (a->dtype == CGAN3D_DT_F32 || a->n <= 32 * cu_count());
 }
 bool few_channels(long long n, long long k) { return n > 0 && k > 0 && n <= 64 && k <= 64; }
-// One pass against dz, two products and their joins, us, f32 and bf16 of 64 -> 64: 16 rows 16.5 / 16.2 and 14.0 / 12.3, 64
-// rows 17.8 / 19.2 and 14.8 / 12.8, 256 rows 17.8 / 27.7 and 14.9 / 14.2, 16384 rows 22.5 / 65 and 19.1 / 61.
-bool rows_bwd_takes(const cgan3d_linear_args* a) { return few_channels(a->n, a->k) && a->rows >= 64 && (a->dx || a->dw); }
+// rows_fwd_kernel against the products' own.  f32 always: 64 rows of 64 -> 64 6.4 / 7.0 us, 16384 7.2 / 7.8, 1048576 148 / 198.
+// 16-bit tensors lose with more than two column tiles until there are rows enough, unless the products have to copy
+// their operands first: bf16 64 -> 64 512 rows 4.7 / 4.0, 16384 5.0 / 4.3, 131072 15.3 / 12.3, 262144 21.3 / 22.5; 32 -> 64
+// 16384 4.9 / 4.3, 65536 6.4 / 7.6; 64 -> 32 4096 3.8 / 4.0; 60 -> 60 4096 5.7 / 6.5.
+bool rows_fwd_takes(const cgan3d_linear_args* a) {
+  if (!few_channels(a->n, a->k)) return false;
+  if (a->dtype == CGAN3D_DT_F32 || a->n <= 32 || !chunked(a->x, a->ldx, a->k) || !chunked(a->w, a->ldw, a->k)) return true;
+  return a->rows > (a->k > 48 ? 1 << 17 : 1 << 14);
+}
+// One pass against dz, two products and their joins.  Always, but for 16-bit tensors of whole chunks with more than two tiles
+// each way and an activation, whose few blocks take longer than the products until there are rows enough.  us, 8 / 256
+// rows with SiLU: f32 64 -> 64 16.5 / 17.1 and 16.0 / 26.8 (products), 16 -> 64 11.1 / 11.4 and 14.0 / 23.9; bf16 64 -> 64
+// 13.5 / 14.3 and 11.9 / 13.6 (512 rows: 14.3 and 15.3), 32 -> 32 9.1 / 9.3 and 12.0 / 13.6, 33 -> 50 12.7 / 14.2 and 15.7 /
+// 18.2; without an activation bf16 64 -> 64 11.0 / 11.7 and 11.0 / 12.5.
+bool rows_bwd_takes(const cgan3d_linear_args* a) {
+  if (!few_channels(a->n, a->k) || a->rows == 0 || !(a->dx || a->dw)) return false;
+  const bool quick = a->dtype != CGAN3D_DT_F32 && a->act != CGAN3D_ACT_NONE && a->n > 32 && a->k > 32 && a->n % 8 == 0 &&
+                     chunked(a->x, a->ldx, a->k) && chunked(a->w, a->ldw, a->k);
+  return !quick || a->rows >= 384;
+}
 int rows_blocks(const cgan3d_linear_args* a) { return (int)std::min<long long>((a->rows + 63) / 64, kRowsBlocks); }
 
 template <typename T, int NT> void rows_fwd_nt(const MatArgs& p, hipStream_t st) {
@@ -949,9 +985,12 @@ Bwd bwd_layout(const cgan3d_linear_args* a) {
     return w;
   }
   // dz goes to planes where both products are better off with them: they share the splitting
-  const long long big = 1LL << 30;
-  w.planes3 = dt == CGAN3D_DT_F32 && a->dx && a->dw && a->rows > 0 && a->rows < big && a->n > 0 && a->n < big && a->k > 0 &&
-              a->k < big && f32_planes(a->rows, a->k, a->n, true) && f32_planes(a->n, a->k, a->rows, true);
+  w.x = {a->x, a->ldx, a->rows, a->k, true, false};
+  w.w = {a->w, a->ldw, a->n, a->k, true, false};
+  if (dt == CGAN3D_DT_F32 && a->dx && a->dw && a->rows > 0 && a->n > 0 && a->k > 0) {
+    const Operand z = {nullptr, 0, a->rows, a->n, false, true}, zt = {nullptr, 0, a->rows, a->n, true, true};
+    w.planes3 = f32_planes(z, w.w, a->rows, a->k, a->n) && f32_planes(zt, w.x, a->n, a->k, a->rows);
+  }
   const bool direct = a->act == CGAN3D_ACT_NONE && !w.planes3 && (dt == CGAN3D_DT_F32 || chunked(a->dy, a->lddy, a->n));
   w.has_dz = !direct && (a->dx || a->dw);
   w.ldz = (int)row_pad(a->n);
@@ -964,8 +1003,6 @@ Bwd bwd_layout(const cgan3d_linear_args* a) {
   if (w.has_dz) w.za.ld = w.ldz;
   w.zb = w.za;
   w.zb.strided = true;
-  w.x = {a->x, a->ldx, a->rows, a->k, true, false};
-  w.w = {a->w, a->ldw, a->n, a->k, true, false};
   const long long m1 = a->dx ? product_bytes(dt, w.za, w.w, a->rows, a->k, a->n) : 0;
   const long long m2 = a->dw ? product_bytes(dt, w.zb, w.x, a->n, a->k, a->rows) : 0;
   w.total = at + std::max(m1, m2);  // the two products run one after the other
@@ -978,7 +1015,7 @@ void fwd_operands(const cgan3d_linear_args* a, Operand* x, Operand* w) {
   *w = {a->w, a->ldw, a->n, a->k, false, false};
 }
 long long fwd_bytes(const cgan3d_linear_args* a) {
-  if (a->rows <= kGemvRows || skinny_takes(a) || few_channels(a->n, a->k)) return 0;
+  if (a->rows <= kGemvRows || skinny_takes(a) || rows_fwd_takes(a)) return 0;
   Operand x, w;
   fwd_operands(a, &x, &w);
   return product_bytes(a->dtype, x, w, a->rows, a->n, a->k);
@@ -989,10 +1026,10 @@ const char* lin_check(const cgan3d_linear_args* a, bool bwd) {
   if (a->dtype < CGAN3D_DT_F32 || a->dtype > CGAN3D_DT_F16) return "unknown dtype";
   if (a->rows < 0 || a->k < 0 || a->n < 0) return "negative size";
   if (a->rows > (1LL << 40) || a->k > 1 << 30 || a->n > 1 << 30) return "size too large";
-  const bool fits = bwd ? rows_bwd_takes(a) || ((!a->dx || launchable(a->dtype, a->rows, a->k, a->n, false)) &&
-                                                (!a->dw || launchable(a->dtype, a->n, a->k, a->rows, false)))
-                        : a->rows <= kGemvRows || skinny_takes(a) || few_channels(a->n, a->k) ||
-                              launchable(a->dtype, a->rows, a->n, a->k, false);
+  const bool fits = bwd ? rows_bwd_takes(a) || ((!a->dx || launchable(a->dtype, a->rows, a->k, a->n)) &&
+                                                (!a->dw || launchable(a->dtype, a->n, a->k, a->rows)))
+                        : a->rows <= kGemvRows || skinny_takes(a) || rows_fwd_takes(a) ||
+                              launchable(a->dtype, a->rows, a->n, a->k);
   if (!fits) return "too many tiles for one launch";
   if (a->act < CGAN3D_ACT_NONE || a->act > CGAN3D_ACT_SILU || a->act == CGAN3D_ACT_NEG_DTANH)
     return "activation must be none, relu, lrelu, tanh, gelu or silu";
@@ -1069,7 +1106,7 @@ extern "C" int cgan3d_linear_fwd(const cgan3d_linear_args* a, void* ws, int64_t 
     if (a->dtype == CGAN3D_DT_F32) skinny_run<float>(p, st);
     else if (a->dtype == CGAN3D_DT_BF16) skinny_run<bf16_t>(p, st);
     else skinny_run<f16_t>(p, st);
-  } else if (few_channels(a->n, a->k)) {
+  } else if (rows_fwd_takes(a)) {
     if (a->dtype == CGAN3D_DT_F32) rows_fwd_run<float>(p, st);
     else if (a->dtype == CGAN3D_DT_BF16) rows_fwd_run<bf16_t>(p, st);
     else rows_fwd_run<f16_t>(p, st);

@@ -418,6 +418,7 @@ struct PlaneShape {
 struct PlanePick {
   int cfg = 0, kchunk = 0;
   long long part_floats = 0;
+  double seconds = 0;  // expected
 };
 // Tile configurations by planes: 0 the largest (8 waves, one block a CU), 1 and 2 smaller ones that give more
 // blocks where there are few.  RATE: a CU's share of the largest tile's.  Measured, us, tiles 0 / 1 / 2 without splits and
@@ -485,6 +486,7 @@ template <int P, bool sym> PlanePick plane_pick(const PlaneShape* s, int n) {
         best.cfg = c;
         best.kchunk = kc;
         best.part_floats = part;
+        best.seconds = t;
       }
       if (kc <= 128 || blocks >= 2 * cus) break;
     }
