@@ -4,7 +4,8 @@
 //   P = 2  two f16 planes, hi + lo = 22 bits of a value kept within f16's range by a power of two:
 //          hi hi + hi lo + lo hi, three products for f32 accuracy (the Newton-Schulz iteration)
 //   P = 3  three bf16 planes, hi + mid + lo = all 24 bits of an f32: the six products of the first two
-//          orders (f32 operands of any size; what is left out is below 2^-24 of a product)
+//          orders (f32 operands of any size; what is left out is below 2^-24 of a product, and of values below 2^-110 what
+//          lies under bf16's smallest step, 2^-133)
 //
 // Bound by the matrix instructions and, there, by the card's power: a Gram product has them busy 68 % of the time at
 // 1.63 GHz, a step 42 % at 1.93.  Reached, whole products with their epilogues: P = 1 275 GFLOP (8192 x 8192 -> 2048) in 250

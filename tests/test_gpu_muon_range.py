@@ -104,3 +104,51 @@ def test_muon_step_far_below_eps(shape):
     ops.muon_step(p, g.reshape(-1).cuda(), m, v, segs, hyper)
     assert torch.equal(m.cpu(), 0.25 * g.reshape(-1))  # exact: powers of two
     check_ns(p.view(shape) * -2.0, 0.25 * g, "f32", f"{shape}")
+
+
+TILES = [  # matrices; tiles of the Gram product, the polynomial and the step
+    ((1, 2049, 2100), ["128x128", "128x128", "128x256"]), ((1, 2100, 2049), ["128x128", "128x128", "128x256"]),
+    ((2, 2048, 8192), ["256x256 split", "256x256 split", "128x256"]), ((1, 4101, 4097), ["256x256 split", "256x256 split", "128x256"]),
+    ((2, 2049, 4099), ["128x128 split", "128x128", "128x256"]), ((1, 5500, 5601), ["256x256", "256x256", "128x256"]),
+    ((1, 3005, 3001), ["256x256 split", "256x256 split", "128x128"]), ((1, 600, 5000), ["64x64 split", "64x64", "128x128"]),
+]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,tiles", TILES)
+def test_the_tiles_of_large_matrices(shape, tiles, dt):
+    """Symmetric and step tiles of every size, wide and tall (a tall result is turned on its way out)."""
+    from test_gpu_linear_tiles import launches
+    from cgan3d_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    g = torch.randn(*shape, generator=gen, device="cuda") * torch.exp(0.5 * torch.randn(*shape[:2], 1, generator=gen, device="cuda"))
+    g = (g * 1e-3).to(DT[dt])
+    out, ws = torch.empty_like(g), torch.empty(1 << 30, dtype=torch.uint8, device="cuda")
+    got = launches(lambda: ops.orthogonalize(g, steps=2, out=out, ws=ws))
+    assert got == tiles + tiles, f"{shape}: {got}"
+    five = ops.orthogonalize(g, ws=ws)
+    for i in range(shape[0]):
+        check_ns(out[i], g[i], dt, f"{shape} matrix {i}", steps=2)
+        check_ns(five[i], g[i], dt, f"{shape} matrix {i}, five steps")
+
+
+@pytest.mark.parametrize("shapes", [[(2049, 2100), (2100, 2049)], [(600, 5000), (3001, 3005), (70, 90)]])
+def test_muon_step_of_large_matrices(shapes):
+    """The parameters' update through the large tiles' last step."""
+    from cgan3d_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    mats, n = [], 0
+    for r, c in shapes:
+        mats.append((n, r, c, 1.0))
+        n += r * c
+    segs = ops.MuonSegments(n, mats, [])
+    g, p = 1e-3 * torch.randn(n, generator=gen, device="cuda"), torch.randn(n, generator=gen, device="cuda")
+    before, m, v = p.clone(), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    hyper = torch.tensor([0.5, 0.75, 0.125, 0.0, 0.0, 0.0, 0.0, 0.9, 0.999, 1e-8], device="cuda")
+    ops.muon_step(p, g, m, v, segs, hyper)
+    for at, r, c, _ in mats:
+        u = 0.25 * g[at:at + r * c].view(r, c)
+        x, tol = ns64(u)
+        want = before[at:at + r * c].view(r, c).double() * (1 - 0.5 * 0.125) - 0.5 * x
+        err = float((p[at:at + r * c].view(r, c).double() - want).norm())
+        assert err <= 0.5 * tol + 4 * U * float(want.norm()), f"{(r, c)}: off by {err:.3e}"
