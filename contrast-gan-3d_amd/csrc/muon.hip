@@ -517,7 +517,7 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, int shift, cons
 // 244 / 182 / 186, four of these 288 / 250 / 399.  G's planes are scaled by the power of two of the slab's largest value,
 // and the norm is the trace of the partial Gram matrices, in 64 bits: no pass of its own.  Vectors' Adam rides on
 // launch 0.
-constexpr int kSlabMats = 28, kMaxSlabs = 64, kBatch = 16, kCols = 256, kSlab = 64 * kCols;
+constexpr int kMaxSlabs = 64, kBatch = 16, kCols = 256, kSlab = 64 * kCols;
 constexpr int kSlabThreads = 4 * kCols, kSlabWaves = kSlabThreads / 64;  // a wave: 16 columns, and one tile of a 64 x 64 matrix
 static_assert(kSlabWaves == 16, "a wave for each tile of the Gram matrix");
 
@@ -535,6 +535,8 @@ struct SlabMat {
   float* part;      // [2][nslab][64 * 64]
   float* expo;      // [nslab]: G = planes * 2^expo; [nslab] X's start exponent, a copy for each block
 };
+// matrices and vectors of a launch: as many as its arguments hold (4096 bytes, 320 of them for the rest), and a lane each
+constexpr int kSlabMats = std::min<int>((4096 - 320) / (sizeof(SlabMat) + sizeof(int)), 64);
 struct SlabList {
   int n, tick;  // tick: the last launch advances the step counter
   int start[kSlabMats + 1];
