@@ -39,8 +39,8 @@ long long mat_ws_bytes(long long I, long long J, long long K) {
   return s > 1 ? (long long)s * I * J * 4 : 0;
 }
 
-template <typename T, bool AT, bool BT>
-void mat_run_t(MatArgs p, void* ws, hipStream_t st) {
+template <bool AT, bool BT>
+void mat_run(MatArgs p, void* ws, hipStream_t st) {
   if (p.I == 0 || p.J == 0) return;
   int splits = mat_splits(p.I, p.J, p.K);
   const long long steps = (p.K + 31) / 32;
@@ -49,17 +49,18 @@ void mat_run_t(MatArgs p, void* ws, hipStream_t st) {
   p.part = splits > 1 ? static_cast<float*>(ws) : nullptr;
   const long long ti = (p.I + kTile - 1) / kTile;
   p.tj = (p.J + kTile - 1) / kTile;
-  launch(mat_kernel<T, AT, BT, kTile, kTile>, dim3((unsigned)(ti * p.tj), splits), dim3(256), 0, st, p);
+  launch(mat_kernel<AT, BT, kTile, kTile>, dim3((unsigned)(ti * p.tj), splits), dim3(256), 0, st, p);
   if (splits > 1) {
     const long long blocks = std::min((p.I * p.J + 255) / 256, 8192LL);
-    launch(mat_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, p, splits);
+    launch(mat_join_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, p, splits);
   }
 }
-template <bool AT, bool BT>
-void mat_run(int dt, const MatArgs& p, void* ws, hipStream_t st) {
-  if (dt == CGAN3D_DT_F32) mat_run_t<float, AT, BT>(p, ws, st);
-  else if (dt == CGAN3D_DT_BF16) mat_run_t<bf16_t, AT, BT>(p, ws, st);
-  else mat_run_t<f16_t, AT, BT>(p, ws, st);
+// an empty sum: the epilogue of zeros
+void mat_zero(int dt, const MatArgs& p, hipStream_t st) {
+  const dim3 grid((unsigned)std::min((p.I * p.J + 255) / 256, 8192LL));
+  if (dt == CGAN3D_DT_F32) launch(mat_join_kernel<float>, grid, dim3(256), 0, st, p, 0);
+  else if (dt == CGAN3D_DT_BF16) launch(mat_join_kernel<bf16_t>, grid, dim3(256), 0, st, p, 0);
+  else launch(mat_join_kernel<f16_t>, grid, dim3(256), 0, st, p, 0);
 }
 
 // --- products on planes ---
@@ -283,7 +284,6 @@ bool f32_planes(const Operand& a, const Operand& b, long long I, long long J, lo
   return m > 15e-6 && m > planes_seconds(a, b, I, J, K);
 }
 Route mat_route(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
-  if (K == 0 || K > 1 << 30 || I > 1 << 30 || J > 1 << 30) return ROUTE_MAT;
   return dt != CGAN3D_DT_F32 || a.planes || f32_planes(a, b, I, J, K) ? ROUTE_PLANES : ROUTE_MAT;
 }
 
@@ -315,7 +315,7 @@ bool launchable(int dt, long long I, long long J, long long K) {
 }
 // workspace of one product: both operands' planes, then partial sums
 long long product_bytes(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
-  if (I == 0 || J == 0) return 0;
+  if (I == 0 || J == 0 || K == 0) return 0;
   if (mat_route(dt, a, b, I, J, K) == ROUTE_MAT) return mat_ws_bytes(I, J, K);
   return operand_bytes(dt, a) + operand_bytes(dt, b) + pick_for(dt, I, J, K).part_floats * 4;
 }
@@ -364,10 +364,10 @@ void planes_run(int dt, Operand a, Operand b, const MatArgs& m, void* ws, hipStr
 // C = A B^T with m's epilogue; m.a / m.b: the operands as the tensors they are
 void product(int dt, const Operand& a, const Operand& b, const MatArgs& m, void* ws, hipStream_t st) {
   if (m.I == 0 || m.J == 0) return;
-  if (mat_route(dt, a, b, m.I, m.J, m.K) == ROUTE_MAT) {
-    if (a.strided) mat_run<true, true>(dt, m, ws, st);
-    else if (b.strided) mat_run<false, true>(dt, m, ws, st);
-    else mat_run<false, false>(dt, m, ws, st);
+  if (m.K == 0) {
+    mat_zero(dt, m, st);
+  } else if (mat_route(dt, a, b, m.I, m.J, m.K) == ROUTE_MAT) {
+    mat_f32(a.strided, b.strided, m, ws, st);
   } else if (dt == CGAN3D_DT_F32) {
     planes_run<float, bf16_t, 3>(dt, a, b, m, ws, st);
   } else if (dt == CGAN3D_DT_BF16) {
@@ -477,7 +477,8 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int n, T
 // of 32 values each in flight; 16 waves where each has U steps to do, else 4.  Measured, us, KW = 4 / 16, 8 rows: bf16
 // 4096 -> 4096 11.1 / 9.5 (3.5 TB/s), 2048 -> 4096 6.3 / 8.4; f32 4096 -> 4096 18.9 / 16.7, 2048 -> 4096 11.4 / 9.7,
 // 1024 -> 8192 10.1 / 15.7.  With more than 32 columns a CU, four waves from ten rows on (f32 16 x 8192 -> 16384 126 / 133,
-// 10 x 110 / 118, 8 x 8192 -> 32768 231 / 219, 3 x 230 / 204).  As products of tiles (planes, mat_kernel) these five take 12.9, 9.8, 28, 17.5 and 18.5.
+// 10 x 110 / 118, 8 x 8192 -> 32768 231 / 219, 3 x 230 / 204).  As products of tiles (planes, mat_kernel) the first five
+// take 12.9, 9.8, 28, 17.5 and 18.5.
 // 16-bit weights with more columns than 32 a CU are the planes' (16 rows, 4096 -> 16384: 40 here, 33 there; 2048 ->
 // 16384: 22 and 18), f32 ones are not (68 and 96).
 constexpr int kSkinnyRows = 16;
@@ -1061,9 +1062,9 @@ bool meet(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
 
 long long mat_f32_ws_bytes(long long I, long long J, long long K) { return mat_ws_bytes(I, J, K); }
 void mat_f32(bool at, bool bt, const MatArgs& p, void* ws, hipStream_t st) {
-  if (at) mat_run_t<float, true, true>(p, ws, st);
-  else if (bt) mat_run_t<float, false, true>(p, ws, st);
-  else mat_run_t<float, false, false>(p, ws, st);
+  if (at) mat_run<true, true>(p, ws, st);
+  else if (bt) mat_run<false, true>(p, ws, st);
+  else mat_run<false, false>(p, ws, st);
 }
 
 }  // namespace cg

@@ -1,5 +1,5 @@
 // Matrix products C[I, J] = sum_t A(i, t) * B(j, t) of the linear block (linear.hip) and the
-// Newton-Schulz iteration (muon.hip): the tile kernel that takes any size, stride and alignment.
+// Newton-Schulz iteration (muon.hip) on f32 instructions: the tile kernel that takes any size, stride and alignment.
 //
 // Either operand is "t-contiguous" (element (i, t) at i * ld + t: a row-major matrix whose columns are
 // summed) or "t-strided" (element (i, t) at t * ld + i: its rows are summed), so the forward product,
@@ -228,9 +228,10 @@ __device__ __forceinline__ void mat_store(const MatEpi& e, long long J, long lon
 // One BM x BN tile, 4 waves as 2 x 2, BK t-values a step: global -> registers -> LDS (rows padded by
 // 16 bytes), the next step's loads in flight under this step's products.  Bound by the f32 matrix instructions where it
 // is used at all: 2048 x 1024 -> 4096 in 184 us, 4096 x 4096 -> 4096 in 1356, 93 and 101 TFLOP/s of 154 that a library
-// product of 8192 reaches (what is larger goes to planes); K = 0 of any type, and the iteration's fallback.
-template <typename T, bool AT, bool BT, int BM, int BN>
+// product of 8192 reaches (what is larger goes to planes), and the iteration's fallback.
+template <bool AT, bool BT, int BM, int BN>
 __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
+  typedef float T;
   constexpr int BK = 32, V = MatT<T>::VEC, LD = BK + MatT<T>::PAD;
   constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
   constexpr int NA = BM * BK / V / 256, NB = BN * BK / V / 256;  // 16-byte chunks per thread
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(256) void mat_kernel(MatArgs p) {
   }
 }
 
-// the splits' partial sums, added in their order, and the epilogue
+// the splits' partial sums, added in their order (none: an empty sum), and the epilogue
 template <typename T>
 __global__ __launch_bounds__(256) void mat_join_kernel(MatArgs p, int splits) {
   const long long total = p.I * p.J;

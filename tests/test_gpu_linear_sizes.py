@@ -56,3 +56,28 @@ def test_grids_beyond_one_axis():
     dy, db = whole(g, 2, n).float(), torch.full((n,), 7.0, device="cuda")
     ops.linear_backward(dy, torch.empty(2, 0, device="cuda"), torch.empty(n, 0, device="cuda"), dbias=db)
     assert torch.equal(db, dy[0] + dy[1])
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_empty_sums_of_many_values(dt):
+    """k, n or rows of zero beside sides of any route: the epilogue of zeros, and gradients of zeros."""
+    from cgan3d_amd import _lib as L
+    from cgan3d_amd import ops
+    t = DT[dt]
+    for rows, n in ((100, 70), (700, 33), (5000, 300)):
+        b, r = torch.randn(n, device="cuda").to(t), torch.randn(rows, n, device="cuda").to(t)
+        y = torch.full((rows, n), 7.0, dtype=t, device="cuda")
+        pre = torch.full((rows, n), 7.0, dtype=ops.linear_preact_dtype(t), device="cuda")
+        ops.linear(torch.empty(rows, 0, dtype=t, device="cuda"), torch.empty(n, 0, dtype=t, device="cuda"), y, bias=b,
+                   residual=r, act=L.ACT_RELU, preact=pre)
+        want = b.double().clamp_min(0) + r.double()
+        low = torch.finfo(t).smallest_normal if dt == "f16" else 0
+        assert ((y.double() - want).abs() <= torch.finfo(t).eps / 2 * 1.01 * want.abs() + low).all()
+        assert ((pre.double() - b.double()).abs() <= 2.0 ** -11 * b.double().abs() + 2.0 ** -25).all()
+        dx = torch.full((rows, n), 7.0, dtype=t, device="cuda")
+        ops.linear_backward(torch.empty(rows, 0, dtype=t, device="cuda"), r, torch.empty(0, n, dtype=t, device="cuda"), dx=dx)
+        assert not dx.any()
+        dw, db = torch.full((n, rows), 7.0, dtype=t, device="cuda"), torch.full((n,), 7.0, dtype=t, device="cuda")
+        ops.linear_backward(torch.empty(0, n, dtype=t, device="cuda"), torch.empty(0, rows, dtype=t, device="cuda"),
+                            torch.empty(n, rows, dtype=t, device="cuda"), dw=dw, dbias=db)
+        assert not dw.any() and not db.any()
