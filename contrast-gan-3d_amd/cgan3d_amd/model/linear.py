@@ -11,6 +11,7 @@ import math
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 
 from .. import _lib as L
 from .. import ops
@@ -45,6 +46,9 @@ def _rows(t: Tensor, cols: int) -> Tensor:
     return t
 
 
+_autocasts = torch.is_autocast_enabled
+
+
 def _autocast(*tensors):
     """The operands in autocast's dtype (float64 ones are left as they are, as torch leaves them)."""
     dt = torch.get_autocast_dtype("cuda")
@@ -60,7 +64,7 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     are (the residual too: bias, activation and sum stay in 32 bits, the result is rounded to that dtype once).
     Differentiable once, in reverse mode.  A HIP graph that captures the backward pass must be the only autograd graph alive
     on its leaves (torch's own rule: their gradient accumulators belong to the stream they were made on)."""
-    if torch.is_autocast_enabled("cuda"):
+    if _autocasts("cuda"):
         x, weight, bias, residual = _autocast(x, weight, bias, residual)
     xs, ws = x.shape, weight.shape
     if len(ws) != 2 or not xs or xs[-1] != ws[1]:
@@ -69,7 +73,8 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
                                  or residual.shape[:-1] != xs[:-1]):
         raise ValueError(f"fused_linear: residual {tuple(residual.shape)} is not of the result's shape "
                          f"{(*xs[:-1], ws[0])}")
-    ops._no_tangents("fused_linear", x, weight, bias, residual)
+    if forward_ad._current_level >= 0:
+        ops._no_tangents("fused_linear", x, weight, bias, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _LinearFn.apply(x, weight, bias, residual, act, slope)
@@ -89,10 +94,6 @@ def _forward(x, x2, w2, bias, residual, act, slope, preact):
     return y, args
 
 
-def _layout(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype)
-
-
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, slope):
@@ -103,7 +104,7 @@ class _LinearFn(torch.autograd.Function):
         y, ctx.args = _forward(x, x2, w2, bias, residual, act, slope, preact)
         ctx.shape, ctx.act, ctx.slope = x.shape, act, slope
         ctx.bias_shape = None if bias is None else bias.shape
-        ctx.layout = _layout(x2), _layout(w2), _layout(preact)
+        ctx.strides = x2.stride(), w2.stride()
         ctx.save_for_backward(x2, w2, preact)
         return y
 
@@ -111,7 +112,8 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, grad_out):
         if torch.is_grad_enabled():
             raise NotImplementedError("double backward through the HIP linear block is not implemented")
-        ops._no_tangents("fused_linear's backward pass", grad_out)
+        if forward_ad._current_level >= 0:
+            ops._no_tangents("fused_linear's backward pass", grad_out)
         x2, w2, preact = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = None
@@ -123,11 +125,13 @@ class _LinearFn(torch.autograd.Function):
         if nx or nw or nb:
             a, dy = ctx.args, _rows(grad_out, w2.shape[0])
             here = (x2.data_ptr() or None, w2.data_ptr() or None, None if preact is None else preact.data_ptr() or None)
-            if here == (a.x, a.w, a.preact) and (_layout(x2), _layout(w2), _layout(preact)) == ctx.layout:
+            if (here == (a.x, a.w, a.preact) and (x2.stride(), w2.stride()) == ctx.strides
+                    and (preact is None or preact.is_contiguous())):
                 ops._linear_backward_of(a, dy, x2, dx, dw, db)
-            else:  # hooks on saved tensors gave others back: elsewhere, or where the freed ones were, but dense
-                ops.linear_backward(dy, x2, w2, dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db,
-                                    ctx.act, ctx.slope, preact)
+            else:  # hooks on saved tensors gave others back: elsewhere, or where the freed ones were with other strides
+                ops.linear_backward(dy, _rows(x2, w2.shape[1]), _rows(w2, w2.shape[1]),
+                                    dx if dx is None or dx.dim() == 2 else dx.view(x2.shape), dw, db, ctx.act, ctx.slope,
+                                    preact if preact is None else preact.contiguous())
         if nb and db.shape != ctx.bias_shape:  # n values in any shape
             db = db.view(ctx.bias_shape)
         return dx, dw, db, grad_out if nr else None, None, None

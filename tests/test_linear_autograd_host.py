@@ -168,3 +168,21 @@ def test_bias_of_any_shape_gets_its_gradient(dry, shape):
     b = torch.randn(shape).requires_grad_(True)
     y = fused_linear(torch.randn(6, 8), torch.randn(5, 8), b)
     assert torch.autograd.grad(y, b, torch.ones(6, 5))[0].shape == b.shape
+
+
+def test_saved_tensors_that_come_back_transposed(calls):
+    """Any strides are the hook's right: what the kernels cannot read is copied."""
+    from cgan3d_amd import _lib as L
+    from cgan3d_amd.model.linear import fused_linear
+    x, w = torch.randn(6, 8).requires_grad_(True), torch.randn(5, 8).requires_grad_(True)
+    back = []
+
+    def unpack(t):
+        back.append(t.detach().t().contiguous().t())
+        return back[-1]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = fused_linear(x, w, act=L.ACT_GELU)
+    torch.autograd.grad(y, (x, w), torch.ones(6, 5))
+    bwd = calls[1][1]
+    assert (bwd.ldx, bwd.ldw) == (8, 8) and len(back) == 3
+    assert not {bwd.x, bwd.w, bwd.preact} & {t.data_ptr() for t in back}
