@@ -1475,12 +1475,15 @@ def _flat(t, n, who, name, dtype, device):
     raise ValueError(f"{who} {name}: {n} contiguous values needed, got shape {tuple(t.shape)}, strides {t.stride()}")
 
 
+_tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
+
+
 def _untraced(what):
     """Refuses tracers: a launch is invisible to them, and the traced program would return memory that nothing has
     written.  Other dispatch modes (counters, loggers) see an ordinary call."""
-    if torch._C._get_tracing_state() is not None:
+    if _tracing_state() is not None:
         raise NotImplementedError(f"{what}: torch.jit.trace cannot record HIP launches")
-    if torch._C._len_torch_dispatch_stack():
+    if _dispatch_modes():
         key = torch._C._TorchDispatchModeKey
         for k in (key.PROXY, key.FAKE, key.FUNCTIONAL):
             if torch._C._get_dispatch_mode(k) is not None:
