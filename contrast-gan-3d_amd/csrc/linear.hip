@@ -14,8 +14,8 @@
 //                           with few rows: rows_fwd_takes, rows_bwd_takes)
 //   16-bit tensors         plane_kernel (planes.h) on the tensors themselves; an operand whose rows are not
 //                          whole aligned 16-byte chunks is copied once into rows that are
-//   f32 tensors            plane_kernel on three bf16 planes where the product is large enough to pay for
-//                          the splitting, else mat_kernel (mat.h: f32 instructions, any layout)
+//   f32 tensors            plane_kernel on three bf16 planes where that is expected to be faster (f32_planes), else
+//                          mat_kernel (mat.h: f32 instructions, any layout)
 #include <climits>
 
 #include "planes.h"
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(const T* __restrict__ x, 
 // Backward: one pass over dy, z and x writes dx and keeps dW and db in registers; a block takes tiles of 64 rows in
 // turn and leaves one partial sum of each.  dz is used as its own type would hold it, for db before that.  dz and x go
 // through LDS in both orders, since one product sums over columns and the other over rows: that, not memory, bounds
-// the 16-bit form (1048576 x 64 -> 64 with SiLU: f32 347 us, 3.1 TB/s, bf16 273 us, 2.0 TB/s).
+// the 16-bit form (1048576 x 64 -> 64 with SiLU: f32 344 us, 3.1 TB/s, bf16 235 us, 2.3 TB/s).
 constexpr int kRowsBlocks = 512;
 template <typename T, int NT, int KT>
 __global__ __launch_bounds__(256) void rows_bwd_kernel(const T* __restrict__ dy, long long lddy,
@@ -850,8 +850,9 @@ template <typename T> void rows_bwd_run(const cgan3d_linear_args* a, void* ws, h
 
 // --- dz = dy * act'(z), and its column sums ---
 // CT threads of a block along the columns (V values each), the rest along the rows; column sums in 32 bits, of dz
-// before its rounding, into part [blockIdx.y][n].  dz goes to rows of ldz values whose padding is zeroed:
-// as it is, or (PL3) split into three planes.  Bound by memory: 8192 x 8192 bf16 with GELU 90 us, 4.5 TB/s.
+// before its rounding, into part [blockIdx.y][n].  dz goes to rows of ldz values whose padding is zeroed: in the tensors'
+// type, or (PL3) split into three planes.  Rounding a 16-bit dz once lets both products read it straight into the
+// matrix instructions; a second plane of what is lost would double them (error of a large bf16 step 0.0023, without 0.0017).  Bound by memory: 8192 x 8192 bf16 with GELU 90 us, 4.5 TB/s.
 template <typename T, bool PL3>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, long long lddy,
                                                        const typename PreT<T>::type* __restrict__ pre, void* __restrict__ dzv,

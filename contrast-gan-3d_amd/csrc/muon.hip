@@ -512,7 +512,7 @@ void plane_iterate(const MatList& l, int n, char* ws, int steps, int shift, cons
 // so five steps are six launches for up to kSlabMats matrices of any shapes, where the general products take
 // seventeen and joins.  Bound by latency: a launch of 64 x 1728 is ~7.5 us, of which a fourth is the trip to the
 // arguments, and about as much each the Gram partials, the step and the Gram product.  Measured, us, here / on planes:
-// 16 x 343 50 / 69, 64 x 1728 55 / 98, 64 x 16384 103 / 139, 64 x 65536 182 / 213, four of these 250 / 417; a
+// 16 x 343 49 / 68, 64 x 1728 53 / 98, 64 x 16384 103 / 139, 64 x 65536 182 / 213, four of these 250 / 417; a
 // very long single one loses (16 x 200000 381 / 332).  kMaxSlabs 32 / 64 / 128: 64 x 16384 99 / 103 / 103, 64 x 65536
 // 244 / 182 / 186, four of these 288 / 250 / 399.  G's planes are scaled by the power of two of the slab's largest value,
 // and the norm is the trace of the partial Gram matrices, in 64 bits: no pass of its own.  Vectors' Adam rides on

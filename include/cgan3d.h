@@ -630,7 +630,8 @@ int cgan3d_linear_bwd(const cgan3d_linear_args* args, void* ws, int64_t ws_bytes
  * Newton-Schulz iteration on each of n matrices (host list): X = g / (|g|_F + eps), then `steps` times
  * X = a X + (b A + c A A) X with A = X X^T (a tall g by its transpose); out = X, of g's dtype.
  * coefficients (host): a, b, c.  out may be g itself.  The norm is summed in f64, the iteration keeps f32
- * accuracy whatever the dtype.  Sides of up to 2^30, zero included. */
+ * accuracy whatever the dtype and the matrix's size.  Sides of up to 2^30, zero included.  Matrices of one call must
+ * not overlap each other. */
 typedef struct cgan3d_ortho_mat {
   const void* g;
   void* out;
