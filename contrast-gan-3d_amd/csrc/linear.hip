@@ -280,7 +280,7 @@ double planes_seconds(const Operand& a, const Operand& b, long long I, long long
   return 0.7 * plane_pick<3, false>(&s, 1).seconds + values * 10 / 8e12 + 4. * I * J / 1.95e12 + 15e-6;
 }
 bool f32_planes(const Operand& a, const Operand& b, long long I, long long J, long long K) {
-  const double m = mat_seconds(a, b, I, J, K);
+  const double m = mat_seconds(a, b, I, J, K);  // planes take 15 us at least: no estimate needed below that
   return m > 15e-6 && m > planes_seconds(a, b, I, J, K);
 }
 Route mat_route(int dt, const Operand& a, const Operand& b, long long I, long long J, long long K) {
@@ -852,7 +852,8 @@ template <typename T> void rows_bwd_run(const cgan3d_linear_args* a, void* ws, h
 // CT threads of a block along the columns (V values each), the rest along the rows; column sums in 32 bits, of dz
 // before its rounding, into part [blockIdx.y][n].  dz goes to rows of ldz values whose padding is zeroed: in the tensors'
 // type, or (PL3) split into three planes.  Rounding a 16-bit dz once lets both products read it straight into the
-// matrix instructions; a second plane of what is lost would double them (error of a large bf16 step 0.0023, without 0.0017).  Bound by memory: 8192 x 8192 bf16 with GELU 90 us, 4.5 TB/s.
+// matrix instructions; a second plane of what is lost would double them (error of a large bf16 step 0.0023, without
+// 0.0017).  Bound by memory: 8192 x 8192 bf16 with GELU 90 us, 4.5 TB/s.
 template <typename T, bool PL3>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, long long lddy,
                                                        const typename PreT<T>::type* __restrict__ pre, void* __restrict__ dzv,
