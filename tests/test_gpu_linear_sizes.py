@@ -81,3 +81,62 @@ def test_empty_sums_of_many_values(dt):
         ops.linear_backward(torch.empty(0, n, dtype=t, device="cuda"), torch.empty(0, rows, dtype=t, device="cuda"),
                             torch.empty(n, rows, dtype=t, device="cuda"), dw=dw, dbias=db)
         assert not dw.any() and not db.any()
+
+
+@pytest.fixture
+def guarded(monkeypatch):
+    """Every workspace is exactly as large as was asked for, with a pattern behind it."""
+    from cgan3d_amd import ops
+    held = []
+
+    def workspace(ws, need, what, device):
+        assert need >= 0
+        buf = torch.full((need + 8192,), 0xA5, dtype=torch.uint8, device=device)
+        held.append((what, need, buf))
+        return buf[:need]
+    monkeypatch.setattr(ops, "_workspace", workspace)
+
+    def check(what):
+        torch.cuda.synchronize()
+        for name, need, buf in held:
+            assert (buf[need:] == 0xA5).all(), f"{name} wrote behind its {need} bytes: {what}"
+        held.clear()
+    return check
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_workspaces_are_large_enough(guarded, dt):
+    from cgan3d_amd import _lib as L
+    from cgan3d_amd.model.linear import fused_linear
+    t = DT[dt]
+    for rows, k, n in ((3, 64, 48), (20, 33, 50), (500, 64, 64), (129, 129, 257), (777, 1001, 515), (64, 16384, 64), (1200, 3000, 1200),
+                       (4001, 203, 4003), (520, 1000, 5000), (70, 300, 9001), (100, 0, 70), (70000, 100, 70)):
+        for act in (L.ACT_NONE, L.ACT_SILU):
+            leaves = [torch.randn(*s, device="cuda").to(t).requires_grad_(True) for s in ((rows, k), (n, k), (n,))]
+            y = fused_linear(*leaves, act=act)
+            dy = torch.randn(rows, n, device="cuda").to(t)
+            torch.autograd.grad(y, leaves, dy, retain_graph=True)
+            for leaf in leaves:
+                torch.autograd.grad(y, leaf, dy, retain_graph=True)
+            guarded(f"{rows}x{k}->{n} {act}")
+
+
+def test_workspaces_of_the_iteration_are_large_enough(guarded):
+    from cgan3d_amd import ops
+    for shape in ((1, 1, 7), (3, 16, 343), (40, 64, 300), (1, 64, 70000), (14, 100, 72), (3, 1001, 333), (1, 600, 5000), (1, 2049, 2100)):
+        g = torch.randn(*shape, device="cuda")
+        for kw in ({}, dict(steps=0), dict(steps=1, coefficients=(70.0, 0.0, -61.0))):
+            ops.orthogonalize(g, **kw)
+            guarded(f"{shape} {kw}")
+    mats, vecs, n = [], [], 0
+    for r, c in [(16, 343), (64, 1728), (1, 5488), (100, 130), (2100, 300)] * 9:
+        mats.append((n, r, c, 1.0))
+        vecs.append((n + r * c, 5))
+        n += r * c + 5
+    segs = ops.MuonSegments(n, mats, vecs)
+    p, g, m, v = (torch.randn(n, device="cuda").abs() for _ in range(4))
+    hyper = torch.tensor([0.5, 0.75, 0.0, 1.0, 0.0, 0.0, 0.1, 0.9, 0.999, 1e-8], device="cuda")
+    for kw in ({}, dict(steps=2, coefficients=(70.0, 0.0, -61.0))):
+        ops.muon_step(p, g, m, v, segs, hyper, **kw)
+        guarded(f"muon {kw}")
+    assert float(hyper[4]) == 2.0

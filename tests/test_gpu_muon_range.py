@@ -152,3 +152,21 @@ def test_muon_step_of_large_matrices(shapes):
         want = before[at:at + r * c].view(r, c).double() * (1 - 0.5 * 0.125) - 0.5 * x
         err = float((p[at:at + r * c].view(r, c).double() - want).norm())
         assert err <= 0.5 * tol + 4 * U * float(want.norm()), f"{(r, c)}: off by {err:.3e}"
+
+
+@pytest.mark.parametrize("shape", [(2, 40, 600), (2, 100, 300)])
+def test_replayed_calls_follow_the_size_of_their_input(shape):
+    """A captured call keeps no exponent of the matrices it was captured on."""
+    from cgan3d_amd import ops
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(13)).cuda()
+    inputs = [g, g * 1e-14, g * 1e-3, g * 1e-9, g]
+    wants = [ops.orthogonalize(v) for v in inputs]
+    static, out = g.clone(), torch.empty_like(g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.orthogonalize(static, out=out)
+    for v, want in zip(inputs, wants):
+        static.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
